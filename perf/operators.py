@@ -138,10 +138,10 @@ def _rows(case, shape, g):
 
 def _quantise(x, kind):
     """Rows [..., D] fp16 -> (codes, scale [...] fp32)."""
-    top = MAXIMA[kind]
     xf = x.float()
     amax = xf.abs().amax(-1)
-    inv = torch.where(amax > 0, top / amax, torch.zeros_like(amax))
+    top = torch.full_like(amax, MAXIMA[kind])  # a tensor: torch divides by a number through its reciprocal
+    inv = torch.where(amax > 0, top / amax, 0.0)
     y = xf * inv[..., None]
     codes = y.round().to(torch.int8) if kind == "int8" else y.to(torch.float8_e4m3fn)
     return codes, amax / top
