@@ -28,7 +28,7 @@ def __getattr__(name):
     # imports without the HIP library.
     import importlib
 
-    mods = ("quantization", "attention", "cache", "batched", "calibrate", "kernels", "workloads")
+    mods = ("quantization", "attention", "cache", "batched", "paged", "calibrate", "kernels", "workloads")
     if name in mods or name.startswith("_"):
         return importlib.import_module(f".{name}", __name__)
     for mod in mods:

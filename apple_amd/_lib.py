@@ -86,6 +86,12 @@ class LinearParams(C.Structure):
                 ("inv_freq", vp), ("cos", vp), ("sin", vp)]
 
 
+class Paged(C.Structure):
+    _fields_ = [("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp), ("bounds", vp), ("table", vp), ("lens", vp),
+                ("page_stride", i64), ("head_stride", i64), ("table_stride", i64), ("pages", i32), ("page_size", i32),
+                ("kv_heads", i32), ("head_dim", i32), ("type", i32), ("batch", i32), ("table_width", i32)]
+
+
 class EncodeJob(C.Structure):
     _fields_ = [("x", vp), ("n", i64), ("ldx", i64), ("pq_cb", vp), ("rvq_cb", vp), ("out", Codes)]
 
@@ -131,6 +137,12 @@ SIGNATURES = {
     "rfsn_fused_workspace_bytes": (sz, [C.POINTER(FusedParams)]),
     "rfsn_fused_decode_attention": (i32, [C.POINTER(FusedParams), vp]),
     "rfsn_fused_decode_attention_noalloc": (i32, [C.POINTER(FusedParams), vp]),
+    "rfsn_paged_append": (i32, [C.POINTER(Paged), vp, vp, i64, i64, i64, vp, vp]),
+    "rfsn_paged_read": (i32, [C.POINTER(Paged), vp, i64, vp, vp, i32, vp]),
+    "rfsn_page_select_workspace_bytes": (sz, [C.POINTER(Paged)]),
+    "rfsn_page_select": (i32, [C.POINTER(Paged), vp, i32, i32, i32, i32, vp, vp, sz, vp]),
+    "rfsn_paged_attention_workspace_bytes": (sz, [C.POINTER(Paged), i32, i32]),
+    "rfsn_paged_attention": (i32, [C.POINTER(Paged), vp, i32, f32, vp, i32, vp, vp, sz, vp]),
     "rfsn_kmeans_workspace_bytes": (sz, [i32, i32, i32]),
     "rfsn_kmeans_update": (i32, [vp, i64, i32, i64, vp, i32, i32, vp, vp, sz, vp]),
     "rfsn_host_alloc": (i32, [sz, C.POINTER(vp)]),

@@ -1,0 +1,71 @@
+// What the paged KV cache's kernels share (paged.hip, paged_attention.hip).
+#pragma once
+
+#include "rfsn_common.h"
+
+namespace rfsn {
+
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef float float8v __attribute__((ext_vector_type(8)));
+typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+typedef uint32_t uint4w __attribute__((ext_vector_type(4)));
+
+// Checks every call makes of the pool, the table and the batch; 0 or a status.
+int paged_check(const rfsn_paged* p, const char* what);
+
+inline int paged_shift(const rfsn_paged& p) { return __builtin_ctz((unsigned)p.page_size); }
+
+template <int TYPE>
+struct PageElem {
+  typedef uint16_t type;
+};
+template <>
+struct PageElem<RFSN_PAGE_INT8> {
+  typedef uint8_t type;
+};
+template <>
+struct PageElem<RFSN_PAGE_E4M3> {
+  typedef uint8_t type;
+};
+
+// 8 consecutive stored values of a row, without the row's scale: exact in fp32.
+template <int TYPE>
+__device__ __forceinline__ float8v load_page8(const void* base, int64_t off) {
+  float8v f;
+  if constexpr (TYPE == RFSN_PAGE_FP16) {
+    const half8v h = *reinterpret_cast<const half8v*>((const uint16_t*)base + off);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = (float)h[e];
+  } else {
+    const uint2v c = *reinterpret_cast<const uint2v*>((const uint8_t*)base + off);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      if constexpr (TYPE == RFSN_PAGE_INT8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[4 * w + e] = (float)(int8_t)(c[w] >> (8 * e));
+      } else {
+        f[4 * w + 0] = __builtin_amdgcn_cvt_f32_fp8((int)c[w], 0);
+        f[4 * w + 1] = __builtin_amdgcn_cvt_f32_fp8((int)c[w], 1);
+        f[4 * w + 2] = __builtin_amdgcn_cvt_f32_fp8((int)c[w], 2);
+        f[4 * w + 3] = __builtin_amdgcn_cvt_f32_fp8((int)c[w], 3);
+      }
+    }
+  }
+  return f;
+}
+
+// Tokens of sequence b that the table can hold.
+__device__ __forceinline__ int paged_len(const rfsn_paged& p, int shift, int b) {
+  const int64_t most = (int64_t)p.table_width << shift;
+  const int n = p.lens[b];
+  return n < 0 ? 0 : (int)(n < most ? n : most);
+}
+
+// Page of ordinal ord of sequence b, or -1.
+__device__ __forceinline__ int paged_page(const rfsn_paged& p, int b, int64_t ord) {
+  if (ord < 0 || ord >= p.table_width) return -1;
+  const int n = p.table[(int64_t)b * p.table_stride + ord];
+  return n >= 0 && n < p.pages ? n : -1;
+}
+
+}  // namespace rfsn

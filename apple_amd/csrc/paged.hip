@@ -1,0 +1,435 @@
+// Paged KV cache: rows into pages and back, and the choice of the pages that a
+// query reads.
+#include "paged.h"
+
+namespace rfsn {
+
+int paged_check(const rfsn_paged* p, const char* what) {
+  const std::string w(what);
+  RFSN_REQUIRE(p != nullptr, w + ": null parameters");
+  RFSN_REQUIRE(p->head_dim == 64 || p->head_dim == 128 || p->head_dim == 256, w + ": head_dim must be 64, 128 or 256");
+  RFSN_REQUIRE(p->page_size == 16 || p->page_size == 32 || p->page_size == 64 || p->page_size == 128 ||
+                   p->page_size == 256,
+               w + ": page_size must be 16, 32, 64, 128 or 256");
+  RFSN_REQUIRE(p->type == RFSN_PAGE_FP16 || p->type == RFSN_PAGE_INT8 || p->type == RFSN_PAGE_E4M3,
+               w + ": unknown page type");
+  RFSN_REQUIRE(p->kv_heads > 0 && p->kv_heads <= 65535, w + ": kv_heads out of range");
+  RFSN_REQUIRE(p->batch >= 0 && p->batch <= 65535, w + ": batch out of range");
+  RFSN_REQUIRE(p->pages > 0, w + ": the pool has no pages");
+  RFSN_REQUIRE(p->table_width >= 0 && (int64_t)p->table_width * p->page_size < (1ll << 31),
+               w + ": the table's positions must stay below 2^31");
+  RFSN_REQUIRE(p->table_width == 0 || p->batch == 0 || p->table != nullptr, w + ": null table");
+  RFSN_REQUIRE(p->batch == 0 || p->lens != nullptr, w + ": null lens");
+  RFSN_REQUIRE(p->k && p->v && ((uintptr_t)p->k & 15) == 0 && ((uintptr_t)p->v & 15) == 0,
+               w + ": k and v must be 16-byte aligned");
+  RFSN_REQUIRE(p->head_stride % 16 == 0 && p->page_stride % 16 == 0 &&
+                   (p->kv_heads == 1 || p->head_stride >= (int64_t)p->page_size * p->head_dim) && p->page_stride >= 0,
+               w + ": page and head strides must be multiples of 16 that leave room for a head's rows");
+  RFSN_REQUIRE((p->type == RFSN_PAGE_FP16) == (p->k_scale == nullptr) &&
+                   (p->type == RFSN_PAGE_FP16) == (p->v_scale == nullptr),
+               w + ": 8-bit pages need both scales, fp16 pages none");
+  RFSN_REQUIRE(((uintptr_t)p->bounds & 15) == 0 && ((uintptr_t)p->k_scale & 15) == 0 && ((uintptr_t)p->v_scale & 15) == 0,
+               w + ": scales and bounds must be 16-byte aligned");
+  return RFSN_OK;
+}
+
+namespace {
+
+// Sequence of row n < cu[batch], or -1: the last b with cu[b] <= n.  Memory-safe
+// whatever cu holds.
+__device__ __forceinline__ int row_sequence(const int32_t* __restrict__ cu, int batch, int64_t n) {
+  if (n >= cu[batch] || n < cu[0]) return -1;
+  int lo = 0, hi = batch;  // cu[lo] <= n < cu[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (n >= cu[mid]) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+struct RowPlace {
+  int page;   // of the pool, or -1
+  int row;    // in the page
+  int count;  // rows of this call in the same page from here on
+  bool start; // the first of them
+};
+__device__ __forceinline__ RowPlace row_place(const rfsn_paged& p, int shift, const int32_t* __restrict__ cu,
+                                              int64_t rows, int64_t n) {
+  RowPlace r = {-1, 0, 0, false};
+  if (n >= rows) return r;
+  int b;
+  int64_t i, left;
+  if (cu) {
+    b = row_sequence(cu, p.batch, n);
+    if (b < 0) return r;
+    i = n - cu[b];
+    const int64_t end = cu[b + 1] < rows ? cu[b + 1] : rows;
+    left = end - n;
+  } else {
+    b = (int)n, i = 0, left = 1;
+  }
+  const int64_t pos = (int64_t)max(p.lens[b], 0) + i;
+  r.page = paged_page(p, b, pos >> shift);
+  r.row = (int)(pos & (p.page_size - 1));
+  r.count = (int)(left < p.page_size - r.row ? left : p.page_size - r.row);
+  r.start = i == 0 || r.row == 0;
+  return r;
+}
+
+// The sum of a quantised row's codes is never formed: rounding is one fp32
+// product, then the code's own.
+template <int TYPE, int LANES>
+__device__ __forceinline__ void store_row(const rfsn_paged& p, void* base, float* scales, int64_t off, int64_t scale_at,
+                                          half8v x, int chunk, bool write) {
+  if constexpr (TYPE == RFSN_PAGE_FP16) {
+    if (write) *reinterpret_cast<half8v*>((uint16_t*)base + off) = x;
+  } else {
+    uint32_t top = 0;  // |x| as bits: infinity and NaN are the largest
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, (uint32_t)__builtin_bit_cast(uint16_t, (f16)x[e]) & 0x7fffu);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    constexpr float kTop = TYPE == RFSN_PAGE_INT8 ? 127.f : 448.f;
+    const bool finite = top < 0x7c00u;
+    const float amax = h2f((uint16_t)top);
+    const float scale = finite ? amax / kTop : __builtin_nanf("");
+    const float inv = finite && top ? kTop / amax : 0.f;
+    uint2v c;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = finite ? (float)x[4 * w + e] * inv : 0.f;
+      if constexpr (TYPE == RFSN_PAGE_INT8) {
+        c[w] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[w] |= ((uint32_t)(int)rintf(y[e]) & 255u) << (8 * e);
+      } else {
+        int q = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+        c[w] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], q, true);
+      }
+    }
+    if (write) {
+      *reinterpret_cast<uint2v*>((uint8_t*)base + off) = c;
+      if (chunk == 0) scales[scale_at] = scale;
+    }
+  }
+}
+
+__device__ __forceinline__ f16 min_nan(f16 a, f16 b) { return a < b || a != a ? a : b; }
+__device__ __forceinline__ f16 max_nan(f16 a, f16 b) { return a > b || a != a ? a : b; }
+
+// A wave writes RS = 64 / (D / 8) rows of one head, K and V; a lane holds 8
+// coordinates of a row.  Bounds: the wave of a run's first row (rows of one
+// sequence in one page) reads the run's keys and writes the page's bounds, so
+// no two waves write the same ones and no order changes them.
+template <int D, int TYPE>
+__global__ void __launch_bounds__(256)
+paged_append_kernel(const rfsn_paged p, int shift, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
+                    int64_t ts, int64_t hs, int64_t rows, const int32_t* __restrict__ cu) {
+  constexpr int LANES = D / 8, RS = 64 / LANES;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int h = blockIdx.y * 4 + wave;
+  if (h >= p.kv_heads) return;
+  const int slot = lane / LANES, chunk = lane % LANES;
+  const int64_t n = (int64_t)blockIdx.x * RS + slot;
+  const int64_t nc = n < rows ? n : rows - 1;
+  const half8v kx = *reinterpret_cast<const half8v*>(k + nc * ts + h * hs + chunk * 8);
+  const half8v vx = *reinterpret_cast<const half8v*>(v + nc * ts + h * hs + chunk * 8);
+  const RowPlace at = row_place(p, shift, cu, rows, n);
+  const bool write = at.page >= 0;
+  const int64_t off = (int64_t)(write ? at.page : 0) * p.page_stride + h * p.head_stride + (int64_t)at.row * D + chunk * 8;
+  const int64_t sc = ((int64_t)(write ? at.page : 0) * p.kv_heads + h) * p.page_size + at.row;
+  store_row<TYPE, LANES>(p, p.k, p.k_scale, off, sc, kx, chunk, write);
+  store_row<TYPE, LANES>(p, p.v, p.v_scale, off, sc, vx, chunk, write);
+  if (p.bounds == nullptr) return;
+  const bool leads = write && at.start;
+  // runs of one row: each row slot on its own; longer ones by the whole wave
+  if (leads && at.count == 1) {
+    half8v* bp = reinterpret_cast<half8v*>((uint16_t*)p.bounds + ((int64_t)at.page * p.kv_heads + h) * 2 * D + chunk * 8);
+    half8v lo = kx, hi = kx;
+    if (at.row > 0) {
+      const half8v lo0 = bp[0], hi0 = bp[D / 8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) lo[e] = min_nan(lo0[e], lo[e]), hi[e] = max_nan(hi0[e], hi[e]);
+    }
+    bp[0] = lo, bp[D / 8] = hi;
+  }
+  uint64_t todo = __ballot(leads && at.count > 1);
+  while (todo) {
+    const int src = __ffsll((unsigned long long)todo) - 1;  // a lane of the run's first row
+    todo &= ~((LANES == 64 ? ~0ull : ((1ull << LANES) - 1)) << (src / LANES * LANES));
+    const int page = __builtin_amdgcn_readlane(at.page, src), row = __builtin_amdgcn_readlane(at.row, src);
+    const int count = __builtin_amdgcn_readlane(at.count, src);
+    const int64_t n0 = (int64_t)blockIdx.x * RS + src / LANES;
+    half8v lo = *reinterpret_cast<const half8v*>(k + (n0 + min(slot, count - 1)) * ts + h * hs + chunk * 8);
+    half8v hi = lo;
+    for (int i = slot + RS; i < count; i += RS) {
+      const half8v x = *reinterpret_cast<const half8v*>(k + (n0 + i) * ts + h * hs + chunk * 8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) lo[e] = min_nan(lo[e], x[e]), hi[e] = max_nan(hi[e], x[e]);
+    }
+    half8v* bp = reinterpret_cast<half8v*>((uint16_t*)p.bounds + ((int64_t)page * p.kv_heads + h) * 2 * D + chunk * 8);
+    if (row > 0) {
+      const half8v lo0 = bp[0], hi0 = bp[D / 8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) lo[e] = min_nan(lo0[e], lo[e]), hi[e] = max_nan(hi0[e], hi[e]);
+    }
+#pragma unroll
+    for (int o = LANES; o < 64; o <<= 1) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        const h2 l2 = __builtin_bit_cast(h2, __shfl_xor((int)__builtin_bit_cast(u4, lo)[w], o, 64));
+        const h2 h2v = __builtin_bit_cast(h2, __shfl_xor((int)__builtin_bit_cast(u4, hi)[w], o, 64));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          lo[2 * w + e] = min_nan(lo[2 * w + e], l2[e]);
+          hi[2 * w + e] = max_nan(hi[2 * w + e], h2v[e]);
+        }
+      }
+    }
+    if (slot == 0) bp[0] = lo, bp[D / 8] = hi;
+  }
+}
+
+template <int D, int TYPE>
+__global__ void __launch_bounds__(256)
+paged_read_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ cu, int64_t rows,
+                  uint16_t* __restrict__ out_k, uint16_t* __restrict__ out_v, int zero_rest) {
+  constexpr int LANES = D / 8, RS = 64 / LANES;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int h = blockIdx.y * 4 + wave;
+  if (h >= p.kv_heads) return;
+  const int slot = lane / LANES, chunk = lane % LANES;
+  const int64_t n = (int64_t)blockIdx.x * RS + slot;
+  if (n >= rows) return;
+  const bool rest = row_sequence(cu, p.batch, n) < 0;
+  if (rest && !zero_rest) return;
+  const RowPlace at = row_place(p, shift, cu, rows, n);
+  half8v ko = {}, vo = {};
+  if (!rest && at.page >= 0) {
+    const int64_t off = (int64_t)at.page * p.page_stride + h * p.head_stride + (int64_t)at.row * D + chunk * 8;
+    if constexpr (TYPE == RFSN_PAGE_FP16) {
+      ko = *reinterpret_cast<const half8v*>((const uint16_t*)p.k + off);
+      vo = *reinterpret_cast<const half8v*>((const uint16_t*)p.v + off);
+    } else {
+      const int64_t sc = ((int64_t)at.page * p.kv_heads + h) * p.page_size + at.row;
+      const float ks = p.k_scale[sc], vs = p.v_scale[sc];
+      const float8v kf = load_page8<TYPE>(p.k, off), vf = load_page8<TYPE>(p.v, off);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ko[e] = (f16)(kf[e] * ks), vo[e] = (f16)(vf[e] * vs);
+    }
+  }
+  const int64_t o = (n * p.kv_heads + h) * D + chunk * 8;
+  *reinterpret_cast<half8v*>(out_k + o) = ko;
+  *reinterpret_cast<half8v*>(out_v + o) = vo;
+}
+
+// ---------------------------------------------------------------- page choice
+
+// Score of every page held by (sequence, KV head): a lane takes 8 coordinates
+// of a page's bounds, D / 8 lanes a page.  Products of fp16 values are exact in
+// fp32, and of q+ hi and q- lo one is zero; sums are held in 64 bits.
+template <int D>
+__global__ void __launch_bounds__(256)
+page_score_kernel(const rfsn_paged p, int shift, const uint16_t* __restrict__ q, int G, float* __restrict__ score) {
+  constexpr int LANES = D / 8, RS = 64 / LANES;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int slot = lane / LANES, chunk = lane % LANES;
+  const int held = (int)(((int64_t)paged_len(p, shift, b) + p.page_size - 1) >> shift);
+  const int n = (blockIdx.x * 4 + wave) * RS + slot;
+  const int page = n < held ? paged_page(p, b, n) : -1;
+  half8v lo = {}, hi = {};
+  if (page >= 0) {
+    const half8v* bp =
+        reinterpret_cast<const half8v*>((const uint16_t*)p.bounds + ((int64_t)page * p.kv_heads + h) * 2 * D + chunk * 8);
+    lo = bp[0], hi = bp[D / 8];
+  }
+  double best = -__builtin_inf();
+  bool nan = false;
+  for (int g = 0; g < G; ++g) {
+    const half8v qv = *reinterpret_cast<const half8v*>(q + (((int64_t)b * p.kv_heads + h) * G + g) * D + chunk * 8);
+    double s = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = (float)qv[e];
+      const float up = x < 0.f ? 0.f : x, down = x > 0.f ? 0.f : x;
+      s += (double)fmaf(up, (float)hi[e], down * (float)lo[e]);
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    nan |= s != s;
+    best = s > best ? s : best;
+  }
+  if (n < held && chunk == 0)
+    score[((int64_t)b * p.kv_heads + h) * p.table_width + n] =
+        page < 0 ? -__builtin_inff() : nan ? __builtin_nanf("") : (float)best;
+}
+
+// Order of the scores as unsigned keys: kept pages over all, NaN as +infinity, -0 as +0.
+__device__ __forceinline__ uint32_t page_key(float s, int n, int held, int first, int last) {
+  if (n < first || n >= held - last) return 0xffffffffu;
+  if (s != s) s = __builtin_inff();
+  const uint32_t u = __builtin_bit_cast(uint32_t, s + 0.f);
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+// The count largest keys of a row, their indices ascending: the count-th
+// largest key by four passes over 8 bits, then one pass that keeps what is above
+// it and, in order, as many equal to it as there is room for.
+__global__ void __launch_bounds__(256)
+page_choose_kernel(const rfsn_paged p, int shift, const float* __restrict__ score, int count, int first, int last,
+                   int32_t* __restrict__ chosen) {
+  __shared__ uint32_t hist[256];
+  __shared__ uint32_t s_digit, s_left, s_part[2][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int h = blockIdx.x, b = blockIdx.y;
+  const int64_t row = (int64_t)b * p.kv_heads + h;
+  const float* s = score + row * p.table_width;
+  int32_t* out = chosen + row * count;
+  const int held = (int)(((int64_t)paged_len(p, shift, b) + p.page_size - 1) >> shift);
+  if (held <= count) {
+    for (int i = tid; i < count; i += 256) out[i] = i < held ? i : -1;
+    return;
+  }
+  uint32_t prefix = 0, mask = 0;
+  uint32_t left = (uint32_t)count;  // of the keys that share the prefix, how many are kept
+  for (int at = 24; at >= 0; at -= 8) {
+    hist[tid] = 0;
+    __syncthreads();
+    for (int n = tid; n < held; n += 256) {
+      const uint32_t key = page_key(s[n], n, held, first, last);
+      if ((key & mask) == prefix) atomicAdd(&hist[(key >> at) & 255u], 1u);
+    }
+    __syncthreads();
+    // thread i: how many keys have a digit above i
+    uint32_t above = 0;
+    for (int i = tid + 1; i < 256; ++i) above += hist[i];
+    if (above < left && above + hist[tid] >= left) s_digit = (uint32_t)tid, s_left = left - above;
+    __syncthreads();
+    prefix |= s_digit << at;
+    mask |= 255u << at;
+    left = s_left;
+    __syncthreads();
+  }
+  uint32_t done = 0, ties = 0;  // written so far; equal keys seen so far
+  for (int base = 0; base < held; base += 256) {
+    const int n = base + tid;
+    const uint32_t key = n < held ? page_key(s[n], n, held, first, last) : 0u;
+    const bool over = n < held && key > prefix, tie = n < held && key == prefix;
+    const uint64_t bt = __ballot(tie), below = (1ull << lane) - 1;
+    if (lane == 0) s_part[0][wave] = (uint32_t)__popcll(bt);
+    __syncthreads();
+    uint32_t before = ties, all = ties;
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) before += s_part[0][w];
+      all += s_part[0][w];
+    }
+    const bool keep = over || (tie && before + (uint32_t)__popcll(bt & below) < left);
+    const uint64_t bk = __ballot(keep);
+    if (lane == 0) s_part[1][wave] = (uint32_t)__popcll(bk);
+    __syncthreads();
+    uint32_t at = done, total = done;
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) at += s_part[1][w];
+      total += s_part[1][w];
+    }
+    if (keep) out[at + (uint32_t)__popcll(bk & below)] = n;
+    done = total, ties = all;
+  }
+}
+
+#define RFSN_PAGED_DISPATCH(D, TYPE, ...)                                                       \
+  do {                                                                                          \
+    if (D == 64 && TYPE == RFSN_PAGE_FP16) { constexpr int DD = 64, TT = RFSN_PAGE_FP16; __VA_ARGS__ }        \
+    else if (D == 64 && TYPE == RFSN_PAGE_INT8) { constexpr int DD = 64, TT = RFSN_PAGE_INT8; __VA_ARGS__ }   \
+    else if (D == 64) { constexpr int DD = 64, TT = RFSN_PAGE_E4M3; __VA_ARGS__ }                             \
+    else if (D == 128 && TYPE == RFSN_PAGE_FP16) { constexpr int DD = 128, TT = RFSN_PAGE_FP16; __VA_ARGS__ } \
+    else if (D == 128 && TYPE == RFSN_PAGE_INT8) { constexpr int DD = 128, TT = RFSN_PAGE_INT8; __VA_ARGS__ } \
+    else if (D == 128) { constexpr int DD = 128, TT = RFSN_PAGE_E4M3; __VA_ARGS__ }                           \
+    else if (TYPE == RFSN_PAGE_FP16) { constexpr int DD = 256, TT = RFSN_PAGE_FP16; __VA_ARGS__ }             \
+    else if (TYPE == RFSN_PAGE_INT8) { constexpr int DD = 256, TT = RFSN_PAGE_INT8; __VA_ARGS__ }             \
+    else { constexpr int DD = 256, TT = RFSN_PAGE_E4M3; __VA_ARGS__ }                                         \
+  } while (0)
+
+}  // namespace
+}  // namespace rfsn
+
+using namespace rfsn;
+
+extern "C" int rfsn_paged_append(const rfsn_paged* p, const void* k, const void* v, int64_t token_stride,
+                                 int64_t head_stride, int64_t rows, const int32_t* cu, void* stream) {
+  if (int st = paged_check(p, "paged_append")) return st;
+  RFSN_REQUIRE(rows >= 0, "paged_append: negative row count");
+  RFSN_REQUIRE(cu != nullptr || rows == p->batch, "paged_append: without cu there is one row per sequence");
+  if (rows == 0 || p->batch == 0) return RFSN_OK;
+  RFSN_REQUIRE(k && v && ((uintptr_t)k & 15) == 0 && ((uintptr_t)v & 15) == 0 && token_stride % 8 == 0 &&
+                   head_stride % 8 == 0,
+               "paged_append: k and v rows must be 16-byte aligned");
+  const int rs = 512 / p->head_dim;
+  RFSN_REQUIRE(ceil_div(rows, rs) < (1ll << 24), "paged_append: too many rows");
+  const int shift = paged_shift(*p);
+  const dim3 grid((unsigned)ceil_div(rows, rs), (unsigned)ceil_div(p->kv_heads, 4));
+  RFSN_PAGED_DISPATCH(p->head_dim, p->type, {
+    hipLaunchKernelGGL((paged_append_kernel<DD, TT>), grid, dim3(256), 0, (hipStream_t)stream, *p, shift,
+                       (const uint16_t*)k, (const uint16_t*)v, token_stride, head_stride, rows, cu);
+  });
+  return check_launch("paged_append");
+}
+
+extern "C" int rfsn_paged_read(const rfsn_paged* p, const int32_t* cu, int64_t rows, void* out_k, void* out_v,
+                               int32_t zero_rest, void* stream) {
+  if (int st = paged_check(p, "paged_read")) return st;
+  RFSN_REQUIRE(rows >= 0, "paged_read: negative row count");
+  if (rows == 0) return RFSN_OK;
+  RFSN_REQUIRE(cu != nullptr, "paged_read: null cu");
+  RFSN_REQUIRE(out_k && out_v && ((uintptr_t)out_k & 15) == 0 && ((uintptr_t)out_v & 15) == 0,
+               "paged_read: outputs must be 16-byte aligned");
+  const int rs = 512 / p->head_dim;
+  RFSN_REQUIRE(ceil_div(rows, rs) < (1ll << 24), "paged_read: too many rows");
+  const int shift = paged_shift(*p);
+  const dim3 grid((unsigned)ceil_div(rows, rs), (unsigned)ceil_div(p->kv_heads, 4));
+  RFSN_PAGED_DISPATCH(p->head_dim, p->type, {
+    hipLaunchKernelGGL((paged_read_kernel<DD, TT>), grid, dim3(256), 0, (hipStream_t)stream, *p, shift, cu, rows,
+                       (uint16_t*)out_k, (uint16_t*)out_v, zero_rest);
+  });
+  return check_launch("paged_read");
+}
+
+extern "C" size_t rfsn_page_select_workspace_bytes(const rfsn_paged* p) {
+  if (p == nullptr || p->batch <= 0 || p->kv_heads <= 0 || p->table_width <= 0) return 0;
+  return (size_t)p->batch * p->kv_heads * p->table_width * sizeof(float);
+}
+
+extern "C" int rfsn_page_select(const rfsn_paged* p, const void* q, int32_t q_heads, int32_t count, int32_t first,
+                                int32_t last, int32_t* chosen, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int st = paged_check(p, "page_select")) return st;
+  RFSN_REQUIRE(p->bounds != nullptr, "page_select: the pages hold no bounds");
+  RFSN_REQUIRE(q_heads > 0 && q_heads % p->kv_heads == 0, "page_select: q_heads must be a multiple of kv_heads");
+  RFSN_REQUIRE(count > 0 && first >= 0 && last >= 0 && (int64_t)first + last <= count,
+               "page_select: count must be positive and have room for the first and last pages");
+  if (p->batch == 0) return RFSN_OK;
+  RFSN_REQUIRE(q && ((uintptr_t)q & 15) == 0 && chosen, "page_select: null or misaligned q, or null output");
+  RFSN_REQUIRE(workspace_bytes >= rfsn_page_select_workspace_bytes(p) && (workspace || p->table_width == 0),
+               "page_select: workspace too small");
+  const int shift = paged_shift(*p);
+  const hipStream_t s = (hipStream_t)stream;
+  const int G = q_heads / p->kv_heads;
+  if (p->table_width > 0) {
+    const int per = 4 * (512 / p->head_dim);
+    const dim3 grid((unsigned)ceil_div(p->table_width, per), (unsigned)p->kv_heads, (unsigned)p->batch);
+#define RFSN_SCORE(DD) \
+  hipLaunchKernelGGL(page_score_kernel<DD>, grid, dim3(256), 0, s, *p, shift, (const uint16_t*)q, G, (float*)workspace)
+    if (p->head_dim == 64) RFSN_SCORE(64);
+    else if (p->head_dim == 128) RFSN_SCORE(128);
+    else RFSN_SCORE(256);
+#undef RFSN_SCORE
+    if (int st = check_launch("page_select")) return st;
+  }
+  hipLaunchKernelGGL(page_choose_kernel, dim3((unsigned)p->kv_heads, (unsigned)p->batch), dim3(256), 0, s, *p, shift,
+                     (const float*)workspace, count, first, last, chosen);
+  return check_launch("page_select");
+}

@@ -11,7 +11,7 @@ import ctypes as C
 import weakref
 from collections import OrderedDict
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -698,6 +698,185 @@ def fused_attention(q: torch.Tensor, fmt: WarmFormat, *, kv_heads: int, scale: f
     if not launch:
         return fl
     fl()
+    return out
+
+
+# --------------------------------------------------------------------------
+# paged KV cache
+# --------------------------------------------------------------------------
+
+PAGE_SIZES = (16, 32, 64, 128, 256)
+PAGE_TYPES = {torch.float16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
+
+
+class KVPages(NamedTuple):
+    """A pool of pages (``rfsn_paged``): k, v [P, Hkv, S, D] fp16, int8 or
+    float8_e4m3fn, of one stride each, rows dense; with 8-bit codes the rows'
+    scales [P, Hkv, S] fp32; bounds [P, Hkv, 2, D] fp16, each page's smallest and
+    largest key per coordinate, where pages are to be selected by them."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
+    bounds: Optional[torch.Tensor] = None
+
+
+def _paged(what: str, pages: KVPages, table: torch.Tensor, lens: torch.Tensor) -> "L.Paged":
+    """The checked parameter block of a pool, a block table [B, W] int32 and lengths [B] int32."""
+    k, v, ks, vs, bounds = pages
+    dev = _dev(k, what).device
+    if k.dim() != 4 or v.shape != k.shape or v.dtype is not k.dtype or v.stride() != k.stride():
+        raise ValueError(f"{what}: k and v pages must be alike, [pages, kv_heads, page_size, head_dim]")
+    P, H, S, D = k.shape
+    kind = PAGE_TYPES.get(k.dtype)
+    if kind is None:
+        raise ValueError(f"{what}: pages of {k.dtype}; float16, int8 and float8_e4m3fn are served")
+    sp, sh, ss, sd = k.stride()
+    if sd != 1 or ss != D:
+        raise ValueError(f"{what}: a head's rows must be dense")
+    if (kind == 0) != (ks is None) or (kind == 0) != (vs is None):
+        raise ValueError(f"{what}: 8-bit pages need k_scale and v_scale, fp16 pages neither")
+    for t, shape, dtype, name in ((ks, (P, H, S), torch.float32, "k_scale"), (vs, (P, H, S), torch.float32, "v_scale"),
+                                  (bounds, (P, H, 2, D), torch.float16, "bounds")):
+        if t is not None and (t.shape != shape or t.dtype is not dtype or not t.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be contiguous {list(shape)} {dtype}")
+    if table.dim() != 2 or table.dtype is not torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError(f"{what}: the block table must be int32 [batch, pages per sequence] with dense rows")
+    if lens.shape != (table.shape[0],) or lens.dtype is not torch.int32 or not lens.is_contiguous():
+        raise ValueError(f"{what}: lengths must be contiguous int32 [batch]")
+    for t in (v, ks, vs, bounds, table, lens):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: pages, table and lengths must be on one device")
+    return L.Paged(k.data_ptr(), v.data_ptr(), L.ptr(ks), L.ptr(vs), L.ptr(bounds), table.data_ptr(), lens.data_ptr(),
+                   sp, sh, table.stride(0), P, S, H, D, kind, table.shape[0], table.shape[1])
+
+
+def _paged_call(device: torch.device, name: str, *args) -> None:
+    """The call on ``device``'s current stream, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        L.call(name, *args, L.stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            L.call(name, *args, L.stream_handle(device))
+
+
+def _cu(what: str, cu: torch.Tensor, batch: int, device: torch.device) -> int:
+    if cu.shape != (batch + 1,) or cu.dtype is not torch.int32 or not cu.is_contiguous() or cu.device != device:
+        raise ValueError(f"{what}: cu must be contiguous int32 [batch + 1] on the pages' device")
+    return cu.data_ptr()
+
+
+def _paged_query(what: str, q: torch.Tensor, p: "L.Paged", device: torch.device) -> torch.Tensor:
+    if q.dim() != 3 or q.dtype is not torch.float16 or q.shape[0] != p.batch or q.shape[2] != p.head_dim \
+            or q.device != device:
+        raise ValueError(f"{what}: q must be fp16 [batch, q_heads, head_dim] = [{p.batch}, *, {p.head_dim}] "
+                         "on the pages' device")
+    q = _contig(q)
+    return q.clone() if q.data_ptr() % 16 else q
+
+
+def paged_append(pages: KVPages, table: torch.Tensor, lens: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                 cu: Optional[torch.Tensor] = None) -> None:
+    """New rows k, v [N, Hkv, D] fp16 into the pages, quantised where they hold
+    codes, with the pages' bounds: rows cu[b] .. cu[b + 1] - 1 (``cu`` [B + 1]
+    int32; None: row b) follow the ``lens[b]`` tokens of sequence b.  Rows
+    behind cu[B] are ignored, as is what the table has no page for; ``lens`` is
+    not changed.  No two sequences of a call may append to one page."""
+    p = _paged("paged_append", pages, table, lens)
+    dev = pages.k.device
+    if k.dim() != 3 or k.shape[1:] != (p.kv_heads, p.head_dim) or v.shape != k.shape \
+            or k.dtype is not torch.float16 or v.dtype is not torch.float16 or k.device != dev or v.device != dev:
+        raise ValueError(f"paged_append: k and v must be fp16 [rows, {p.kv_heads}, {p.head_dim}] on the pages' device")
+    n = k.shape[0]
+    if cu is None:
+        if n != p.batch:
+            raise ValueError(f"paged_append: without cu there is one row per sequence ({p.batch}), got {n}")
+    else:
+        cu_ptr = _cu("paged_append", cu, p.batch, dev)
+    if n == 0:
+        return
+    ts, hs, cs = k.stride()
+    if v.stride() != (ts, hs, cs) or cs != 1 or ts % 8 or hs % 8 or k.data_ptr() % 16 or v.data_ptr() % 16:
+        k, v = k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format)
+        ts, hs, _ = k.stride()
+    _paged_call(dev, "rfsn_paged_append", C.byref(p), k.data_ptr(), v.data_ptr(), ts, hs, n,
+                None if cu is None else cu_ptr)
+
+
+def paged_read(pages: KVPages, table: torch.Tensor, starts: torch.Tensor, cu: torch.Tensor, rows: int,
+               out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """K and V rows [rows, Hkv, D] fp16 read back: rows cu[b] .. cu[b + 1] - 1
+    are positions starts[b], starts[b] + 1, ... of sequence b, zeros where the
+    table has no page.  Rows behind cu[B] are zeros; in ``out`` (k, v of that
+    shape, contiguous) they are left as they were."""
+    p = _paged("paged_read", pages, table, starts)
+    dev = pages.k.device
+    rows = int(rows)
+    if rows < 0:
+        raise ValueError("paged_read: negative row count")
+    shape = (rows, p.kv_heads, p.head_dim)
+    cu_ptr = _cu("paged_read", cu, p.batch, dev)
+    if out is None:
+        ko = torch.empty(shape, dtype=torch.float16, device=dev)
+        vo = torch.empty(shape, dtype=torch.float16, device=dev)
+    else:
+        ko, vo = out
+        for t in out:
+            if t.shape != shape or t.dtype is not torch.float16 or not t.is_contiguous() or t.device != dev \
+                    or t.data_ptr() % 16:
+                raise ValueError(f"paged_read: out must be two contiguous fp16 {list(shape)} on the pages' device")
+    if rows:
+        _paged_call(dev, "rfsn_paged_read", C.byref(p), cu_ptr, rows, ko.data_ptr(), vo.data_ptr(), int(out is None))
+    return ko, vo
+
+
+def page_select(q: torch.Tensor, pages: KVPages, table: torch.Tensor, lens: torch.Tensor, count: int, *,
+                first: int = 1, last: int = 1) -> torch.Tensor:
+    """The pages that q [B, Hq, D] reads when it reads ``count`` of each
+    sequence's: int32 [B, Hkv, count] page ordinals, ascending, then -1.  The
+    ``first`` and ``last`` ones are always among them, the others those with the
+    largest upper bound of q . k by the pages' bounds, over the KV head's query
+    heads (``rfsn_page_select``)."""
+    p = _paged("page_select", pages, table, lens)
+    dev = pages.k.device
+    if pages.bounds is None:
+        raise ValueError("page_select: the pages hold no bounds")
+    q = _paged_query("page_select", q, p, dev)
+    count, first, last = int(count), int(first), int(last)
+    if count <= 0 or first < 0 or last < 0 or first + last > count:
+        raise ValueError("page_select: count must be positive and have room for the first and last pages")
+    chosen = torch.empty((p.batch, p.kv_heads, count), dtype=torch.int32, device=dev)
+    wsb = L.load().rfsn_page_select_workspace_bytes(C.byref(p))
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    _paged_call(dev, "rfsn_page_select", C.byref(p), q.data_ptr(), q.shape[1], count, first, last, chosen.data_ptr(),
+                ws.data_ptr(), wsb)
+    return chosen
+
+
+def paged_attention(q: torch.Tensor, pages: KVPages, table: torch.Tensor, lens: torch.Tensor, scale: float,
+                    chosen: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Exact attention of one query per sequence, q [B, Hq, D] fp16, over the
+    sequence's first ``lens[b]`` positions, or over those of its pages that
+    ``chosen`` [B, Hkv, n] (``page_select``) lists; zeros where there are none.
+    Codes are attended as code * scale in fp32, not rounded to fp16."""
+    p = _paged("paged_attention", pages, table, lens)
+    dev = pages.k.device
+    q = _paged_query("paged_attention", q, p, dev)
+    count = 0
+    if chosen is not None:
+        if chosen.dim() != 3 or chosen.shape[:2] != (p.batch, p.kv_heads) or chosen.dtype is not torch.int32 \
+                or chosen.device != dev:
+            raise ValueError(f"paged_attention: chosen must be int32 [{p.batch}, {p.kv_heads}, n] on the pages' device")
+        chosen = _contig(chosen)
+        count = chosen.shape[2]
+    out = torch.empty_like(q)
+    if chosen is not None and count == 0:
+        return out.zero_()
+    wsb = L.load().rfsn_paged_attention_workspace_bytes(C.byref(p), q.shape[1], count)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+    _paged_call(dev, "rfsn_paged_attention", C.byref(p), q.data_ptr(), q.shape[1], float(scale), L.ptr(chosen), count,
+                out.data_ptr(), L.ptr(ws), wsb)
     return out
 
 

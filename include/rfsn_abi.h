@@ -574,6 +574,85 @@ int rfsn_ref_tables_ok(const rfsn_ref_params* p);
  * the params' format and codebooks only; depends on nothing else. */
 int rfsn_ref_table_stats(const rfsn_ref_params* p, float* stats_dev, void* stream);
 
+/* ---------------------------------------------------------------- paged KV
+ * A pool of pages that all sequences of a batch share (no counterpart in the
+ * reference, which keeps one cache per sequence, cache.py:33-57).  Position t
+ * of sequence b is row t % page_size of page table[b][t / page_size].
+ * K/V rows are fp16, or 8-bit codes with one fp32 scale per row (value =
+ * code * scale): int8 (scale = amax / 127) or OCP e4m3 (amax / 448).  bounds
+ * holds, per page and KV head, the smallest and the largest key of each
+ * coordinate, as fp16 of the rows before they are quantised; a NaN key makes
+ * both NaN.
+ *  - page_size: 16, 32, 64, 128 or 256; head_dim: 64, 128 or 256.
+ *  - A table entry outside [0, pages) is no page: what would be written there
+ *    is dropped, positions there are not attended and read back as zeros.
+ *  - lens below 0 count as 0, lens past table_width * page_size as that.
+ *  - Device values are never trusted for addressing: every page, row and
+ *    sequence index is checked by the kernels.
+ *  - k, v, bounds 16-byte aligned, strides multiples of 16 elements. */
+#define RFSN_PAGE_FP16 0
+#define RFSN_PAGE_INT8 1
+#define RFSN_PAGE_E4M3 2
+typedef struct rfsn_paged {
+  void* k;              /* [pages][kv_heads][page_size][head_dim]; page_stride and     */
+  void* v;              /*   head_stride elements between pages and heads, rows dense  */
+  float* k_scale;       /* [pages][kv_heads][page_size], NULL with fp16 pages          */
+  float* v_scale;
+  void* bounds;         /* fp16 [pages][kv_heads][2][head_dim], or NULL                */
+  const int32_t* table; /* [batch][table_width], table_stride entries between rows     */
+  const int32_t* lens;  /* [batch] tokens of each sequence (append, read: the first position) */
+  int64_t page_stride;
+  int64_t head_stride;
+  int64_t table_stride;
+  int32_t pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t type;         /* RFSN_PAGE_* */
+  int32_t batch;
+  int32_t table_width;
+} rfsn_paged;
+
+/* Rows k, v [rows][kv_heads][head_dim] fp16 (token_stride, head_stride
+ * elements, multiples of 8; 16-byte aligned) into the pages: rows cu[b] ..
+ * cu[b + 1] - 1 are the positions lens[b], lens[b] + 1, ... of sequence b (cu NULL: row b is
+ * sequence b's next token, rows = batch).  Rows behind cu[batch] are
+ * ignored.  The bounds of a page that starts with this call are set, those of
+ * one that goes on are widened.  A row with a value that is not finite gets
+ * scale NaN in an 8-bit page.  Sequences that append must not share a page. */
+int rfsn_paged_append(const rfsn_paged* p, const void* k, const void* v, int64_t token_stride, int64_t head_stride,
+                      int64_t rows, const int32_t* cu, void* stream);
+
+/* The reverse: out_k, out_v [rows][kv_heads][head_dim] fp16, contiguous; rows
+ * cu[b] .. cu[b + 1] - 1 become positions lens[b], ... of sequence b (whether
+ * written before or not).  Rows behind cu[batch]: zeros with zero_rest, else
+ * left as they are. */
+int rfsn_paged_read(const rfsn_paged* p, const int32_t* cu, int64_t rows, void* out_k, void* out_v, int32_t zero_rest,
+                    void* stream);
+
+/* The pages that a query reads, [batch][kv_heads][count] page ordinals of the
+ * sequence (not page numbers of the pool), ascending, then -1: the first and last
+ * ones, then those of the highest score max_g sum_d max(q_d, 0) hi_d +
+ * min(q_d, 0) lo_d over the KV head's query heads g, which no q . k of the
+ * page exceeds.  The sum is exact up to 64-bit rounding and rounded to fp32;
+ * NaN counts as infinite, ties go to the lower ordinal.  q [batch][q_heads]
+ * [head_dim] fp16. */
+size_t rfsn_page_select_workspace_bytes(const rfsn_paged* p);
+int rfsn_page_select(const rfsn_paged* p, const void* q, int32_t q_heads, int32_t count, int32_t first, int32_t last,
+                     int32_t* chosen, void* workspace, size_t workspace_bytes, void* stream);
+
+/* softmax(scale q . k) v of one query per sequence over positions [0, lens[b])
+ * (_blockwise_exact_attention, attention.py:39-105, for a batch of paged
+ * windows), out [batch][q_heads][head_dim] fp16; query head i reads KV head
+ * i / (q_heads / kv_heads).  chosen (or NULL): [batch][kv_heads][count] page ordinals,
+ * the only pages that are attended, one listed twice counting twice.  Nothing
+ * to attend, or scores all -infinite: zeros.  Weights are fp32: one under its
+ * smallest value is 0, which makes an infinite value NaN.  The workspace size depends on
+ * q_heads and, with chosen, count (0: dense). */
+size_t rfsn_paged_attention_workspace_bytes(const rfsn_paged* p, int32_t q_heads, int32_t count);
+int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t q_heads, float scale, const int32_t* chosen,
+                         int32_t count, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- k-means
  * One Lloyd update of PQ codebooks (rfsn_v10_mlx_ane_complete.py:197-207):
  * every centroid with members becomes fp16(fp32 mean of its members); empty

@@ -1,0 +1,204 @@
+"""The paged KV cache without a GPU: what its entry points refuse before a
+launch, its workspace sizes, the parameter block's layout, and the cache's own
+bookkeeping."""
+
+import ctypes
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+ROOT = Path(__file__).resolve().parent.parent
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from apple_amd import _lib
+
+    return _lib.load()
+
+
+def block(**kw):
+    """A parameter block whose addresses are never followed on the host."""
+    from apple_amd import _lib
+
+    p = _lib.Paged(k=4096, v=8192, table=16384, lens=20480, page_stride=8 * 16 * 64, head_stride=16 * 64,
+                   table_stride=10, pages=5, page_size=16, kv_heads=8, head_dim=64, type=0, batch=2, table_width=10)
+    for name, value in kw.items():
+        setattr(p, name, value)
+    return p
+
+
+def test_parameter_block_layout(tmp_path):
+    from apple_amd import _lib
+
+    fields = [f for f, _ in _lib.Paged._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "rfsn_abi.h"\nint main(void) {\n'
+                   'printf("size %zu\\n", sizeof(rfsn_paged));\n'
+                   + "".join(f'printf("{f} %zu\\n", offsetof(rfsn_paged, {f}));\n' for f in fields) + "return 0; }\n")
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-std=c11", f"-I{ROOT / 'include'}", str(src), "-o", str(exe)], check=True)
+    got = dict(l.split() for l in subprocess.run([str(exe)], capture_output=True, text=True,
+                                                  check=True).stdout.splitlines())
+    assert int(got["size"]) == ctypes.sizeof(_lib.Paged)
+    for f in fields:
+        assert int(got[f]) == getattr(_lib.Paged, f).offset, f
+
+
+@pytest.mark.parametrize("bad, says", [
+    (dict(head_dim=96), "head_dim"), (dict(page_size=8), "page_size"), (dict(page_size=48), "page_size"),
+    (dict(type=3), "page type"), (dict(kv_heads=0), "kv_heads"), (dict(batch=-1), "batch"), (dict(batch=70000), "batch"),
+    (dict(pages=0), "no pages"), (dict(table_width=-1), "table"), (dict(table_width=1 << 28), "2^31"),
+    (dict(table=0), "null table"), (dict(lens=0), "null lens"), (dict(k=0), "aligned"), (dict(v=8200), "aligned"),
+    (dict(page_stride=8), "strides"), (dict(head_stride=64), "strides"), (dict(type=1), "scales"),
+    (dict(k_scale=4096), "scales"), (dict(bounds=4100), "bounds must be")])
+def test_pools_are_refused_before_a_launch(lib, bad, says):
+    p = ctypes.byref(block(**bad))
+    for name, args in (("rfsn_paged_append", (4096, 8192, 512, 64, 2, None, None)),
+                       ("rfsn_paged_read", (4096, 2, 4096, 8192, 1, None)),
+                       ("rfsn_page_select", (4096, 8, 4, 1, 1, 4096, 4096, 1 << 30, None)),
+                       ("rfsn_paged_attention", (4096, 8, 0.125, None, 0, 4096, 4096, 1 << 30, None))):
+        assert getattr(lib, name)(p, *args) == -1, name
+        assert says.encode() in lib.rfsn_last_error(), (name, lib.rfsn_last_error())
+        assert getattr(lib, name)(None, *args) == -1
+
+
+@pytest.mark.parametrize("name, args, says", [
+    ("rfsn_paged_append", (4096, 8192, 512, 64, -1, 4096, None), "row count"),
+    ("rfsn_paged_append", (4096, 8192, 512, 64, 3, None, None), "one row per sequence"),
+    ("rfsn_paged_append", (4098, 8192, 512, 64, 2, None, None), "aligned"),
+    ("rfsn_paged_append", (4096, 8192, 510, 64, 2, None, None), "aligned"),
+    ("rfsn_paged_append", (4096, 8192, 512, 64, 1 << 40, 4096, None), "too many rows"),
+    ("rfsn_paged_read", (None, 2, 4096, 8192, 1, None), "null cu"),
+    ("rfsn_paged_read", (4096, 2, 4096, 8200, 1, None), "aligned"),
+    ("rfsn_paged_read", (4096, -2, 4096, 8192, 1, None), "row count"),
+    ("rfsn_page_select", (4096, 8, 4, 1, 1, 4096, 4096, 1 << 30, None), "no bounds"),
+    ("rfsn_paged_attention", (4096, 12, 0.125, None, 0, 4096, 4096, 1 << 30, None), "multiple of kv_heads"),
+    ("rfsn_paged_attention", (4096, 8, 0.125, 4096, 0, 4096, 4096, 1 << 30, None), "together"),
+    ("rfsn_paged_attention", (4096, 8, 0.125, None, 4, 4096, 4096, 1 << 30, None), "together"),
+    ("rfsn_paged_attention", (4096, 8, 0.125, 4096, 1 << 29, 4096, 4096, 1 << 30, None), "too many chosen"),
+    ("rfsn_paged_attention", (4096, 8, float("nan"), None, 0, 4096, 4096, 1 << 30, None), "finite"),
+    ("rfsn_paged_attention", (4100, 8, 0.125, None, 0, 4096, 4096, 1 << 30, None), "aligned")])
+def test_calls_are_refused_before_a_launch(lib, name, args, says):
+    assert getattr(lib, name)(ctypes.byref(block()), *args) == -1
+    assert says.encode() in lib.rfsn_last_error(), lib.rfsn_last_error()
+
+
+@pytest.mark.parametrize("args, says", [
+    ((4096, 12, 4, 1, 1, 4096, 4096, 1 << 30, None), "multiple of kv_heads"),
+    ((4096, 8, 0, 0, 0, 4096, 4096, 1 << 30, None), "count"), ((4096, 8, 2, 2, 1, 4096, 4096, 1 << 30, None), "count"),
+    ((4096, 8, 2, -1, 1, 4096, 4096, 1 << 30, None), "count"), ((4096, 8, 2, 1, 1, None, 4096, 1 << 30, None), "null"),
+    ((4096, 8, 2, 1, 1, 4096, 4096, 8, None), "workspace")])
+def test_selection_is_refused_before_a_launch(lib, args, says):
+    assert lib.rfsn_page_select(ctypes.byref(block(bounds=4096)), *args) == -1
+    assert says.encode() in lib.rfsn_last_error(), lib.rfsn_last_error()
+
+
+def test_workspace_sizes(lib):
+    size = lib.rfsn_paged_attention_workspace_bytes
+    assert size(None, 8, 0) == 0
+    assert size(ctypes.byref(block()), 8, 0) == 0  # 160 positions: one chunk, no partials
+    wide = block(table_width=4096)
+    need = size(ctypes.byref(wide), 32, 0)
+    assert need > 0 and need % (32 * 66 * 4) == 0
+    assert lib.rfsn_paged_attention(ctypes.byref(wide), 4096, 32, 0.125, None, 0, 4096, 4096, need - 1, None) == -1
+    assert b"workspace" in lib.rfsn_last_error()
+    assert lib.rfsn_page_select_workspace_bytes(ctypes.byref(wide)) >= 2 * 8 * 4096 * 4
+    # an empty batch is no error and launches nothing
+    none = ctypes.byref(block(batch=0, table=0, lens=0))
+    assert lib.rfsn_paged_attention(none, None, 8, 0.125, None, 0, None, None, 0, None) == 0
+    assert lib.rfsn_paged_append(none, None, None, 0, 0, 0, None, None) == 0
+
+
+def tensors(kind=torch.float16, batch=2):
+    from apple_amd.kernels import KVPages
+
+    k = torch.zeros((4, 2, 16, 64), dtype=kind)
+    s = None if kind == torch.float16 else torch.zeros((4, 2, 16))
+    return (KVPages(k, k.clone(), s, s, torch.zeros((4, 2, 2, 64), dtype=torch.float16)),
+            torch.zeros((batch, 4), dtype=torch.int32), torch.zeros(batch, dtype=torch.int32))
+
+
+def test_host_tensors_are_refused():
+    from apple_amd import kernels as K
+
+    pages, table, lens = tensors()
+    q = torch.zeros((2, 4, 64), dtype=torch.float16)
+    for call in (lambda: K.paged_attention(q, pages, table, lens, 0.125),
+                 lambda: K.page_select(q, pages, table, lens, 2),
+                 lambda: K.paged_append(pages, table, lens, q[:, :2], q[:, :2]),
+                 lambda: K.paged_read(pages, table, lens, torch.zeros(3, dtype=torch.int32), 0)):
+        with pytest.raises(RuntimeError, match="GPU only"):
+            call()
+
+
+def config(**kw):
+    from apple_amd.storage import RFSNConfig
+
+    return RFSNConfig(**{**dict(hidden_dim=512, num_heads=8, num_kv_heads=2, head_dim=64, num_subspaces=8,
+                                subspace_dim=8), **kw})
+
+
+def test_cache_arguments():
+    from apple_amd.paged import RFSNPagedKVCache
+
+    make = lambda **kw: RFSNPagedKVCache(config(), **{**dict(batch=2, pages=8, device="cpu"), **kw})
+    for bad in (dict(batch=0), dict(pages=0), dict(page_size=24), dict(page_type="bf16"), dict(max_tokens=0)):
+        with pytest.raises(ValueError):
+            make(**bad)
+    with pytest.raises(ValueError):
+        RFSNPagedKVCache(config(head_dim=32, num_subspaces=8, subspace_dim=4), 2, 8, device="cpu")
+    assert make().table.shape == (2, 8)
+    assert make(max_tokens=100).table.shape == (2, 2) and make(max_tokens=100).max_tokens == 100
+    assert make(bounds=False).pages.bounds is None
+
+
+def test_cache_page_bookkeeping(monkeypatch):
+    """Pages are taken when a sequence passes its last one's end and return on release; a refused call takes none."""
+    from apple_amd import kernels as K
+    from apple_amd.paged import RFSNPagedKVCache
+
+    calls = []
+    monkeypatch.setattr(K, "paged_append", lambda pages, table, lens, k, v, cu=None: calls.append(
+        (lens.clone(), None if cu is None else cu.clone())))
+    c = RFSNPagedKVCache(config(), batch=3, pages=5, page_size=16, max_tokens=64, device="cpu")
+    rows = lambda n: torch.zeros((n, 2, 64), dtype=torch.float16)
+    c.append(rows(20), rows(20), [16, 0, 4])
+    assert c.free_pages == 3 and c.num_tokens == [16, 0, 4] and c.lens.tolist() == [16, 0, 4]
+    assert calls[-1][0].tolist() == [0, 0, 0] and calls[-1][1].tolist() == [0, 16, 16, 20]
+    c.append(rows(3), rows(3))
+    assert calls[-1][1] is None and c.lens.tolist() == [17, 1, 5] and c.free_pages == 1
+    held = c.table[c.table >= 0].tolist()
+    assert len(set(held)) == len(held) == 4
+    for bad, error in ((lambda: c.append(rows(2), rows(2)), ValueError), (lambda: c.prefill(3, rows(1), rows(1)), ValueError),
+                       (lambda: c.append(rows(3), rows(2)), ValueError), (lambda: c.prefill(1, rows(64), rows(64)), ValueError),
+                       (lambda: c.append(rows(3), rows(3), [4, -1, 0]), ValueError),
+                       (lambda: c.append(rows(40), rows(40), [0, 20, 20]), RuntimeError),
+                       (lambda: c.attention_forward(torch.zeros((2, 8, 64))), ValueError),
+                       (lambda: c.attention_forward(torch.zeros((3, 8, 64)), sparse_pages=1), ValueError),
+                       (lambda: c.prompt_attention(2, torch.zeros((6, 8, 64))), ValueError)):
+        with pytest.raises(error):
+            bad()
+    assert c.free_pages == 1 and c.num_tokens == [17, 1, 5] and c.lens.tolist() == [17, 1, 5]
+    c.release(0)
+    assert c.free_pages == 3 and c.num_tokens == [0, 1, 5] and c.table[0].tolist() == [-1] * 4
+    assert c.lens.tolist() == [0, 1, 5]
+    use = c.memory_usage_bytes()
+    assert use["in_use"] * 5 == use["pool"] * 2 > 0
+
+
+def test_reference_quantiser_round_trip():
+    """The host restatement itself: a value comes back within half a code step."""
+    from tests.paged_reference import quantise
+
+    g = torch.Generator().manual_seed(3)
+    x = (torch.randn((50, 64), generator=g) * torch.rand((50, 1), generator=g) * 30).half()
+    x[7] = 0
+    for dtype, step in ((torch.int8, None), (torch.float8_e4m3fn, 2.0 ** -4)):
+        codes, scale = quantise(x, dtype)
+        back = codes.float() * scale[:, None]
+        half = scale[:, None] * 0.5 if step is None else torch.maximum(x.float().abs() * step, scale[:, None] * 2.0 ** -10)
+        assert ((back - x.float()).abs() <= half * (1 + 1e-5)).all()
+        assert (codes[7].float() == 0).all() and scale[7] == 0
