@@ -16,7 +16,7 @@ int paged_check(const rfsn_paged* p, const char* what) {
   RFSN_REQUIRE(p->kv_heads > 0 && p->kv_heads <= 65535, w + ": kv_heads out of range");
   RFSN_REQUIRE(p->batch >= 0 && p->batch <= 65535, w + ": batch out of range");
   RFSN_REQUIRE(p->pages > 0, w + ": the pool has no pages");
-  RFSN_REQUIRE(p->table_width >= 0 && (int64_t)p->table_width * p->page_size < (1ll << 31),
+  RFSN_REQUIRE(p->table_width >= 0 && (int64_t)p->table_width * p->page_size <= (1ll << 31) - 1024,
                w + ": the table's positions must stay below 2^31");
   RFSN_REQUIRE(p->table_width == 0 || p->batch == 0 || p->table != nullptr, w + ": null table");
   RFSN_REQUIRE(p->batch == 0 || p->lens != nullptr, w + ": null lens");

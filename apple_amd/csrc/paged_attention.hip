@@ -146,16 +146,111 @@ __device__ __forceinline__ void attend_row(const rfsn_paged& p, int shift, const
   }
 }
 
+// ---- tiles on the matrix cores
+//
+// A wave takes 32 positions at a time (two groups of 16, each inside one page), a
+// block's waves take them in turn, and a lane's 16 columns are the query heads of the KV
+// head (the others repeat the last: the matrix cores are idle otherwise).
+//   S = K Q^T      MFMA 16x16x32, A = 16 rows of K as they lie in memory (16 bytes a
+//                  lane, the coordinates of Q in the same order), so K goes from
+//                  memory to its operand without LDS; a lane holds 8 scores of one head;
+//   O^T += V^T P^T with the weights' registers as the B operand as they are: k slot
+//                  (lane group g, j) is position 16 (j >> 2) + 4 g + (j & 3).  V passes
+//                  through LDS of the wave's own, and ds_read_b64_tr_b16 reads V^T from it
+//                  in that order.
+// Weights are kept to 2^-22 of themselves (fp16 pages: p 2^8 as fp16 hi + lo) or 2^-16
+// (8-bit pages: p times the row's scale as bf16 hi + lo, which has fp32's range; codes
+// are exact in bf16).  Scores, maxima, sums and O are fp32.
+// Where V or a score is infinite or NaN, hi, lo and weights of 0 meet it apart; a block that
+// finds a sum that is not finite takes its chunk again by attend_row.
+
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef _Float16 half2w __attribute__((ext_vector_type(2)));
+typedef _Float16 half4w __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short short4w __attribute__((ext_vector_type(4)));
+typedef short short8w __attribute__((ext_vector_type(8)));
+
+constexpr int kTile = 32;          // positions per wave and step
+constexpr int kWaves = 4;
+constexpr float kPBias = 8.f;      // a weight is kept as p 2^8
+constexpr float kPSum = 32768.f;   // a lane's sum below it: every weight is finite in fp16
+
+// 16-byte chunk c of row t of the [32][D] 16-bit tile sits at chunk c ^ v_swz(t): the
+// transposed reads take 32 bytes of 8 rows at once, which then lie in different banks.
+template <int D>
+__device__ __forceinline__ int v_swz(int t) { return D == 64 ? ((t >> 1) & 3) << 1 : (t & 7) << 1; }
+
+// 8 codes as fp16 (exact).
+template <int TYPE>
+__device__ __forceinline__ half8v codes_f16(uint32_t a, uint32_t b) {
+  half8v r;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const uint32_t c = w ? b : a;
+    half2w lo, hi;
+    if constexpr (TYPE == RFSN_PAGE_INT8) {
+      const uint32_t u = c ^ 0x80808080u;  // code + 128 as the low bits of 1024 + code + 128
+      lo = __builtin_bit_cast(half2w, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - (f16)1152.f;
+      hi = __builtin_bit_cast(half2w, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - (f16)1152.f;
+    } else {
+      lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.f, false);
+      hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.f, true);
+    }
+    r[4 * w] = lo[0], r[4 * w + 1] = lo[1], r[4 * w + 2] = hi[0], r[4 * w + 3] = hi[1];
+  }
+  return r;
+}
+
+// 8 codes as bf16 (exact), packed.
+template <int TYPE>
+__device__ __forceinline__ uint4w codes_bf16(uint32_t a, uint32_t b) {
+  uint4w r;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const uint32_t c = w ? b : a;
+    float f[4];
+    if constexpr (TYPE == RFSN_PAGE_INT8) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = (float)(int8_t)(c >> (8 * e));
+    } else {
+      f[0] = __builtin_amdgcn_cvt_f32_fp8((int)c, 0);
+      f[1] = __builtin_amdgcn_cvt_f32_fp8((int)c, 1);
+      f[2] = __builtin_amdgcn_cvt_f32_fp8((int)c, 2);
+      f[3] = __builtin_amdgcn_cvt_f32_fp8((int)c, 3);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)  // the high halves
+      r[2 * w + e] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, f[2 * e + 1]),
+                                           __builtin_bit_cast(uint32_t, f[2 * e]), 0x07060302u);
+  }
+  return r;
+}
+
 // per_seq > 0: every sequence has that many chunks of chunk_fixed listed
 // positions (a list of pages, or one chunk); 0: cut by the lengths.
 template <int D, int TYPE>
-__global__ void __launch_bounds__(256)
-paged_attn_kernel(const rfsn_paged p, int shift, const uint16_t* __restrict__ q, int G, float scale_log2,
-                  const int32_t* __restrict__ chosen, int count, int per_seq, int64_t chunk_fixed, int target,
-                  uint16_t* __restrict__ out, float* __restrict__ part_acc, float* __restrict__ part_ml) {
+__global__ void __launch_bounds__(kWaves * 64, D == 64 ? 4 : D == 128 ? 2 : 1)
+paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ table, const uint16_t* __restrict__ q, int G,
+                  float scale_log2, const int32_t* __restrict__ chosen, int count, int per_seq, int64_t chunk_fixed,
+                  int target, uint16_t* __restrict__ out, float* __restrict__ part_acc, float* __restrict__ part_ml) {
+  constexpr bool kCodes = TYPE != RFSN_PAGE_FP16;
   constexpr int E = D / 64;
+  constexpr int ES = kCodes ? 1 : 2;                 // bytes of a stored value
+  constexpr int KS = D / 32;                         // MFMA k steps of a score
+  constexpr int KL = D * ES / 64;                    // 16-byte loads of a lane's share of a K row
+  constexpr int DT = D / 16;                         // 16-coordinate tiles of O^T
+  constexpr int VC = D * ES / 16;                    // 16-byte chunks of a stored row
+  constexpr int VL = kTile * VC / 64;                // V loads of a lane
+  constexpr int CH = D / 8;                          // 16-byte chunks of a row in LDS
+  __shared__ uint4w smem[kWaves * kTile * CH];       // V tiles; then the waves' O, m, l
+  __shared__ float s_ml[kWaves][2][16];
+  __shared__ int s_odd[kWaves];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = blockIdx.x, w = blockIdx.y;
+  const int col = lane & 15, grp = lane >> 4;
+  const int h = blockIdx.x, w = blockIdx.y, g0 = blockIdx.z * 16;
+  const int heads = G - g0 < 16 ? G - g0 : 16;
   Chunk c;
   if (per_seq) {
     c.b = w / per_seq;
@@ -166,19 +261,249 @@ paged_attn_kernel(const rfsn_paged p, int shift, const uint16_t* __restrict__ q,
     c = find_chunk(p, shift, chunk_size(p, shift, target, lane), w, lane);
     if (c.b < 0) return;
   }
-  const int32_t* list = chosen ? chosen + ((int64_t)c.b * p.kv_heads + h) * count : nullptr;
-  for (int g = wave; g < G; g += 4) {
-    const int64_t row = ((int64_t)c.b * p.kv_heads + h) * G + g;
-    float m, l, acc[E];
-    attend_row<D, TYPE>(p, shift, list, c.b, h, c.t0, c.t1, q + row * D, scale_log2, lane, m, l, acc);
+  c.b = __builtin_amdgcn_readfirstlane(c.b);
+  const int t0 = __builtin_amdgcn_readfirstlane((int)c.t0), t1 = __builtin_amdgcn_readfirstlane((int)c.t1);
+  const int len = __builtin_amdgcn_readfirstlane(paged_len(p, shift, c.b));
+  const int32_t* const list = chosen ? chosen + ((int64_t)c.b * p.kv_heads + h) * count : nullptr;
+  const int32_t* const pages = table + (int64_t)c.b * p.table_stride;
+  const int64_t row0 = ((int64_t)c.b * p.kv_heads + h) * G + g0;  // of q and out
+
+  half8v qf[KS];
+  {
+    const uint16_t* qr = q + (row0 + (col < heads ? col : heads - 1)) * D;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      qf[s] = *reinterpret_cast<const half8v*>(qr + (kCodes ? (s >> 1) * 64 + grp * 16 + (s & 1) * 8 : s * 32 + grp * 8));
+  }
+  float4v o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d) o[d] = float4v{0.f, 0.f, 0.f, 0.f};
+  float m_run = -__builtin_inff(), l_run = 0.f;  // reference exponent of the head's weights, this lane's sum of them
+
+  uint4w kr[2][KL], vr[VL];
+  float4v ks[2], vs[2];
+  int n_next[2] = {0, 0};  // rows of the fetched groups that are attended
+  // Rows past the last one attended re-read it: their weights are 0.  A group with none
+  // reads page 0, and its V is not used.
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int tu = t + 16 * u;
+      int n = t1 - tu, page = 0, row = tu & (p.page_size - 1);
+      if (n > 0) {
+        int ord = tu >> shift;
+        if (list) {
+          ord = list[ord];
+          const int64_t left = (int64_t)len - (((int64_t)ord << shift) + row);
+          n = ord < 0 || left <= 0 ? 0 : left < 16 ? (int)left : 16;
+        }
+        if (n > 0 && ord < p.table_width) {
+          page = pages[ord];
+          if (page < 0 || page >= p.pages) n = 0;
+        } else {
+          n = 0;
+        }
+      }
+      n = n < 0 ? 0 : n > 16 ? 16 : n;
+      if (n == 0) page = 0;
+      page = __builtin_amdgcn_readfirstlane(page);
+      n = __builtin_amdgcn_readfirstlane(n);
+      n_next[u] = n;
+      const int last = n > 0 ? n - 1 : 0;
+      const int64_t base = ((int64_t)page * p.page_stride + (int64_t)h * p.head_stride + (int64_t)row * D) * ES;
+      const uint8_t* kb = (const uint8_t*)p.k + base;
+      const uint8_t* vb = (const uint8_t*)p.v + base;
+      const int kl = min(col, last) * (D * ES) + grp * 16;
+#pragma unroll
+      for (int i = 0; i < KL; ++i) kr[u][i] = *reinterpret_cast<const uint4w*>(kb + kl + i * 64);
+#pragma unroll
+      for (int i = 0; i < VL / 2; ++i) {
+        const int idx = i * 64 + lane, r = idx / VC, ch = idx % VC;
+        vr[u * (VL / 2) + i] = *reinterpret_cast<const uint4w*>(vb + min(r, last) * (D * ES) + ch * 16);
+      }
+      if constexpr (kCodes) {
+        const int64_t sc = ((int64_t)page * p.kv_heads + h) * p.page_size + row + grp * 4;
+        ks[u] = *reinterpret_cast<const float4v*>(p.k_scale + sc);
+        vs[u] = *reinterpret_cast<const float4v*>(p.v_scale + sc);
+      }
+    }
+  };
+  uint4w* const sv = smem + wave * kTile * CH;
+  const int step = kWaves * kTile;
+  int t = t0 + wave * kTile;
+  if (t < t1) fetch(t);
+  for (; t < t1; t += step) {
+    int n[2] = {n_next[0], n_next[1]};
+    // V to LDS
+#pragma unroll
+    for (int i = 0; i < VL; ++i) {
+      const int idx = (i % (VL / 2)) * 64 + lane, r = (i / (VL / 2)) * 16 + idx / VC, ch = idx % VC;
+      uint4w x = vr[i];
+      if (n[i / (VL / 2)] == 0) x = uint4w{0, 0, 0, 0};
+      if constexpr (!kCodes) {
+        sv[r * CH + (ch ^ v_swz<D>(r))] = x;
+      } else {
+        sv[r * CH + ((2 * ch) ^ v_swz<D>(r))] = codes_bf16<TYPE>(x[0], x[1]);
+        sv[r * CH + ((2 * ch + 1) ^ v_swz<D>(r))] = codes_bf16<TYPE>(x[2], x[3]);
+      }
+    }
+    // scores in base 2
+    float4v s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      s[u] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        half8v kf;
+        if constexpr (!kCodes) kf = __builtin_bit_cast(half8v, kr[u][k]);
+        else kf = codes_f16<TYPE>(kr[u][k >> 1][2 * (k & 1)], kr[u][k >> 1][2 * (k & 1) + 1]);
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[k], s[u], 0, 0, 0);
+      }
+    }
+    float4v vscale[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if constexpr (kCodes) {
+        s[u] *= ks[u];
+        vscale[u] = vs[u];
+      }
+      s[u] *= scale_log2;
+      if (n[u] < 16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (grp * 4 + i >= n[u]) {
+            s[u][i] = -__builtin_inff();
+            if constexpr (kCodes) vscale[u][i] = 0.f;
+          }
+        }
+      }
+    }
+    if (t + step < t1) fetch(t + step);
+    float pw[8], ls;
+    auto weights = [&]() {
+      const float mb = m_run > -__builtin_inff() ? m_run : 0.f;
+      ls = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        pw[i] = __builtin_amdgcn_exp2f(s[i >> 2][i & 3] - mb);
+        ls += pw[i];
+      }
+    };
+    weights();
+    // The maximum is moved only when a lane's sum says that a weight may leave
+    // fp16's range (or nothing was seen yet): no weight exceeds the sum.
+    if (__any(!(ls < kPSum) || m_run == -__builtin_inff())) {
+      float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float m_new = fmaxf(m_run, mx - kPBias);
+      const float corr = m_run > -__builtin_inff() ? __builtin_amdgcn_exp2f(m_run - m_new) : 0.f;
+      l_run *= corr;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= corr;
+      m_run = m_new;
+      weights();
+    }
+    l_run += ls;
+    uint4w bh, bl;  // 8 weights as the B operand, high and low parts
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (!kCodes) {
+        const half2w hi = {(f16)pw[2 * i], (f16)pw[2 * i + 1]};
+        const half2w lo = {(f16)(pw[2 * i] - (float)hi[0]), (f16)(pw[2 * i + 1] - (float)hi[1])};
+        bh[i] = __builtin_bit_cast(uint32_t, hi), bl[i] = __builtin_bit_cast(uint32_t, lo);
+      } else {
+        const float a = pw[2 * i] * vscale[i >> 1][(2 * i) & 3], b = pw[2 * i + 1] * vscale[i >> 1][(2 * i + 1) & 3];
+        const bf16x2 hi = {(__bf16)a, (__bf16)b};
+        const bf16x2 lo = {(__bf16)(a - (float)hi[0]), (__bf16)(b - (float)hi[1])};
+        bh[i] = __builtin_bit_cast(uint32_t, hi), bl[i] = __builtin_bit_cast(uint32_t, lo);
+      }
+    }
+    // the tile was written by all lanes of this wave: LDS keeps a wave's order, the compiler has to as well
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      typedef __attribute__((address_space(3))) short4w lds4;
+      short4w a[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int tv = 16 * e + 4 * grp + (col >> 2), cc = 2 * d + ((col & 3) >> 1);
+        const int off = (tv * CH + (cc ^ v_swz<D>(tv))) * 16 + (col & 1) * 8;
+        a[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)((__attribute__((address_space(3))) char*)sv + off));
+      }
+      const short8w av = {a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]};
+      if constexpr (!kCodes) {
+        const half8v vf = __builtin_bit_cast(half8v, av);
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_bit_cast(half8v, bh), o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_bit_cast(half8v, bl), o[d], 0, 0, 0);
+      } else {
+        const bf16x8 vf = __builtin_bit_cast(bf16x8, av);
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8, bh), o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8, bl), o[d], 0, 0, 0);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+  }
+
+  float zero = l_run * 0.f;  // NaN where a sum is infinite or NaN
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) zero = fmaf(o[d][i], 0.f, zero);
+  const int odd = __any(zero != 0.f);
+  l_run += __shfl_xor(l_run, 16, 64);
+  l_run += __shfl_xor(l_run, 32, 64);
+  float* const so = reinterpret_cast<float*>(smem);
+  if (lane == 0) s_odd[wave] = odd;
+  if (grp == 0) s_ml[wave][0][col] = m_run, s_ml[wave][1][col] = l_run;
+  // the waves' V tiles are done with: each wave's O lies over its own
+#pragma unroll
+  for (int d = 0; d < DT; ++d) *reinterpret_cast<float4v*>(so + ((wave * DT + d) * 64 + lane) * 4) = o[d];
+  __syncthreads();
+  if (s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3]) {  // block-uniform: the chunk again, a head at a time
+    for (int g = wave; g < heads; g += kWaves) {
+      const int64_t row = row0 + g;
+      float m, l, acc[E];
+      attend_row<D, TYPE>(p, shift, list, c.b, h, c.t0, c.t1, q + row * D, scale_log2, lane, m, l, acc);
+      if (part_ml == nullptr) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) out[row * D + lane * E + e] = f2h(l == 0.f ? 0.f : acc[e] / l);
+      } else {
+        const int64_t slot = ((int64_t)w * p.kv_heads + h) * G + g0 + g;
+        if (lane == 0) part_ml[2 * slot] = m, part_ml[2 * slot + 1] = l;
+#pragma unroll
+        for (int e = 0; e < E; ++e) part_acc[slot * D + lane * E + e] = acc[e];
+      }
+    }
+    return;
+  }
+  float m = s_ml[0][0][col], f[kWaves], l = 0.f;
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) m = fmaxf(m, s_ml[i][0][col]);
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    const float mi = s_ml[i][0][col];
+    f[i] = mi > -__builtin_inff() ? __builtin_amdgcn_exp2f(mi - m) : 0.f;
+    l += f[i] * s_ml[i][1][col];
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const int64_t slot = ((int64_t)w * p.kv_heads + h) * G + g0 + col;
+  if (part_ml != nullptr && wave == 0 && grp == 0 && col < heads) part_ml[2 * slot] = m, part_ml[2 * slot + 1] = l;
+#pragma unroll
+  for (int i = 0; i < DT / kWaves; ++i) {
+    const int d = i * kWaves + wave;
+    float4v a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < kWaves; ++x) a += f[x] * *reinterpret_cast<const float4v*>(so + ((x * DT + d) * 64 + lane) * 4);
+    if (col >= heads) continue;
     if (part_ml == nullptr) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) out[row * D + lane * E + e] = f2h(l == 0.f ? 0.f : acc[e] / l);
+      const half4w r = {(f16)(a[0] * inv), (f16)(a[1] * inv), (f16)(a[2] * inv), (f16)(a[3] * inv)};
+      *reinterpret_cast<half4w*>(out + (row0 + col) * D + d * 16 + grp * 4) = r;
     } else {
-      const int64_t slot = ((int64_t)w * p.kv_heads + h) * G + g;
-      if (lane == 0) part_ml[2 * slot] = m, part_ml[2 * slot + 1] = l;
-#pragma unroll
-      for (int e = 0; e < E; ++e) part_acc[slot * D + lane * E + e] = acc[e];
+      *reinterpret_cast<float4v*>(part_acc + slot * D + d * 16 + grp * 4) = a;
     }
   }
 }
@@ -234,9 +559,9 @@ struct Plan {
   int target;
   bool split() const { return per_seq != 1; }
 };
-Plan plan(const rfsn_paged& p, int count) {
+Plan plan(const rfsn_paged& p, int q_heads, int count) {
   const int64_t most = (int64_t)(count ? count : p.table_width) * p.page_size;
-  const int64_t want = ceil_div(kBlocks, p.kv_heads);  // chunks that fill the chip
+  const int64_t want = ceil_div(kBlocks, p.kv_heads * ceil_div(q_heads / p.kv_heads, 16));  // chunks that fill the chip
   if (most <= kMinChunk) return {p.batch, 1, kMinChunk, 0};
   if (count) {
     int64_t n = ceil_div(want, p.batch);
@@ -256,8 +581,8 @@ Plan plan(const rfsn_paged& p, int count) {
 using namespace rfsn;
 
 extern "C" size_t rfsn_paged_attention_workspace_bytes(const rfsn_paged* p, int32_t q_heads, int32_t count) {
-  if (p == nullptr || p->batch <= 0 || p->kv_heads <= 0 || p->page_size <= 0 || q_heads <= 0 || count < 0) return 0;
-  const Plan c = plan(*p, count);
+  if (p == nullptr || p->batch <= 0 || p->kv_heads <= 0 || p->page_size <= 0 || q_heads < p->kv_heads || count < 0) return 0;
+  const Plan c = plan(*p, q_heads, count);
   return c.split() ? (size_t)c.slots * q_heads * (p->head_dim + 2) * sizeof(float) : 0;
 }
 
@@ -268,13 +593,13 @@ extern "C" int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t 
   RFSN_REQUIRE(q_heads > 0 && q_heads % p->kv_heads == 0 && q_heads <= 65535,
                "paged_attention: q_heads must be a multiple of kv_heads");
   RFSN_REQUIRE((chosen == nullptr) == (count == 0) && count >= 0, "paged_attention: chosen and count go together");
-  RFSN_REQUIRE((int64_t)count * p->page_size < (1ll << 31), "paged_attention: too many chosen pages");
+  RFSN_REQUIRE((int64_t)count * p->page_size <= (1ll << 31) - 1024, "paged_attention: too many chosen pages");
   RFSN_REQUIRE(scale == scale && scale < __builtin_inff() && scale > -__builtin_inff(),
                "paged_attention: scale must be finite");
   if (p->batch == 0) return RFSN_OK;
   RFSN_REQUIRE(q && out && ((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 15) == 0,
                "paged_attention: q and out must be 16-byte aligned");
-  const Plan c = plan(*p, count);
+  const Plan c = plan(*p, q_heads, count);
   RFSN_REQUIRE(workspace_bytes >= rfsn_paged_attention_workspace_bytes(p, q_heads, count) && (workspace || !c.split()),
                "paged_attention: workspace too small");
   RFSN_REQUIRE(c.slots <= 65535, "paged_attention: too many sequences");
@@ -284,8 +609,8 @@ extern "C" int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t 
   float* acc = c.split() ? (float*)workspace : nullptr;
   float* ml = c.split() ? acc + c.slots * q_heads * p->head_dim : nullptr;
 #define RFSN_ATTEND(DD, TT)                                                                                            \
-  hipLaunchKernelGGL((paged_attn_kernel<DD, TT>), dim3((unsigned)p->kv_heads, (unsigned)c.slots), dim3(256), 0, s, *p, \
-                     shift, (const uint16_t*)q, G, sl2, chosen, count, c.per_seq, c.chunk, c.target, (uint16_t*)out,   \
+  hipLaunchKernelGGL((paged_attn_kernel<DD, TT>), dim3((unsigned)p->kv_heads, (unsigned)c.slots, (unsigned)ceil_div(G, 16)), \
+                     dim3(kWaves * 64), 0, s, *p, shift, p->table, (const uint16_t*)q, G, sl2, chosen, count, c.per_seq, c.chunk, c.target, (uint16_t*)out,   \
                      acc, ml)
 #define RFSN_ATTEND_D(DD)                                            \
   do {                                                               \
