@@ -137,12 +137,13 @@ SIGNATURES = {
     "rfsn_fused_workspace_bytes": (sz, [C.POINTER(FusedParams)]),
     "rfsn_fused_decode_attention": (i32, [C.POINTER(FusedParams), vp]),
     "rfsn_fused_decode_attention_noalloc": (i32, [C.POINTER(FusedParams), vp]),
-    "rfsn_paged_append": (i32, [C.POINTER(Paged), vp, vp, i64, i64, i64, vp, vp]),
-    "rfsn_paged_read": (i32, [C.POINTER(Paged), vp, i64, vp, vp, i32, vp]),
+    # the paged calls take their parameter block by address or as packed bytes
+    "rfsn_paged_append": (i32, [vp, vp, vp, i64, i64, i64, vp, vp]),
+    "rfsn_paged_read": (i32, [vp, vp, i64, vp, vp, i32, vp]),
     "rfsn_page_select_workspace_bytes": (sz, [C.POINTER(Paged)]),
-    "rfsn_page_select": (i32, [C.POINTER(Paged), vp, i32, i32, i32, i32, vp, vp, sz, vp]),
+    "rfsn_page_select": (i32, [vp, vp, i32, i32, i32, i32, vp, vp, sz, vp]),
     "rfsn_paged_attention_workspace_bytes": (sz, [C.POINTER(Paged), i32, i32]),
-    "rfsn_paged_attention": (i32, [C.POINTER(Paged), vp, i32, f32, vp, i32, vp, vp, sz, vp]),
+    "rfsn_paged_attention": (i32, [vp, vp, i32, f32, vp, i32, vp, vp, sz, vp]),
     "rfsn_kmeans_workspace_bytes": (sz, [i32, i32, i32]),
     "rfsn_kmeans_update": (i32, [vp, i64, i32, i64, vp, i32, i32, vp, vp, sz, vp]),
     "rfsn_host_alloc": (i32, [sz, C.POINTER(vp)]),

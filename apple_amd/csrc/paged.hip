@@ -229,117 +229,204 @@ paged_read_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ cu,
 
 // ---------------------------------------------------------------- page choice
 
-// Score of every page held by (sequence, KV head): a lane takes 8 coordinates
-// of a page's bounds, D / 8 lanes a page.  Products of fp16 values are exact in
-// fp32, and of q+ hi and q- lo one is zero; sums are held in 64 bits.
+// x + the value of the lane that `ctrl` (a DPP pattern) names.
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, CTRL, 15, 15, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, 15, 15, true);
+  return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// Sum over groups of 8, 16 or 32 lanes: lanes ^ 1, ^ 2, then mirrored halves of 8 and rows of 16.
+template <int LANES>
+__device__ __forceinline__ double group_sum(double x) {
+  x = dpp_add<0xb1>(x);   // quad_perm 1,0,3,2
+  x = dpp_add<0x4e>(x);   // quad_perm 2,3,0,1
+  x = dpp_add<0x141>(x);  // row_half_mirror
+  if constexpr (LANES >= 16) x = dpp_add<0x140>(x);  // row_mirror
+  if constexpr (LANES >= 32) x += __shfl_xor(x, 16, 64);
+  return x;
+}
+
+// Score of every page held by (sequence, KV head): a lane takes 8 coordinates of a page's
+// bounds, D / 8 lanes a page, a wave kScoreSets sets of pages, whose loads are all in
+// flight together.  Products of fp16 values are exact in fp32, and of q+ hi and q- lo one
+// is zero; sums are held in 64 bits.
+constexpr int kScoreSets = 4;
 template <int D>
 __global__ void __launch_bounds__(256)
 page_score_kernel(const rfsn_paged p, int shift, const uint16_t* __restrict__ q, int G, float* __restrict__ score) {
-  constexpr int LANES = D / 8, RS = 64 / LANES;
+  constexpr int LANES = D / 8, RS = 64 / LANES, U = kScoreSets;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int h = blockIdx.y, b = blockIdx.z;
   const int slot = lane / LANES, chunk = lane % LANES;
   const int held = (int)(((int64_t)paged_len(p, shift, b) + p.page_size - 1) >> shift);
-  const int n = (blockIdx.x * 4 + wave) * RS + slot;
-  const int page = n < held ? paged_page(p, b, n) : -1;
-  half8v lo = {}, hi = {};
-  if (page >= 0) {
-    const half8v* bp =
-        reinterpret_cast<const half8v*>((const uint16_t*)p.bounds + ((int64_t)page * p.kv_heads + h) * 2 * D + chunk * 8);
-    lo = bp[0], hi = bp[D / 8];
+  const int n0 = (blockIdx.x * 4 + wave) * (RS * U) + slot;
+  if (n0 - slot >= held) return;
+  int page[U];
+  half8v lo[U], hi[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) page[u] = n0 + u * RS < held ? paged_page(p, b, n0 + u * RS) : -1;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const half8v* bp = reinterpret_cast<const half8v*>(
+        (const uint16_t*)p.bounds + ((int64_t)max(page[u], 0) * p.kv_heads + h) * 2 * D + chunk * 8);
+    lo[u] = bp[0], hi[u] = bp[D / 8];
   }
-  double best = -__builtin_inf();
-  bool nan = false;
+  double best[U];
+  bool nan[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) best[u] = -__builtin_inf(), nan[u] = false;
+#pragma unroll 1
   for (int g = 0; g < G; ++g) {
     const half8v qv = *reinterpret_cast<const half8v*>(q + (((int64_t)b * p.kv_heads + h) * G + g) * D + chunk * 8);
-    double s = 0.0;
+    float up[8], down[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float x = (float)qv[e];
-      const float up = x < 0.f ? 0.f : x, down = x > 0.f ? 0.f : x;
-      s += (double)fmaf(up, (float)hi[e], down * (float)lo[e]);
+      up[e] = x < 0.f ? 0.f : x, down[e] = x > 0.f ? 0.f : x;
     }
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    nan |= s != s;
-    best = s > best ? s : best;
+    for (int u = 0; u < U; ++u) {
+      double s = 0.0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += (double)fmaf(up[e], (float)hi[u][e], down[e] * (float)lo[u][e]);
+      s = group_sum<LANES>(s);
+      nan[u] |= s != s;
+      best[u] = s > best[u] ? s : best[u];
+    }
   }
-  if (n < held && chunk == 0)
-    score[((int64_t)b * p.kv_heads + h) * p.table_width + n] =
-        page < 0 ? -__builtin_inff() : nan ? __builtin_nanf("") : (float)best;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int n = n0 + u * RS;
+    if (n < held && chunk == 0)
+      score[((int64_t)b * p.kv_heads + h) * p.table_width + n] =
+          page[u] < 0 ? -__builtin_inff() : nan[u] ? __builtin_nanf("") : (float)best[u];
+  }
 }
 
-// Order of the scores as unsigned keys: kept pages over all, NaN as +infinity, -0 as +0.
-__device__ __forceinline__ uint32_t page_key(float s, int n, int held, int first, int last) {
-  if (n < first || n >= held - last) return 0xffffffffu;
+// Order of the scores as unsigned keys: NaN as +infinity, -0 as +0.
+__device__ __forceinline__ uint32_t page_key(float s) {
   if (s != s) s = __builtin_inff();
   const uint32_t u = __builtin_bit_cast(uint32_t, s + 0.f);
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// The count largest keys of a row, their indices ascending: the count-th
-// largest key by four passes over 8 bits, then one pass that keeps what is above
-// it and, in order, as many equal to it as there is room for.
-__global__ void __launch_bounds__(256)
+// The pages of a row's largest keys besides the kept ones, all in ascending order.  A block a row.
+// The smallest key to keep is found by narrowing [lo, hi], at first the smallest and largest key: a histogram of
+// 2,048 equal parts of it says which part holds the key wanted.  Scores share their exponent mostly, so parts
+// of their range spread over the counters where their leading bits would meet in one; two rounds are the rule,
+// three the most.  Then each of 16 waves counts what it keeps of its own run of pages and writes it
+// behind the waves before it.  Keys past the LDS copy are read again from the scores.
+constexpr int kChooseWaves = 16, kChooseBins = 2048, kChooseKeys = 8192;
+__global__ void __launch_bounds__(kChooseWaves * 64)
 page_choose_kernel(const rfsn_paged p, int shift, const float* __restrict__ score, int count, int first, int last,
                    int32_t* __restrict__ chosen) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t s_digit, s_left, s_part[2][4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int T = kChooseWaves * 64, PER = kChooseBins / T;
+  __shared__ uint32_t s_key[kChooseKeys];
+  __shared__ uint32_t hist[kChooseBins];
+  __shared__ uint32_t s_wave[2][kChooseWaves], s_found[3];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = blockIdx.x, b = blockIdx.y;
   const int64_t row = (int64_t)b * p.kv_heads + h;
   const float* s = score + row * p.table_width;
   int32_t* out = chosen + row * count;
   const int held = (int)(((int64_t)paged_len(p, shift, b) + p.page_size - 1) >> shift);
   if (held <= count) {
-    for (int i = tid; i < count; i += 256) out[i] = i < held ? i : -1;
+    for (int i = tid; i < count; i += T) out[i] = i < held ? i : -1;
     return;
   }
-  uint32_t prefix = 0, mask = 0;
-  uint32_t left = (uint32_t)count;  // of the keys that share the prefix, how many are kept
-  for (int at = 24; at >= 0; at -= 8) {
-    hist[tid] = 0;
+  // held > count >= first + last: the kept pages are apart, the others lie between them
+  const int begin = first, end = held - last;
+  uint32_t left = (uint32_t)(count - first - last);
+  auto key = [&](int n) { return n - begin < kChooseKeys ? s_key[n - begin] : page_key(s[n]); };
+  uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll 4
+  for (int n = begin + tid; n < end; n += T) {
+    const uint32_t k = page_key(s[n]);
+    if (n - begin < kChooseKeys) s_key[n - begin] = k;
+    lo = min(lo, k), hi = max(hi, k);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) lo = min(lo, (uint32_t)__shfl_xor((int)lo, o, 64)), hi = max(hi, (uint32_t)__shfl_xor((int)hi, o, 64));
+  if (lane == 0) s_wave[0][wave] = lo, s_wave[1][wave] = hi;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kChooseWaves; ++w) lo = min(lo, s_wave[0][w]), hi = max(hi, s_wave[1][w]);
+  __syncthreads();  // s_wave is written again
+  uint32_t over = 0xffffffffu, tie = 0xffffffffu;  // keys from `over` on are kept, and `left` of those equal to `tie`
+  while (left > 0) {
+    if (lo == hi) {
+      over = lo + 1, tie = lo;
+      break;
+    }
+    const int bits = 32 - __builtin_clz(hi - lo), sh = bits > 11 ? bits - 11 : 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) hist[tid + i * T] = 0;
     __syncthreads();
-    for (int n = tid; n < held; n += 256) {
-      const uint32_t key = page_key(s[n], n, held, first, last);
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> at) & 255u], 1u);
+    for (int n = begin + tid; n < end; n += T) {
+      const uint32_t k = key(n);
+      if (k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> sh], 1u);
     }
     __syncthreads();
-    // thread i: how many keys have a digit above i
-    uint32_t above = 0;
-    for (int i = tid + 1; i < 256; ++i) above += hist[i];
-    if (above < left && above + hist[tid] >= left) s_digit = (uint32_t)tid, s_left = left - above;
+    // keys in the parts above each thread's PER parts, from the top down
+    uint32_t c[PER], mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mine += c[i] = hist[kChooseBins - 1 - (tid * PER + i)];
+    uint32_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t x = (uint32_t)__shfl_up((int)upto, o, 64);
+      if (lane >= o) upto += x;
+    }
+    if (lane == 63) s_wave[0][wave] = upto;
     __syncthreads();
-    prefix |= s_digit << at;
-    mask |= 255u << at;
-    left = s_left;
+    uint32_t above = upto - mine;
+    for (int w = 0; w < wave; ++w) above += s_wave[0][w];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (above < left && above + c[i] >= left) {
+        s_found[0] = (uint32_t)(kChooseBins - 1 - (tid * PER + i));
+        s_found[1] = left - above;
+        s_found[2] = c[i];
+      }
+      above += c[i];
+    }
+    __syncthreads();
+    lo += s_found[0] << sh;
+    hi = min(hi, lo + ((1u << sh) - 1u));
+    left = s_found[1];
+    if (s_found[2] == left) {  // the whole part
+      over = lo, left = 0;
+    }
+    // s_found and hist are written again behind the next barriers
     __syncthreads();
   }
-  uint32_t done = 0, ties = 0;  // written so far; equal keys seen so far
-  for (int base = 0; base < held; base += 256) {
-    const int n = base + tid;
-    const uint32_t key = n < held ? page_key(s[n], n, held, first, last) : 0u;
-    const bool over = n < held && key > prefix, tie = n < held && key == prefix;
-    const uint64_t bt = __ballot(tie), below = (1ull << lane) - 1;
-    if (lane == 0) s_part[0][wave] = (uint32_t)__popcll(bt);
-    __syncthreads();
-    uint32_t before = ties, all = ties;
-    for (int w = 0; w < 4; ++w) {
-      if (w < wave) before += s_part[0][w];
-      all += s_part[0][w];
-    }
-    const bool keep = over || (tie && before + (uint32_t)__popcll(bt & below) < left);
+  const int seg = ((end - begin + kChooseWaves - 1) / kChooseWaves + 63) / 64 * 64;
+  const int n0 = begin + wave * seg, n1 = min(end, n0 + seg);
+  uint32_t kept = 0, ties = 0;
+  for (int n = n0 + lane; n - lane < n1; n += 64) {
+    const uint32_t k = n < n1 ? key(n) : 0;
+    kept += (uint32_t)__popcll(__ballot(n < n1 && k >= over));
+    ties += (uint32_t)__popcll(__ballot(n < n1 && left && k == tie));
+  }
+  if (lane == 0) s_wave[0][wave] = kept, s_wave[1][wave] = ties;
+  __syncthreads();
+  uint32_t at = (uint32_t)first, before = 0;
+  for (int w = 0; w < wave; ++w) at += s_wave[0][w], before += s_wave[1][w];
+  at += min(before, left);
+  const uint64_t below = (1ull << lane) - 1;
+  for (int n = n0 + lane; n - lane < n1; n += 64) {
+    const uint32_t k = n < n1 ? key(n) : 0;
+    const bool is_tie = n < n1 && left && k == tie;
+    const uint64_t bt = __ballot(is_tie);
+    const bool keep = (n < n1 && k >= over) || (is_tie && before + (uint32_t)__popcll(bt & below) < left);
     const uint64_t bk = __ballot(keep);
-    if (lane == 0) s_part[1][wave] = (uint32_t)__popcll(bk);
-    __syncthreads();
-    uint32_t at = done, total = done;
-    for (int w = 0; w < 4; ++w) {
-      if (w < wave) at += s_part[1][w];
-      total += s_part[1][w];
-    }
     if (keep) out[at + (uint32_t)__popcll(bk & below)] = n;
-    done = total, ties = all;
+    at += (uint32_t)__popcll(bk), before += (uint32_t)__popcll(bt);
   }
+  for (int i = tid; i < first; i += T) out[i] = i;
+  for (int i = tid; i < last; i += T) out[count - last + i] = end + i;
 }
 
 #define RFSN_PAGED_DISPATCH(D, TYPE, ...)                                                       \
@@ -419,7 +506,7 @@ extern "C" int rfsn_page_select(const rfsn_paged* p, const void* q, int32_t q_he
   const hipStream_t s = (hipStream_t)stream;
   const int G = q_heads / p->kv_heads;
   if (p->table_width > 0) {
-    const int per = 4 * (512 / p->head_dim);
+    const int per = 4 * kScoreSets * (512 / p->head_dim);
     const dim3 grid((unsigned)ceil_div(p->table_width, per), (unsigned)p->kv_heads, (unsigned)p->batch);
 #define RFSN_SCORE(DD) \
   hipLaunchKernelGGL(page_score_kernel<DD>, grid, dim3(256), 0, s, *p, shift, (const uint16_t*)q, G, (float*)workspace)
@@ -429,7 +516,7 @@ extern "C" int rfsn_page_select(const rfsn_paged* p, const void* q, int32_t q_he
 #undef RFSN_SCORE
     if (int st = check_launch("page_select")) return st;
   }
-  hipLaunchKernelGGL(page_choose_kernel, dim3((unsigned)p->kv_heads, (unsigned)p->batch), dim3(256), 0, s, *p, shift,
-                     (const float*)workspace, count, first, last, chosen);
+  hipLaunchKernelGGL(page_choose_kernel, dim3((unsigned)p->kv_heads, (unsigned)p->batch), dim3(kChooseWaves * 64), 0, s, *p,
+                     shift, (const float*)workspace, count, first, last, chosen);
   return check_launch("page_select");
 }

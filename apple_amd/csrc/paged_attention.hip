@@ -11,61 +11,59 @@
 namespace rfsn {
 namespace {
 
-constexpr int kUnit = 128;       // chunks are multiples of this many positions
-constexpr int kMinChunk = 512;   // and no shorter
-constexpr int kBlocks = 1024;    // blocks a launch aims at
-
 __device__ __forceinline__ int64_t wave_sum64(int64_t v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor((long long)v, o, 64);
   return v;
 }
 
-// Positions per chunk of a batch: at most `target` chunks over the sum of the
-// lengths, one more per sequence for its last, shorter one.
-__device__ __forceinline__ int64_t chunk_size(const rfsn_paged& p, int shift, int target, int lane) {
-  int64_t total = 0;
-  for (int b = lane; b < p.batch; b += 64) total += paged_len(p, shift, b);
-  total = wave_sum64(total);
-  int64_t c = (total + target - 1) / target;
-  c = (c + kUnit - 1) / kUnit * kUnit;
-  return c < kMinChunk ? kMinChunk : c;
-}
-
-// Chunks of the sequences before b.
-__device__ __forceinline__ int chunks_before(const rfsn_paged& p, int shift, int64_t size, int b, int lane) {
-  int64_t n = 0;
-  for (int i = lane; i < b; i += 64) n += (paged_len(p, shift, i) + size - 1) / size;
-  return (int)wave_sum64(n);
-}
+// How a call is cut (Plan, below): per_seq > 0 gives every sequence that many chunks of
+// `chunk` listed positions (a list of pages, or one chunk); 0 cuts by the lengths, into at
+// most `target` chunks of at least `chunk` positions over their sum and one more per sequence
+// for its last, shorter one.
+struct Cut {
+  int per_seq;
+  int target;
+  int64_t chunk;
+};
 
 struct Chunk {
   int b;       // sequence, -1: none
+  int j, n;    // number in the sequence, and of how many
   int64_t t0, t1;
 };
-// Chunk number w of the batch, by one wave.
-__device__ __forceinline__ Chunk find_chunk(const rfsn_paged& p, int shift, int64_t size, int w, int lane) {
+
+// Chunk number w of a batch that is cut by the lengths, by one wave.
+__device__ __forceinline__ Chunk find_chunk(const rfsn_paged& p, int shift, const Cut& cut, int w, int lane) {
+  const int len0 = lane < p.batch ? paged_len(p, shift, lane) : 0;  // of the first 64, which are most batches
+  int64_t total = len0;
+  for (int b = 64 + lane; b < p.batch; b += 64) total += paged_len(p, shift, b);
+  total = p.batch == 1 ? __builtin_amdgcn_readfirstlane(len0) : wave_sum64(total);
+  int64_t size = (total + cut.target - 1) / cut.target;
+  size = size <= cut.chunk ? cut.chunk : (size + 127) / 128 * 128;
   int seen = 0;
   for (int base = 0; base < p.batch; base += 64) {
     const int b = base + lane;
-    const int len = b < p.batch ? paged_len(p, shift, b) : 0;
+    const int len = base == 0 ? len0 : b < p.batch ? paged_len(p, shift, b) : 0;
     const int n = (int)((len + size - 1) / size);
     int upto = n;  // inclusive prefix over the wave
+    if (p.batch > 1) {
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(upto, o, 64);
-      if (lane >= o) upto += x;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(upto, o, 64);
+        if (lane >= o) upto += x;
+      }
     }
     const uint64_t in = __ballot(w < seen + upto && w >= seen + upto - n);
     if (in) {
       const int src = __ffsll((unsigned long long)in) - 1;
-      const int64_t t0 = (int64_t)(w - seen - __shfl(upto - n, src, 64)) * size;
-      const int64_t end = __shfl(len, src, 64);
-      return {base + src, t0, t0 + size < end ? t0 + size : end};
+      const int j = w - seen - __shfl(upto - n, src, 64);
+      const int64_t t0 = (int64_t)j * size, end = __shfl(len, src, 64);
+      return {base + src, j, __shfl(n, src, 64), t0, t0 + size < end ? t0 + size : end};
     }
     seen += __shfl(upto, 63, 64);
   }
-  return {-1, 0, 0};
+  return {-1, 0, 0, 0, 0};
 }
 
 // Where listed position t of (b, h) lies: t itself without a list, else row t %
@@ -173,7 +171,7 @@ typedef short short4w __attribute__((ext_vector_type(4)));
 typedef short short8w __attribute__((ext_vector_type(8)));
 
 constexpr int kTile = 32;          // positions per wave and step
-constexpr int kWaves = 4;
+constexpr int kWideTiles = 8192;   // tiles of a call up to which blocks have many waves
 constexpr float kPBias = 8.f;      // a weight is kept as p 2^8
 constexpr float kPSum = 32768.f;   // a lane's sum below it: every weight is finite in fp16
 
@@ -228,13 +226,19 @@ __device__ __forceinline__ uint4w codes_bf16(uint32_t a, uint32_t b) {
   return r;
 }
 
-// per_seq > 0: every sequence has that many chunks of chunk_fixed listed
-// positions (a list of pages, or one chunk); 0: cut by the lengths.
-template <int D, int TYPE>
-__global__ void __launch_bounds__(kWaves * 64, D == 64 ? 4 : D == 128 ? 2 : 1)
+// Partial results of a split call: (m, l) and O of each chunk and query head, and for each
+// sequence that has any its first chunk and their number.
+struct Parts {
+  float* acc;   // [slots][q_heads][D]
+  float* ml;    // [slots][q_heads][2]
+  int32_t* seq; // [batch][2]
+};
+
+template <int D, int TYPE, int kWaves>
+__global__ void __launch_bounds__(kWaves * 64, kWaves > 4 ? 1 : D == 64 ? 4 : D == 128 ? 2 : 1)
 paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ table, const uint16_t* __restrict__ q, int G,
-                  float scale_log2, const int32_t* __restrict__ chosen, int count, int per_seq, int64_t chunk_fixed,
-                  int target, uint16_t* __restrict__ out, float* __restrict__ part_acc, float* __restrict__ part_ml) {
+                  float scale_log2, const int32_t* __restrict__ chosen, int count, const Cut cut,
+                  uint16_t* __restrict__ out, const Parts parts) {
   constexpr bool kCodes = TYPE != RFSN_PAGE_FP16;
   constexpr int E = D / 64;
   constexpr int ES = kCodes ? 1 : 2;                 // bytes of a stored value
@@ -252,14 +256,15 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
   const int h = blockIdx.x, w = blockIdx.y, g0 = blockIdx.z * 16;
   const int heads = G - g0 < 16 ? G - g0 : 16;
   Chunk c;
-  if (per_seq) {
-    c.b = w / per_seq;
-    c.t0 = (int64_t)(w % per_seq) * chunk_fixed;
+  if (cut.per_seq) {
+    c.b = w / cut.per_seq;
+    c.t0 = (int64_t)(w % cut.per_seq) * cut.chunk;
     const int64_t end = chosen ? (int64_t)count << shift : paged_len(p, shift, c.b);
-    c.t1 = c.t0 + chunk_fixed < end ? c.t0 + chunk_fixed : end;
+    c.t1 = c.t0 + cut.chunk < end ? c.t0 + cut.chunk : end;
   } else {
-    c = find_chunk(p, shift, chunk_size(p, shift, target, lane), w, lane);
+    c = find_chunk(p, shift, cut, w, lane);
     if (c.b < 0) return;
+    if (c.j == 0 && h == 0 && g0 == 0 && threadIdx.x == 0) parts.seq[2 * c.b] = w, parts.seq[2 * c.b + 1] = c.n;
   }
   c.b = __builtin_amdgcn_readfirstlane(c.b);
   const int t0 = __builtin_amdgcn_readfirstlane((int)c.t0), t1 = __builtin_amdgcn_readfirstlane((int)c.t1);
@@ -463,19 +468,22 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
 #pragma unroll
   for (int d = 0; d < DT; ++d) *reinterpret_cast<float4v*>(so + ((wave * DT + d) * 64 + lane) * 4) = o[d];
   __syncthreads();
-  if (s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3]) {  // block-uniform: the chunk again, a head at a time
+  int any = s_odd[0];
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) any |= s_odd[i];
+  if (any) {  // block-uniform: the chunk again, a head at a time
     for (int g = wave; g < heads; g += kWaves) {
       const int64_t row = row0 + g;
       float m, l, acc[E];
       attend_row<D, TYPE>(p, shift, list, c.b, h, c.t0, c.t1, q + row * D, scale_log2, lane, m, l, acc);
-      if (part_ml == nullptr) {
+      if (parts.ml == nullptr) {
 #pragma unroll
         for (int e = 0; e < E; ++e) out[row * D + lane * E + e] = f2h(l == 0.f ? 0.f : acc[e] / l);
       } else {
         const int64_t slot = ((int64_t)w * p.kv_heads + h) * G + g0 + g;
-        if (lane == 0) part_ml[2 * slot] = m, part_ml[2 * slot + 1] = l;
+        if (lane == 0) parts.ml[2 * slot] = m, parts.ml[2 * slot + 1] = l;
 #pragma unroll
-        for (int e = 0; e < E; ++e) part_acc[slot * D + lane * E + e] = acc[e];
+        for (int e = 0; e < E; ++e) parts.acc[slot * D + lane * E + e] = acc[e];
       }
     }
     return;
@@ -491,88 +499,115 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;
   const int64_t slot = ((int64_t)w * p.kv_heads + h) * G + g0 + col;
-  if (part_ml != nullptr && wave == 0 && grp == 0 && col < heads) part_ml[2 * slot] = m, part_ml[2 * slot + 1] = l;
-#pragma unroll
-  for (int i = 0; i < DT / kWaves; ++i) {
-    const int d = i * kWaves + wave;
+  if (parts.ml != nullptr && wave == 0 && grp == 0 && col < heads) parts.ml[2 * slot] = m, parts.ml[2 * slot + 1] = l;
+  for (int d = wave; d < DT; d += kWaves) {
     float4v a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < kWaves; ++x) a += f[x] * *reinterpret_cast<const float4v*>(so + ((x * DT + d) * 64 + lane) * 4);
     if (col >= heads) continue;
-    if (part_ml == nullptr) {
+    if (parts.ml == nullptr) {
       const half4w r = {(f16)(a[0] * inv), (f16)(a[1] * inv), (f16)(a[2] * inv), (f16)(a[3] * inv)};
       *reinterpret_cast<half4w*>(out + (row0 + col) * D + d * 16 + grp * 4) = r;
     } else {
-      *reinterpret_cast<float4v*>(part_acc + slot * D + d * 16 + grp * 4) = a;
+      *reinterpret_cast<float4v*>(parts.acc + slot * D + d * 16 + grp * 4) = a;
     }
   }
 }
 
 // out = sum_j w_j acc_j / sum_j w_j l_j over a sequence's chunks, w_j = 2^(m_j - max m).
+// The (m, l) of 64 chunks are one load of a wave, and the rows of O do not wait for them.
 template <int D>
 __global__ void __launch_bounds__(256)
-paged_merge_kernel(const rfsn_paged p, int shift, int q_heads, int per_seq, int target, const float* __restrict__ part_acc,
-                   const float* __restrict__ part_ml, uint16_t* __restrict__ out) {
-  constexpr int E = D / 64;
+paged_merge_kernel(const rfsn_paged p, int shift, int q_heads, int per_seq, const Parts parts, uint16_t* __restrict__ out) {
+  constexpr int E = D / 64, U = 4;
   __shared__ float s_l[4], s_acc[4][D];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = blockIdx.x, b = blockIdx.y;
-  int slot0, n;
-  if (per_seq) {
-    slot0 = b * per_seq, n = per_seq;
-  } else {
-    const int64_t size = chunk_size(p, shift, target, lane);
-    slot0 = chunks_before(p, shift, size, b, lane);
-    n = (int)((paged_len(p, shift, b) + size - 1) / size);
+  int slot0 = b * per_seq, n = per_seq;
+  if (!per_seq) {
+    const int len = paged_len(p, shift, b);
+    slot0 = parts.seq[2 * b], n = parts.seq[2 * b + 1];
+    if (len == 0) slot0 = 0, n = 0;  // an empty sequence has no chunk, and nothing was written there
   }
-  float mx = -__builtin_inff();
-  for (int j = lane; j < n; j += 64) mx = fmaxf(mx, part_ml[2 * ((int64_t)(slot0 + j) * q_heads + i)]);
-  mx = wave_max(mx);
-  float l = 0.f, acc[E];
+  float m = -__builtin_inff(), l = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int j = wave; j < n; j += 4) {
-    const int64_t s = (int64_t)(slot0 + j) * q_heads + i;
-    const float m = part_ml[2 * s];
-    const float w = m > -__builtin_inff() ? exp2f(m - mx) : 1.f;  // with m -infinite the sums are 0 or NaN
-    l += w * part_ml[2 * s + 1];
+  for (int base = 0; base < n; base += 64) {
+    const int here = min(64, n - base);
+    float mj = -__builtin_inff(), lj = 0.f;
+    if (lane < here) {
+      const int64_t s = (int64_t)(slot0 + base + lane) * q_heads + i;
+      mj = parts.ml[2 * s], lj = parts.ml[2 * s + 1];
+    }
+    const float mn = fmaxf(m, wave_max(mj)), mref = mn > -__builtin_inff() ? mn : 0.f;
+    const float corr = m > -__builtin_inff() ? exp2f(m - mref) : 1.f;
+    const float wj = mj > -__builtin_inff() ? exp2f(mj - mref) : 1.f;  // with m -infinite the sums are 0 or NaN
+    l = l * corr + wave_sum(lane < here ? wj * lj : 0.f);
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(w, part_acc[s * D + lane * E + e], acc[e]);
+    for (int e = 0; e < E; ++e) acc[e] *= corr;
+    for (int j0 = wave; j0 < here; j0 += 4 * U) {
+      float x[U][E];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = min(j0 + 4 * u, here - 1);
+        const float* a = parts.acc + ((int64_t)(slot0 + base + j) * q_heads + i) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[u][e] = a[e];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (j0 + 4 * u >= here) break;
+        const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wj), j0 + 4 * u));
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(w, x[u][e], acc[e]);
+      }
+    }
+    m = mn;
   }
-  if (lane == 0) s_l[wave] = l;
 #pragma unroll
   for (int e = 0; e < E; ++e) s_acc[wave][lane * E + e] = acc[e];
   __syncthreads();
-  const float total = s_l[0] + s_l[1] + s_l[2] + s_l[3];
   for (int d = threadIdx.x; d < D; d += 256) {
     const float a = s_acc[0][d] + s_acc[1][d] + s_acc[2][d] + s_acc[3][d];
-    out[((int64_t)b * q_heads + i) * D + d] = f2h(total == 0.f ? 0.f : a / total);
+    out[((int64_t)b * q_heads + i) * D + d] = f2h(l == 0.f ? 0.f : a / l);
   }
 }
 
-// Chunks of a call: slots of partial results, chunks per sequence (0: cut by the
-// lengths on the device), their size, and the number the device aims at.
+// How a call is cut, by what the host knows: the sequences' capacity.
 struct Plan {
-  int64_t slots;
-  int per_seq;
-  int64_t chunk;
-  int target;
-  bool split() const { return per_seq != 1; }
+  int64_t slots;  // of partial results
+  Cut cut;
+  bool wide;      // blocks of many waves
+  bool split() const { return cut.per_seq != 1; }
 };
+int waves_of(int D, bool wide) { return !wide || D == 256 ? 4 : D == 64 ? 16 : 8; }  // (256: 8 would spill)
 Plan plan(const rfsn_paged& p, int q_heads, int count) {
   const int64_t most = (int64_t)(count ? count : p.table_width) * p.page_size;
-  const int64_t want = ceil_div(kBlocks, p.kv_heads * ceil_div(q_heads / p.kv_heads, 16));  // chunks that fill the chip
-  if (most <= kMinChunk) return {p.batch, 1, kMinChunk, 0};
+  const int64_t units = (int64_t)p.kv_heads * ceil_div(q_heads / p.kv_heads, 16);  // blocks of a chunk
+  Plan r;
+  r.wide = (int64_t)p.batch * units * ceil_div(most, kTile) <= kWideTiles;
+  const int per_step = waves_of(p.head_dim, r.wide) * kTile;
+  const int64_t least = r.wide ? per_step : 4 * per_step;  // positions of a chunk
+  if (most <= 4 * per_step) {
+    r.slots = p.batch, r.cut = {1, 0, most > 0 ? most : 1};
+    return r;
+  }
+  const int64_t want = ceil_div(r.wide ? 256 : 1024, units);  // chunks that fill the chip
   if (count) {
     int64_t n = ceil_div(want, p.batch);
-    if (n > ceil_div(most, kMinChunk)) n = ceil_div(most, kMinChunk);
-    const int64_t chunk = ceil_div(ceil_div(most, n), kUnit) * kUnit;
+    if (n > ceil_div(most, least)) n = ceil_div(most, least);
+    const int64_t chunk = ceil_div(ceil_div(most, n), per_step) * per_step;
     n = ceil_div(most, chunk);
-    return {n * p.batch, (int)n, chunk, 0};
+    r.slots = n * p.batch, r.cut = {(int)n, 0, chunk};
+    return r;
   }
   int64_t target = want;
-  if (target > ceil_div(most, kMinChunk) * p.batch) target = ceil_div(most, kMinChunk) * p.batch;
-  return {target + p.batch, 0, 0, (int)target};
+  if (target > ceil_div(most, least) * p.batch) target = ceil_div(most, least) * p.batch;
+  r.slots = target + p.batch, r.cut = {0, (int)target, least};
+  return r;
+}
+size_t parts_bytes(const rfsn_paged& p, const Plan& c, int q_heads) {
+  return (size_t)c.slots * q_heads * (p.head_dim + 2) * sizeof(float) + (size_t)p.batch * 2 * sizeof(int32_t);
 }
 
 }  // namespace
@@ -583,7 +618,7 @@ using namespace rfsn;
 extern "C" size_t rfsn_paged_attention_workspace_bytes(const rfsn_paged* p, int32_t q_heads, int32_t count) {
   if (p == nullptr || p->batch <= 0 || p->kv_heads <= 0 || p->page_size <= 0 || q_heads < p->kv_heads || count < 0) return 0;
   const Plan c = plan(*p, q_heads, count);
-  return c.split() ? (size_t)c.slots * q_heads * (p->head_dim + 2) * sizeof(float) : 0;
+  return c.split() ? parts_bytes(*p, c, q_heads) : 0;
 }
 
 extern "C" int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t q_heads, float scale,
@@ -600,34 +635,40 @@ extern "C" int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t 
   RFSN_REQUIRE(q && out && ((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 15) == 0,
                "paged_attention: q and out must be 16-byte aligned");
   const Plan c = plan(*p, q_heads, count);
-  RFSN_REQUIRE(workspace_bytes >= rfsn_paged_attention_workspace_bytes(p, q_heads, count) && (workspace || !c.split()),
-               "paged_attention: workspace too small");
+  RFSN_REQUIRE(workspace_bytes >= rfsn_paged_attention_workspace_bytes(p, q_heads, count) && ((workspace && ((uintptr_t)workspace & 15) == 0) || !c.split()),
+               "paged_attention: workspace too small or misaligned");
   RFSN_REQUIRE(c.slots <= 65535, "paged_attention: too many sequences");
   const hipStream_t s = (hipStream_t)stream;
   const int shift = paged_shift(*p), G = q_heads / p->kv_heads;
   const float sl2 = scale * 1.44269504088896340736f;
-  float* acc = c.split() ? (float*)workspace : nullptr;
-  float* ml = c.split() ? acc + c.slots * q_heads * p->head_dim : nullptr;
-#define RFSN_ATTEND(DD, TT)                                                                                            \
-  hipLaunchKernelGGL((paged_attn_kernel<DD, TT>), dim3((unsigned)p->kv_heads, (unsigned)c.slots, (unsigned)ceil_div(G, 16)), \
-                     dim3(kWaves * 64), 0, s, *p, shift, p->table, (const uint16_t*)q, G, sl2, chosen, count, c.per_seq, c.chunk, c.target, (uint16_t*)out,   \
-                     acc, ml)
-#define RFSN_ATTEND_D(DD)                                            \
-  do {                                                               \
-    if (p->type == RFSN_PAGE_FP16) RFSN_ATTEND(DD, RFSN_PAGE_FP16);  \
-    else if (p->type == RFSN_PAGE_INT8) RFSN_ATTEND(DD, RFSN_PAGE_INT8); \
-    else RFSN_ATTEND(DD, RFSN_PAGE_E4M3);                            \
+  Parts parts = {nullptr, nullptr, nullptr};
+  if (c.split()) {
+    parts.acc = (float*)workspace;
+    parts.ml = parts.acc + c.slots * q_heads * p->head_dim;
+    parts.seq = (int32_t*)(parts.ml + c.slots * q_heads * 2);
+  }
+  const dim3 grid((unsigned)p->kv_heads, (unsigned)c.slots, (unsigned)ceil_div(G, 16));
+#define RFSN_ATTEND(DD, TT, NW)                                                                                     \
+  hipLaunchKernelGGL((paged_attn_kernel<DD, TT, NW>), grid, dim3(NW * 64), 0, s, *p, shift, p->table,               \
+                     (const uint16_t*)q, G, sl2, chosen, count, c.cut, (uint16_t*)out, parts)
+#define RFSN_ATTEND_D(DD, NW)                                            \
+  do {                                                                   \
+    if (p->type == RFSN_PAGE_FP16) RFSN_ATTEND(DD, RFSN_PAGE_FP16, NW);  \
+    else if (p->type == RFSN_PAGE_INT8) RFSN_ATTEND(DD, RFSN_PAGE_INT8, NW); \
+    else RFSN_ATTEND(DD, RFSN_PAGE_E4M3, NW);                            \
   } while (0)
-  if (p->head_dim == 64) RFSN_ATTEND_D(64);
-  else if (p->head_dim == 128) RFSN_ATTEND_D(128);
-  else RFSN_ATTEND_D(256);
+  if (p->head_dim == 64 && c.wide) RFSN_ATTEND_D(64, 16);
+  else if (p->head_dim == 64) RFSN_ATTEND_D(64, 4);
+  else if (p->head_dim == 128 && c.wide) RFSN_ATTEND_D(128, 8);
+  else if (p->head_dim == 128) RFSN_ATTEND_D(128, 4);
+  else RFSN_ATTEND_D(256, 4);
 #undef RFSN_ATTEND_D
 #undef RFSN_ATTEND
   if (int st = check_launch("paged_attention")) return st;
   if (c.split()) {
-    const dim3 grid((unsigned)q_heads, (unsigned)p->batch);
-#define RFSN_MERGE(DD)                                                                                            \
-  hipLaunchKernelGGL(paged_merge_kernel<DD>, grid, dim3(256), 0, s, *p, shift, q_heads, c.per_seq, c.target, acc, ml, \
+    const dim3 rows((unsigned)q_heads, (unsigned)p->batch);
+#define RFSN_MERGE(DD)                                                                                           \
+  hipLaunchKernelGGL(paged_merge_kernel<DD>, rows, dim3(256), 0, s, *p, shift, q_heads, c.cut.per_seq, parts, \
                      (uint16_t*)out)
     if (p->head_dim == 64) RFSN_MERGE(64);
     else if (p->head_dim == 128) RFSN_MERGE(128);

@@ -8,6 +8,8 @@ library itself never allocates device memory) and raises on failure.
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import struct
 import weakref
 from collections import OrderedDict
 from dataclasses import dataclass
@@ -722,58 +724,86 @@ class KVPages(NamedTuple):
     bounds: Optional[torch.Tensor] = None
 
 
-def _paged(what: str, pages: KVPages, table: torch.Tensor, lens: torch.Tensor) -> "L.Paged":
-    """The checked parameter block of a pool, a block table [B, W] int32 and lengths [B] int32."""
+_PAGED_BLOCK = struct.Struct("7P3q7i4x")  # rfsn_paged, packed: a call's fields as they are, without a ctypes object
+
+
+def _paged(what: str, pages: KVPages, table: torch.Tensor, lens: torch.Tensor) -> Tuple[bytes, tuple, int]:
+    """The checked parameter block of a pool, a block table [B, W] int32 and
+    lengths [B] int32: (block, (B, Hkv, D, S, W), device index)."""
     k, v, ks, vs, bounds = pages
-    dev = _dev(k, what).device
-    if k.dim() != 4 or v.shape != k.shape or v.dtype is not k.dtype or v.stride() != k.stride():
-        raise ValueError(f"{what}: k and v pages must be alike, [pages, kv_heads, page_size, head_dim]")
-    P, H, S, D = k.shape
-    kind = PAGE_TYPES.get(k.dtype)
+    dev = _dev(k, what).get_device()
+    if k.dim() != 4 or v.dim() != 4:
+        raise ValueError(f"{what}: k and v pages must be [pages, kv_heads, page_size, head_dim]")
+    shape, (sp, sh, ss, sd), dtype = k.shape, k.stride(), k.dtype
+    if v.shape != shape or v.dtype is not dtype or v.stride() != (sp, sh, ss, sd):
+        raise ValueError(f"{what}: k and v pages must be of one shape, type and stride")
+    P, H, S, D = shape
+    kind = PAGE_TYPES.get(dtype)
     if kind is None:
-        raise ValueError(f"{what}: pages of {k.dtype}; float16, int8 and float8_e4m3fn are served")
-    sp, sh, ss, sd = k.stride()
+        raise ValueError(f"{what}: pages of {dtype}; float16, int8 and float8_e4m3fn are served")
     if sd != 1 or ss != D:
         raise ValueError(f"{what}: a head's rows must be dense")
-    if (kind == 0) != (ks is None) or (kind == 0) != (vs is None):
-        raise ValueError(f"{what}: 8-bit pages need k_scale and v_scale, fp16 pages neither")
-    for t, shape, dtype, name in ((ks, (P, H, S), torch.float32, "k_scale"), (vs, (P, H, S), torch.float32, "v_scale"),
-                                  (bounds, (P, H, 2, D), torch.float16, "bounds")):
-        if t is not None and (t.shape != shape or t.dtype is not dtype or not t.is_contiguous()):
-            raise ValueError(f"{what}: {name} must be contiguous {list(shape)} {dtype}")
-    if table.dim() != 2 or table.dtype is not torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError(f"{what}: the block table must be int32 [batch, pages per sequence] with dense rows")
-    if lens.shape != (table.shape[0],) or lens.dtype is not torch.int32 or not lens.is_contiguous():
+    apart = v.get_device() != dev or table.get_device() != dev or lens.get_device() != dev
+    if kind:
+        if ks is None or vs is None:
+            raise ValueError(f"{what}: 8-bit pages need k_scale and v_scale")
+        for t in (ks, vs):
+            if t.shape != (P, H, S) or t.dtype is not torch.float32 or not t.is_contiguous():
+                raise ValueError(f"{what}: scales must be contiguous fp32 {[P, H, S]}")
+            apart = apart or t.get_device() != dev
+        ks, vs = ks.data_ptr(), vs.data_ptr()
+    elif ks is not None or vs is not None:
+        raise ValueError(f"{what}: fp16 pages have no scales")
+    if bounds is not None:
+        if bounds.shape != (P, H, 2, D) or bounds.dtype is not torch.float16 or not bounds.is_contiguous():
+            raise ValueError(f"{what}: bounds must be contiguous fp16 {[P, H, 2, D]}")
+        apart = apart or bounds.get_device() != dev
+        bounds = bounds.data_ptr()
+    if table.dim() != 2 or table.dtype is not torch.int32:
+        raise ValueError(f"{what}: the block table must be int32 [batch, pages per sequence]")
+    (B, W), (st, sw) = table.shape, table.stride()
+    if sw != 1 and W > 1:
+        raise ValueError(f"{what}: the block table's rows must be dense")
+    if lens.dtype is not torch.int32 or lens.shape != (B,) or not lens.is_contiguous():
         raise ValueError(f"{what}: lengths must be contiguous int32 [batch]")
-    for t in (v, ks, vs, bounds, table, lens):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: pages, table and lengths must be on one device")
-    return L.Paged(k.data_ptr(), v.data_ptr(), L.ptr(ks), L.ptr(vs), L.ptr(bounds), table.data_ptr(), lens.data_ptr(),
-                   sp, sh, table.stride(0), P, S, H, D, kind, table.shape[0], table.shape[1])
+    if apart:
+        raise ValueError(f"{what}: pages, table and lengths must be on one device")
+    if max(P, H, S, D, B, W) >= 1 << 31:
+        raise ValueError(f"{what}: sizes must stay below 2^31")
+    return (_PAGED_BLOCK.pack(k.data_ptr(), v.data_ptr(), ks or 0, vs or 0, bounds or 0, table.data_ptr(),
+                              lens.data_ptr(), sp, sh, st, P, S, H, D, kind, B, W), (B, H, D, S, W), dev)
 
 
-def _paged_call(device: torch.device, name: str, *args) -> None:
-    """The call on ``device``'s current stream, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        L.call(name, *args, L.stream_handle(device))
+def _paged_call(device: int, name: str, *args) -> None:
+    """The call on the device's current stream, whichever device is current."""
+    if device == torch.cuda.current_device():
+        L.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            L.call(name, *args, L.stream_handle(device))
+            L.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
 
 
-def _cu(what: str, cu: torch.Tensor, batch: int, device: torch.device) -> int:
-    if cu.shape != (batch + 1,) or cu.dtype is not torch.int32 or not cu.is_contiguous() or cu.device != device:
+def _cu(what: str, cu: torch.Tensor, batch: int, device: int) -> int:
+    if cu.shape != (batch + 1,) or cu.dtype is not torch.int32 or not cu.is_contiguous() or cu.get_device() != device:
         raise ValueError(f"{what}: cu must be contiguous int32 [batch + 1] on the pages' device")
     return cu.data_ptr()
 
 
-def _paged_query(what: str, q: torch.Tensor, p: "L.Paged", device: torch.device) -> torch.Tensor:
-    if q.dim() != 3 or q.dtype is not torch.float16 or q.shape[0] != p.batch or q.shape[2] != p.head_dim \
-            or q.device != device:
-        raise ValueError(f"{what}: q must be fp16 [batch, q_heads, head_dim] = [{p.batch}, *, {p.head_dim}] "
+def _paged_query(what: str, q: torch.Tensor, batch: int, head_dim: int, device: int) -> torch.Tensor:
+    if q.dim() != 3 or q.dtype is not torch.float16 or q.shape[0] != batch or q.shape[2] != head_dim \
+            or q.get_device() != device:
+        raise ValueError(f"{what}: q must be fp16 [batch, q_heads, head_dim] = [{batch}, *, {head_dim}] "
                          "on the pages' device")
-    q = _contig(q)
+    if not q.is_contiguous():
+        q = q.contiguous()
     return q.clone() if q.data_ptr() % 16 else q
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_workspace(name: str, batch: int, kv_heads: int, head_dim: int, page_size: int, width: int, *more: int) -> int:
+    """A call's workspace, which its sizes alone determine."""
+    p = L.Paged(kv_heads=kv_heads, head_dim=head_dim, page_size=page_size, batch=batch, table_width=width)
+    return getattr(L.load(), name)(C.byref(p), *more)
 
 
 def paged_append(pages: KVPages, table: torch.Tensor, lens: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -783,25 +813,23 @@ def paged_append(pages: KVPages, table: torch.Tensor, lens: torch.Tensor, k: tor
     int32; None: row b) follow the ``lens[b]`` tokens of sequence b.  Rows
     behind cu[B] are ignored, as is what the table has no page for; ``lens`` is
     not changed.  No two sequences of a call may append to one page."""
-    p = _paged("paged_append", pages, table, lens)
-    dev = pages.k.device
-    if k.dim() != 3 or k.shape[1:] != (p.kv_heads, p.head_dim) or v.shape != k.shape \
-            or k.dtype is not torch.float16 or v.dtype is not torch.float16 or k.device != dev or v.device != dev:
-        raise ValueError(f"paged_append: k and v must be fp16 [rows, {p.kv_heads}, {p.head_dim}] on the pages' device")
+    block, (B, H, D, _, _), dev = _paged("paged_append", pages, table, lens)
+    if k.dim() != 3 or k.shape[1:] != (H, D) or v.shape != k.shape or k.dtype is not torch.float16 \
+            or v.dtype is not torch.float16 or k.get_device() != dev or v.get_device() != dev:
+        raise ValueError(f"paged_append: k and v must be fp16 [rows, {H}, {D}] on the pages' device")
     n = k.shape[0]
-    if cu is None:
-        if n != p.batch:
-            raise ValueError(f"paged_append: without cu there is one row per sequence ({p.batch}), got {n}")
-    else:
-        cu_ptr = _cu("paged_append", cu, p.batch, dev)
+    if cu is not None:
+        cu = _cu("paged_append", cu, B, dev)
+    elif n != B:
+        raise ValueError(f"paged_append: without cu there is one row per sequence ({B}), got {n}")
     if n == 0:
         return
     ts, hs, cs = k.stride()
-    if v.stride() != (ts, hs, cs) or cs != 1 or ts % 8 or hs % 8 or k.data_ptr() % 16 or v.data_ptr() % 16:
+    kp, vp = k.data_ptr(), v.data_ptr()
+    if v.stride() != (ts, hs, cs) or cs != 1 or ts % 8 or hs % 8 or kp % 16 or vp % 16:
         k, v = k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format)
-        ts, hs, _ = k.stride()
-    _paged_call(dev, "rfsn_paged_append", C.byref(p), k.data_ptr(), v.data_ptr(), ts, hs, n,
-                None if cu is None else cu_ptr)
+        (ts, hs, _), kp, vp = k.stride(), k.data_ptr(), v.data_ptr()
+    _paged_call(dev, "rfsn_paged_append", block, kp, vp, ts, hs, n, cu)
 
 
 def paged_read(pages: KVPages, table: torch.Tensor, starts: torch.Tensor, cu: torch.Tensor, rows: int,
@@ -810,24 +838,22 @@ def paged_read(pages: KVPages, table: torch.Tensor, starts: torch.Tensor, cu: to
     are positions starts[b], starts[b] + 1, ... of sequence b, zeros where the
     table has no page.  Rows behind cu[B] are zeros; in ``out`` (k, v of that
     shape, contiguous) they are left as they were."""
-    p = _paged("paged_read", pages, table, starts)
-    dev = pages.k.device
+    block, (B, H, D, _, _), dev = _paged("paged_read", pages, table, starts)
     rows = int(rows)
     if rows < 0:
         raise ValueError("paged_read: negative row count")
-    shape = (rows, p.kv_heads, p.head_dim)
-    cu_ptr = _cu("paged_read", cu, p.batch, dev)
+    cu = _cu("paged_read", cu, B, dev)
     if out is None:
-        ko = torch.empty(shape, dtype=torch.float16, device=dev)
-        vo = torch.empty(shape, dtype=torch.float16, device=dev)
+        ko = torch.empty((rows, H, D), dtype=torch.float16, device=pages.k.device)
+        vo = torch.empty_like(ko)
     else:
         ko, vo = out
         for t in out:
-            if t.shape != shape or t.dtype is not torch.float16 or not t.is_contiguous() or t.device != dev \
-                    or t.data_ptr() % 16:
-                raise ValueError(f"paged_read: out must be two contiguous fp16 {list(shape)} on the pages' device")
+            if t.shape != (rows, H, D) or t.dtype is not torch.float16 or not t.is_contiguous() \
+                    or t.get_device() != dev or t.data_ptr() % 16:
+                raise ValueError(f"paged_read: out must be two contiguous fp16 [{rows}, {H}, {D}] on the pages' device")
     if rows:
-        _paged_call(dev, "rfsn_paged_read", C.byref(p), cu_ptr, rows, ko.data_ptr(), vo.data_ptr(), int(out is None))
+        _paged_call(dev, "rfsn_paged_read", block, cu, rows, ko.data_ptr(), vo.data_ptr(), int(out is None))
     return ko, vo
 
 
@@ -838,18 +864,19 @@ def page_select(q: torch.Tensor, pages: KVPages, table: torch.Tensor, lens: torc
     ``first`` and ``last`` ones are always among them, the others those with the
     largest upper bound of q . k by the pages' bounds, over the KV head's query
     heads (``rfsn_page_select``)."""
-    p = _paged("page_select", pages, table, lens)
-    dev = pages.k.device
+    block, sizes, dev = _paged("page_select", pages, table, lens)
+    B, H, D, S, W = sizes
     if pages.bounds is None:
         raise ValueError("page_select: the pages hold no bounds")
-    q = _paged_query("page_select", q, p, dev)
+    q = _paged_query("page_select", q, B, D, dev)
     count, first, last = int(count), int(first), int(last)
     if count <= 0 or first < 0 or last < 0 or first + last > count:
         raise ValueError("page_select: count must be positive and have room for the first and last pages")
-    chosen = torch.empty((p.batch, p.kv_heads, count), dtype=torch.int32, device=dev)
-    wsb = L.load().rfsn_page_select_workspace_bytes(C.byref(p))
-    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-    _paged_call(dev, "rfsn_page_select", C.byref(p), q.data_ptr(), q.shape[1], count, first, last, chosen.data_ptr(),
+    device = pages.k.device
+    chosen = torch.empty((B, H, count), dtype=torch.int32, device=device)
+    wsb = _paged_workspace("rfsn_page_select_workspace_bytes", *sizes)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=device)
+    _paged_call(dev, "rfsn_page_select", block, q.data_ptr(), q.shape[1], count, first, last, chosen.data_ptr(),
                 ws.data_ptr(), wsb)
     return chosen
 
@@ -860,23 +887,24 @@ def paged_attention(q: torch.Tensor, pages: KVPages, table: torch.Tensor, lens: 
     sequence's first ``lens[b]`` positions, or over those of its pages that
     ``chosen`` [B, Hkv, n] (``page_select``) lists; zeros where there are none.
     Codes are attended as code * scale in fp32, not rounded to fp16."""
-    p = _paged("paged_attention", pages, table, lens)
-    dev = pages.k.device
-    q = _paged_query("paged_attention", q, p, dev)
-    count = 0
+    block, sizes, dev = _paged("paged_attention", pages, table, lens)
+    B, H, D, _, _ = sizes
+    q = _paged_query("paged_attention", q, B, D, dev)
+    count, listed = 0, None
     if chosen is not None:
-        if chosen.dim() != 3 or chosen.shape[:2] != (p.batch, p.kv_heads) or chosen.dtype is not torch.int32 \
-                or chosen.device != dev:
-            raise ValueError(f"paged_attention: chosen must be int32 [{p.batch}, {p.kv_heads}, n] on the pages' device")
+        if chosen.dim() != 3 or chosen.shape[:2] != (B, H) or chosen.dtype is not torch.int32 \
+                or chosen.get_device() != dev:
+            raise ValueError(f"paged_attention: chosen must be int32 [{B}, {H}, n] on the pages' device")
         chosen = _contig(chosen)
-        count = chosen.shape[2]
+        count, listed = chosen.shape[2], chosen.data_ptr()
     out = torch.empty_like(q)
     if chosen is not None and count == 0:
         return out.zero_()
-    wsb = L.load().rfsn_paged_attention_workspace_bytes(C.byref(p), q.shape[1], count)
-    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
-    _paged_call(dev, "rfsn_paged_attention", C.byref(p), q.data_ptr(), q.shape[1], float(scale), L.ptr(chosen), count,
-                out.data_ptr(), L.ptr(ws), wsb)
+    Hq = q.shape[1]
+    wsb = _paged_workspace("rfsn_paged_attention_workspace_bytes", *sizes, Hq, count)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
+    _paged_call(dev, "rfsn_paged_attention", block, q.data_ptr(), Hq, float(scale), listed, count, out.data_ptr(),
+                None if ws is None else ws.data_ptr(), wsb)
     return out
 
 

@@ -47,6 +47,15 @@ def test_parameter_block_layout(tmp_path):
         assert int(got[f]) == getattr(_lib.Paged, f).offset, f
 
 
+def test_packed_block_is_the_parameter_block():
+    """What the wrappers pack is the ctypes mirror's bytes."""
+    from apple_amd import _lib
+    from apple_amd.kernels import _PAGED_BLOCK
+
+    values = [(i + 1) << 33 if ctypes.sizeof(t) == 8 else i + 1 for i, (_, t) in enumerate(_lib.Paged._fields_)]
+    assert _PAGED_BLOCK.pack(*values) == bytes(_lib.Paged(*values))
+
+
 @pytest.mark.parametrize("bad, says", [
     (dict(head_dim=96), "head_dim"), (dict(page_size=8), "page_size"), (dict(page_size=48), "page_size"),
     (dict(type=3), "page type"), (dict(kv_heads=0), "kv_heads"), (dict(batch=-1), "batch"), (dict(batch=70000), "batch"),
@@ -102,7 +111,7 @@ def test_workspace_sizes(lib):
     assert size(ctypes.byref(block()), 8, 0) == 0  # 160 positions: one chunk, no partials
     wide = block(table_width=4096)
     need = size(ctypes.byref(wide), 32, 0)
-    assert need > 0 and need % (32 * 66 * 4) == 0
+    assert need > 32 * 66 * 4  # partial results of several chunks
     assert lib.rfsn_paged_attention(ctypes.byref(wide), 4096, 32, 0.125, None, 0, 4096, 4096, need - 1, None) == -1
     assert b"workspace" in lib.rfsn_last_error()
     assert lib.rfsn_page_select_workspace_bytes(ctypes.byref(wide)) >= 2 * 8 * 4096 * 4
