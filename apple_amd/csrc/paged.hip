@@ -52,23 +52,43 @@ struct RowPlace {
   int row;    // in the page
   int count;  // rows of this call in the same page from here on
   bool start; // the first of them
+  bool rest;  // behind the last sequence, or before the first
 };
+// Where the lanes' rows go: row n0 + lane / LANES of the call, one wave, n0 the wave's.
+// Up to 63 sequences lie in the wave's lanes, so that no load waits for another but the table's.
+template <int LANES>
 __device__ __forceinline__ RowPlace row_place(const rfsn_paged& p, int shift, const int32_t* __restrict__ cu,
-                                              int64_t rows, int64_t n) {
-  RowPlace r = {-1, 0, 0, false};
-  if (n >= rows) return r;
-  int b;
-  int64_t i, left;
-  if (cu) {
+                                              int64_t rows, int64_t n0, int lane) {
+  const int64_t n = n0 + lane / LANES;
+  RowPlace r = {-1, 0, 0, false, true};
+  int64_t i = 0, left = 0;
+  int b = -1, len = 0;
+  if (cu == nullptr) {
+    if (n < rows) b = (int)n, left = 1, len = p.lens[b];
+  } else if (p.batch > 0 && p.batch < 64) {
+    const int c = cu[min(lane, p.batch)], ln = p.lens[min(lane, p.batch - 1)];
+    int before = 0;  // bounds at or below the lane's row
+#pragma unroll
+    for (int s = 0; s < 64 / LANES; ++s) {
+      const int x = (int)__popcll(__ballot(lane <= p.batch && c <= n0 + s));
+      if (s == lane / LANES) before = x;
+    }
+    const int at = min(max(before - 1, 0), p.batch - 1);
+    const int64_t c0 = __shfl(c, at, 64), c1 = __shfl(c, at + 1, 64);
+    len = __shfl(ln, at, 64);
+    if (n < rows && n >= c0 && n < c1) b = at, i = n - c0, left = (c1 < rows ? c1 : rows) - n;
+  } else if (p.batch >= 64 && n < rows) {
     b = row_sequence(cu, p.batch, n);
-    if (b < 0) return r;
-    i = n - cu[b];
-    const int64_t end = cu[b + 1] < rows ? cu[b + 1] : rows;
-    left = end - n;
-  } else {
-    b = (int)n, i = 0, left = 1;
+    if (b >= 0) {
+      i = n - cu[b];
+      left = (cu[b + 1] < rows ? cu[b + 1] : rows) - n;
+      len = p.lens[b];
+      if (i < 0 || left <= 0) b = -1;  // no prefix
+    }
   }
-  const int64_t pos = (int64_t)max(p.lens[b], 0) + i;
+  if (b < 0) return r;
+  const int64_t pos = (int64_t)max(len, 0) + i;
+  r.rest = false;
   r.page = paged_page(p, b, pos >> shift);
   r.row = (int)(pos & (p.page_size - 1));
   r.count = (int)(left < p.page_size - r.row ? left : p.page_size - r.row);
@@ -76,8 +96,7 @@ __device__ __forceinline__ RowPlace row_place(const rfsn_paged& p, int shift, co
   return r;
 }
 
-// The sum of a quantised row's codes is never formed: rounding is one fp32
-// product, then the code's own.
+// A row's values by the row's largest: rounding is one fp32 product, then the code's own.
 template <int TYPE, int LANES>
 __device__ __forceinline__ void store_row(const rfsn_paged& p, void* base, float* scales, int64_t off, int64_t scale_at,
                                           half8v x, int chunk, bool write) {
@@ -116,27 +135,60 @@ __device__ __forceinline__ void store_row(const rfsn_paged& p, void* base, float
   }
 }
 
-__device__ __forceinline__ f16 min_nan(f16 a, f16 b) { return a < b || a != a ? a : b; }
-__device__ __forceinline__ f16 max_nan(f16 a, f16 b) { return a > b || a != a ? a : b; }
+typedef unsigned short ushort8v __attribute__((ext_vector_type(8)));
+
+// Smallest and largest keys of 8 coordinates, and their largest magnitude's bits, which are past infinity's where one is NaN.
+struct Bounds {
+  half8v lo, hi;
+  ushort8v top;
+  __device__ __forceinline__ void add(half8v x) {
+    lo = __builtin_elementwise_min(lo, x), hi = __builtin_elementwise_max(hi, x);
+    top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort8v, x) & (unsigned short)0x7fff);
+  }
+  // what a page holds already
+  __device__ __forceinline__ void add(half8v l, half8v h) { add(l), add(h); }
+  __device__ __forceinline__ void across(int o) {  // with the lanes o apart
+    const uint4w l = __builtin_bit_cast(uint4w, lo), h = __builtin_bit_cast(uint4w, hi), t = __builtin_bit_cast(uint4w, top);
+    uint4w l2, h2, t2;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      l2[w] = (uint32_t)__shfl_xor((int)l[w], o, 64);
+      h2[w] = (uint32_t)__shfl_xor((int)h[w], o, 64);
+      t2[w] = (uint32_t)__shfl_xor((int)t[w], o, 64);
+    }
+    lo = __builtin_elementwise_min(lo, __builtin_bit_cast(half8v, l2));
+    hi = __builtin_elementwise_max(hi, __builtin_bit_cast(half8v, h2));
+    top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort8v, t2));
+  }
+  __device__ __forceinline__ void store(half8v* l, half8v* h) const {
+    ushort8v a = __builtin_bit_cast(ushort8v, lo), b = __builtin_bit_cast(ushort8v, hi);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (top[e] > 0x7c00) a[e] = b[e] = 0x7e00;
+    *l = __builtin_bit_cast(half8v, a), *h = __builtin_bit_cast(half8v, b);
+  }
+};
+__device__ __forceinline__ Bounds bounds_of(half8v x) {
+  return {x, x, __builtin_bit_cast(ushort8v, x) & (unsigned short)0x7fff};
+}
 
 // A wave writes RS = 64 / (D / 8) rows of one head, K and V; a lane holds 8
 // coordinates of a row.  Bounds: the wave of a run's first row (rows of one
-// sequence in one page) reads the run's keys and writes the page's bounds, so
-// no two waves write the same ones and no order changes them.
+// sequence in one page) reads the run's keys, eight rows of a lane in flight, and writes
+// the page's bounds, so no two waves write the same ones and no order changes them.
 template <int D, int TYPE>
 __global__ void __launch_bounds__(256)
 paged_append_kernel(const rfsn_paged p, int shift, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
                     int64_t ts, int64_t hs, int64_t rows, const int32_t* __restrict__ cu) {
-  constexpr int LANES = D / 8, RS = 64 / LANES;
+  constexpr int LANES = D / 8, RS = 64 / LANES, U = 8;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int h = blockIdx.y * 4 + wave;
   if (h >= p.kv_heads) return;
   const int slot = lane / LANES, chunk = lane % LANES;
-  const int64_t n = (int64_t)blockIdx.x * RS + slot;
-  const int64_t nc = n < rows ? n : rows - 1;
+  const int64_t n0 = (int64_t)blockIdx.x * RS, nc = n0 + slot < rows ? n0 + slot : rows - 1;
   const half8v kx = *reinterpret_cast<const half8v*>(k + nc * ts + h * hs + chunk * 8);
   const half8v vx = *reinterpret_cast<const half8v*>(v + nc * ts + h * hs + chunk * 8);
-  const RowPlace at = row_place(p, shift, cu, rows, n);
+  const RowPlace at = row_place<LANES>(p, shift, cu, rows, n0, lane);
   const bool write = at.page >= 0;
   const int64_t off = (int64_t)(write ? at.page : 0) * p.page_stride + h * p.head_stride + (int64_t)at.row * D + chunk * 8;
   const int64_t sc = ((int64_t)(write ? at.page : 0) * p.kv_heads + h) * p.page_size + at.row;
@@ -144,53 +196,37 @@ paged_append_kernel(const rfsn_paged p, int shift, const uint16_t* __restrict__ 
   store_row<TYPE, LANES>(p, p.v, p.v_scale, off, sc, vx, chunk, write);
   if (p.bounds == nullptr) return;
   const bool leads = write && at.start;
+  auto bounds_at = [&](int page) {
+    return reinterpret_cast<half8v*>((uint16_t*)p.bounds + ((int64_t)page * p.kv_heads + h) * 2 * D + chunk * 8);
+  };
   // runs of one row: each row slot on its own; longer ones by the whole wave
   if (leads && at.count == 1) {
-    half8v* bp = reinterpret_cast<half8v*>((uint16_t*)p.bounds + ((int64_t)at.page * p.kv_heads + h) * 2 * D + chunk * 8);
-    half8v lo = kx, hi = kx;
-    if (at.row > 0) {
-      const half8v lo0 = bp[0], hi0 = bp[D / 8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) lo[e] = min_nan(lo0[e], lo[e]), hi[e] = max_nan(hi0[e], hi[e]);
-    }
-    bp[0] = lo, bp[D / 8] = hi;
+    half8v* bp = bounds_at(at.page);
+    Bounds m = bounds_of(kx);
+    if (at.row > 0) m.add(bp[0], bp[D / 8]);
+    m.store(bp, bp + D / 8);
   }
   uint64_t todo = __ballot(leads && at.count > 1);
   while (todo) {
     const int src = __ffsll((unsigned long long)todo) - 1;  // a lane of the run's first row
-    todo &= ~((LANES == 64 ? ~0ull : ((1ull << LANES) - 1)) << (src / LANES * LANES));
+    todo &= ~(((1ull << LANES) - 1) << (src / LANES * LANES));
     const int page = __builtin_amdgcn_readlane(at.page, src), row = __builtin_amdgcn_readlane(at.row, src);
     const int count = __builtin_amdgcn_readlane(at.count, src);
-    const int64_t n0 = (int64_t)blockIdx.x * RS + src / LANES;
-    half8v lo = *reinterpret_cast<const half8v*>(k + (n0 + min(slot, count - 1)) * ts + h * hs + chunk * 8);
-    half8v hi = lo;
-    for (int i = slot + RS; i < count; i += RS) {
-      const half8v x = *reinterpret_cast<const half8v*>(k + (n0 + i) * ts + h * hs + chunk * 8);
+    const uint16_t* run = k + (n0 + src / LANES) * ts + h * hs + chunk * 8;
+    half8v* bp = bounds_at(page);
+    const half8v x0 = *reinterpret_cast<const half8v*>(run + min(slot, count - 1) * ts);
+    Bounds m = bounds_of(x0);
+    if (row > 0) m.add(bp[0], bp[D / 8]);
+    for (int i = slot + RS; i - slot < count; i += U * RS) {
+      half8v x[U];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) lo[e] = min_nan(lo[e], x[e]), hi[e] = max_nan(hi[e], x[e]);
-    }
-    half8v* bp = reinterpret_cast<half8v*>((uint16_t*)p.bounds + ((int64_t)page * p.kv_heads + h) * 2 * D + chunk * 8);
-    if (row > 0) {
-      const half8v lo0 = bp[0], hi0 = bp[D / 8];
+      for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const half8v*>(run + min(i + u * RS, count - 1) * ts);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) lo[e] = min_nan(lo0[e], lo[e]), hi[e] = max_nan(hi0[e], hi[e]);
+      for (int u = 0; u < U; ++u) m.add(x[u]);
     }
 #pragma unroll
-    for (int o = LANES; o < 64; o <<= 1) {
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-        const h2 l2 = __builtin_bit_cast(h2, __shfl_xor((int)__builtin_bit_cast(u4, lo)[w], o, 64));
-        const h2 h2v = __builtin_bit_cast(h2, __shfl_xor((int)__builtin_bit_cast(u4, hi)[w], o, 64));
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          lo[2 * w + e] = min_nan(lo[2 * w + e], l2[e]);
-          hi[2 * w + e] = max_nan(hi[2 * w + e], h2v[e]);
-        }
-      }
-    }
-    if (slot == 0) bp[0] = lo, bp[D / 8] = hi;
+    for (int o = LANES; o < 64; o <<= 1) m.across(o);
+    if (slot == 0) m.store(bp, bp + D / 8);
   }
 }
 
@@ -204,12 +240,10 @@ paged_read_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ cu,
   if (h >= p.kv_heads) return;
   const int slot = lane / LANES, chunk = lane % LANES;
   const int64_t n = (int64_t)blockIdx.x * RS + slot;
-  if (n >= rows) return;
-  const bool rest = row_sequence(cu, p.batch, n) < 0;
-  if (rest && !zero_rest) return;
-  const RowPlace at = row_place(p, shift, cu, rows, n);
+  const RowPlace at = row_place<LANES>(p, shift, cu, rows, (int64_t)blockIdx.x * RS, lane);
+  if (n >= rows || (at.rest && !zero_rest)) return;
   half8v ko = {}, vo = {};
-  if (!rest && at.page >= 0) {
+  if (at.page >= 0) {
     const int64_t off = (int64_t)at.page * p.page_stride + h * p.head_stride + (int64_t)at.row * D + chunk * 8;
     if constexpr (TYPE == RFSN_PAGE_FP16) {
       ko = *reinterpret_cast<const half8v*>((const uint16_t*)p.k + off);

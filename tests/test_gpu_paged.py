@@ -101,6 +101,51 @@ def test_append_and_read(device, kind, dim, heads, size, starts, counts, pad):
         assert torch.equal(out[0][:at[-1]], ko[:at[-1]]) and (out[0][at[-1]:] == 7.0).all() and (out[1][at[-1]:] == 8.0).all()
 
 
+@pytest.mark.parametrize("batch", [63, 64, 200])
+def test_append_and_read_of_many_sequences(device, batch):
+    """More sequences than a wave's lanes hold, most of them with few rows or none, rows of one sequence in every wave."""
+    K = kernels()
+    g = torch.Generator().manual_seed(batch)
+    starts = torch.randint(0, 40, (batch,), generator=g).tolist()
+    counts = torch.randint(0, 5, (batch,), generator=g).tolist()
+    counts[0], counts[batch // 2], counts[-1] = 0, 90, 3
+    ends = [a + n for a, n in zip(starts, counts)]
+    pool = R.Pool("int8", sum(-(-e // 16) for e in ends) + 1, 2, 16, 64, seed=batch)
+    table, n = pool.tables(ends), sum(counts)
+    k, v = pool.randn((n + 7, 2, 64)), pool.randn((n + 7, 2, 64))
+    cu = [0]
+    for c in counts:
+        cu.append(cu[-1] + c)
+    pages = pool.pages(device)
+    K.paged_append(pages, table.to(device), i32(starts, device), k.to(device), v.to(device), i32(cu, device))
+    pool.append(table, starts, k, v, cu)
+    for name, got in pages._asdict().items():
+        assert same(got, getattr(pool, name)), name
+    ko, vo = K.paged_read(pages, table.to(device), i32(starts, device), i32(cu, device), n + 7)
+    for b in range(batch):
+        wk, wv, _ = pool.window(table, b, starts[b], ends[b])
+        for got, want in ((ko, wk), (vo, wv)):
+            assert ((got[cu[b]:cu[b + 1]].cpu().double() - want).abs() <= want.abs() * (2.0 ** -11 + 2.0 ** -24)).all()
+    assert not ko[n:].any()
+
+
+def test_no_sequences(device):
+    """An empty batch: no rows, and zeros read back."""
+    K = kernels()
+    pages = R.Pool("fp16", 2, 2, 16, 64, seed=1).pages(device)
+    table, lens, cu = torch.zeros((0, 3), dtype=torch.int32, device=device), i32([], device), i32([0], device)
+    K.paged_append(pages, table, lens, *(torch.ones((5, 2, 64), dtype=D16, device=device),) * 2, cu)
+    ko, vo = K.paged_read(pages, table, lens, cu, 5)
+    assert not ko.any() and not vo.any()
+    q = torch.ones((0, 4, 64), dtype=D16, device=device)
+    assert K.paged_attention(q, pages, table, lens, 0.1).shape == (0, 4, 64)
+    assert K.page_select(q, pages, table, lens, 3).shape == (0, 2, 3)
+    # and sequences whose table has no columns
+    table, lens, q = torch.zeros((2, 0), dtype=torch.int32, device=device), i32([4, 0], device), torch.ones((2, 4, 64), dtype=D16, device=device)
+    assert not K.paged_attention(q, pages, table, lens, 0.1).any()
+    assert (K.page_select(q, pages, table, lens, 3) == -1).all()
+
+
 @pytest.mark.parametrize("kind", ["fp16", "int8", "e4m3"])
 def test_rows_that_are_not_finite(device, kind):
     """A row with an infinity or NaN: as it is in fp16, scale NaN in 8 bits; bounds keep the NaN, later rows do not clear it."""
