@@ -15,43 +15,37 @@ int paged_check(const rfsn_paged* p, const char* what);
 
 inline int paged_shift(const rfsn_paged& p) { return __builtin_ctz((unsigned)p.page_size); }
 
+// 8 codes in fp32, where each is exact.
 template <int TYPE>
-struct PageElem {
-  typedef uint16_t type;
-};
-template <>
-struct PageElem<RFSN_PAGE_INT8> {
-  typedef uint8_t type;
-};
-template <>
-struct PageElem<RFSN_PAGE_E4M3> {
-  typedef uint8_t type;
-};
-
-// 8 consecutive stored values of a row, without the row's scale: exact in fp32.
-template <int TYPE>
-__device__ __forceinline__ float8v load_page8(const void* base, int64_t off) {
+__device__ __forceinline__ float8v page8(uint2v c) {
   float8v f;
-  if constexpr (TYPE == RFSN_PAGE_FP16) {
-    const half8v h = *reinterpret_cast<const half8v*>((const uint16_t*)base + off);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = (float)h[e];
-  } else {
-    const uint2v c = *reinterpret_cast<const uint2v*>((const uint8_t*)base + off);
+  for (int w = 0; w < 2; ++w) {
+    if constexpr (TYPE == RFSN_PAGE_INT8) {
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      if constexpr (TYPE == RFSN_PAGE_INT8) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[4 * w + e] = (float)(int8_t)(c[w] >> (8 * e));
-      } else {
-        f[4 * w + 0] = __builtin_amdgcn_cvt_f32_fp8((int)c[w], 0);
-        f[4 * w + 1] = __builtin_amdgcn_cvt_f32_fp8((int)c[w], 1);
-        f[4 * w + 2] = __builtin_amdgcn_cvt_f32_fp8((int)c[w], 2);
-        f[4 * w + 3] = __builtin_amdgcn_cvt_f32_fp8((int)c[w], 3);
-      }
+      for (int e = 0; e < 4; ++e) f[4 * w + e] = (float)(int8_t)(c[w] >> (8 * e));
+    } else {
+      f[4 * w + 0] = __builtin_amdgcn_cvt_f32_fp8((int)c[w], 0);
+      f[4 * w + 1] = __builtin_amdgcn_cvt_f32_fp8((int)c[w], 1);
+      f[4 * w + 2] = __builtin_amdgcn_cvt_f32_fp8((int)c[w], 2);
+      f[4 * w + 3] = __builtin_amdgcn_cvt_f32_fp8((int)c[w], 3);
     }
   }
   return f;
+}
+
+// 8 consecutive stored values of a row, without the row's scale.
+template <int TYPE>
+__device__ __forceinline__ float8v load_page8(const void* base, int64_t off) {
+  if constexpr (TYPE == RFSN_PAGE_FP16) {
+    const half8v h = *reinterpret_cast<const half8v*>((const uint16_t*)base + off);
+    float8v f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = (float)h[e];
+    return f;
+  } else {
+    return page8<TYPE>(*reinterpret_cast<const uint2v*>((const uint8_t*)base + off));
+  }
 }
 
 // Tokens of sequence b that the table can hold.

@@ -54,88 +54,128 @@ struct RowPlace {
   bool start; // the first of them
   bool rest;  // behind the last sequence, or before the first
 };
-// Where the lanes' rows go: row n0 + lane / LANES of the call, one wave, n0 the wave's.
+// Where a wave's rows go: a lane's row i is n0 + i RS + lane / LANES of the call, RS = 64 / LANES.
 // Up to 63 sequences lie in the wave's lanes, so that no load waits for another but the table's.
-template <int LANES>
-__device__ __forceinline__ RowPlace row_place(const rfsn_paged& p, int shift, const int32_t* __restrict__ cu,
-                                              int64_t rows, int64_t n0, int lane) {
-  const int64_t n = n0 + lane / LANES;
-  RowPlace r = {-1, 0, 0, false, true};
-  int64_t i = 0, left = 0;
-  int b = -1, len = 0;
+template <int LANES, int I>
+__device__ __forceinline__ void place_rows(const rfsn_paged& p, int shift, const int32_t* __restrict__ cu, int64_t rows,
+                                           int64_t n0, int lane, RowPlace (&r)[I]) {
+  constexpr int RS = 64 / LANES;
+  const int slot = lane / LANES;
+  int b[I], len[I];
+  int64_t at[I], left[I];
+#pragma unroll
+  for (int i = 0; i < I; ++i) b[i] = -1, len[i] = 0, at[i] = 0, left[i] = 0;
   if (cu == nullptr) {
-    if (n < rows) b = (int)n, left = 1, len = p.lens[b];
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const int64_t n = n0 + i * RS + slot;
+      if (n < rows) b[i] = (int)n, left[i] = 1, len[i] = p.lens[n];
+    }
   } else if (p.batch > 0 && p.batch < 64) {
     const int c = cu[min(lane, p.batch)], ln = p.lens[min(lane, p.batch - 1)];
-    int before = 0;  // bounds at or below the lane's row
+    auto bounds_upto = [&](int64_t n) { return (int)__popcll(__ballot(lane <= p.batch && c <= n)); };
+    int before[I];  // bounds at or below the lane's rows
+    const int x0 = bounds_upto(n0);
 #pragma unroll
-    for (int s = 0; s < 64 / LANES; ++s) {
-      const int x = (int)__popcll(__ballot(lane <= p.batch && c <= n0 + s));
-      if (s == lane / LANES) before = x;
+    for (int i = 0; i < I; ++i) before[i] = x0;
+    if (bounds_upto(n0 + I * RS - 1) != x0) {  // rows of several sequences
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+        for (int s = 0; s < RS; ++s) {
+          const int x = bounds_upto(n0 + i * RS + s);
+          if (s == slot) before[i] = x;
+        }
     }
-    const int at = min(max(before - 1, 0), p.batch - 1);
-    const int64_t c0 = __shfl(c, at, 64), c1 = __shfl(c, at + 1, 64);
-    len = __shfl(ln, at, 64);
-    if (n < rows && n >= c0 && n < c1) b = at, i = n - c0, left = (c1 < rows ? c1 : rows) - n;
-  } else if (p.batch >= 64 && n < rows) {
-    b = row_sequence(cu, p.batch, n);
-    if (b >= 0) {
-      i = n - cu[b];
-      left = (cu[b + 1] < rows ? cu[b + 1] : rows) - n;
-      len = p.lens[b];
-      if (i < 0 || left <= 0) b = -1;  // no prefix
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const int64_t n = n0 + i * RS + slot;
+      const int seq = min(max(before[i] - 1, 0), p.batch - 1);
+      const int64_t c0 = __shfl(c, seq, 64), c1 = __shfl(c, seq + 1, 64);
+      len[i] = __shfl(ln, seq, 64);
+      if (n < rows && n >= c0 && n < c1) b[i] = seq, at[i] = n - c0, left[i] = (c1 < rows ? c1 : rows) - n;
+    }
+  } else if (p.batch >= 64) {
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const int64_t n = n0 + i * RS + slot;
+      if (n >= rows) continue;
+      const int seq = row_sequence(cu, p.batch, n);
+      if (seq < 0) continue;
+      const int64_t c0 = cu[seq], c1 = cu[seq + 1];
+      if (n >= c0 && n < c1) b[i] = seq, at[i] = n - c0, left[i] = (c1 < rows ? c1 : rows) - n, len[i] = p.lens[seq];
     }
   }
-  if (b < 0) return r;
-  const int64_t pos = (int64_t)max(len, 0) + i;
-  r.rest = false;
-  r.page = paged_page(p, b, pos >> shift);
-  r.row = (int)(pos & (p.page_size - 1));
-  r.count = (int)(left < p.page_size - r.row ? left : p.page_size - r.row);
-  r.start = i == 0 || r.row == 0;
-  return r;
-}
-
-// A row's values by the row's largest: rounding is one fp32 product, then the code's own.
-template <int TYPE, int LANES>
-__device__ __forceinline__ void store_row(const rfsn_paged& p, void* base, float* scales, int64_t off, int64_t scale_at,
-                                          half8v x, int chunk, bool write) {
-  if constexpr (TYPE == RFSN_PAGE_FP16) {
-    if (write) *reinterpret_cast<half8v*>((uint16_t*)base + off) = x;
-  } else {
-    uint32_t top = 0;  // |x| as bits: infinity and NaN are the largest
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, (uint32_t)__builtin_bit_cast(uint16_t, (f16)x[e]) & 0x7fffu);
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-    constexpr float kTop = TYPE == RFSN_PAGE_INT8 ? 127.f : 448.f;
-    const bool finite = top < 0x7c00u;
-    const float amax = h2f((uint16_t)top);
-    const float scale = finite ? amax / kTop : __builtin_nanf("");
-    const float inv = finite && top ? kTop / amax : 0.f;
-    uint2v c;
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      float y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = finite ? (float)x[4 * w + e] * inv : 0.f;
-      if constexpr (TYPE == RFSN_PAGE_INT8) {
-        c[w] = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c[w] |= ((uint32_t)(int)rintf(y[e]) & 255u) << (8 * e);
-      } else {
-        int q = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-        c[w] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], q, true);
-      }
-    }
-    if (write) {
-      *reinterpret_cast<uint2v*>((uint8_t*)base + off) = c;
-      if (chunk == 0) scales[scale_at] = scale;
-    }
+  for (int i = 0; i < I; ++i) {
+    r[i] = {-1, 0, 0, false, true};
+    if (b[i] < 0) continue;
+    const int64_t pos = (int64_t)max(len[i], 0) + at[i];
+    r[i].rest = false;
+    r[i].page = paged_page(p, b[i], pos >> shift);
+    r[i].row = (int)(pos & (p.page_size - 1));
+    r[i].count = (int)(left[i] < p.page_size - r[i].row ? left[i] : p.page_size - r[i].row);
+    r[i].start = at[i] == 0 || r[i].row == 0;
   }
 }
 
 typedef unsigned short ushort8v __attribute__((ext_vector_type(8)));
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
+typedef unsigned short ushort4v __attribute__((ext_vector_type(4)));
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_top(uint32_t x) {
+  const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 15, 15, true);
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, x), __builtin_bit_cast(ushort2v, y)));
+}
+// The largest |x| of a K and a V row as bits, K's in the low half: infinity and NaN are the largest.
+template <int LANES>
+__device__ __forceinline__ uint32_t row_tops(half8v k, half8v v) {
+  const ushort8v a = __builtin_bit_cast(ushort8v, k) & (unsigned short)0x7fff;
+  const ushort8v b = __builtin_bit_cast(ushort8v, v) & (unsigned short)0x7fff;
+  const ushort4v a4 = __builtin_elementwise_max(a.lo, a.hi), b4 = __builtin_elementwise_max(b.lo, b.hi);
+  const ushort2v a2 = __builtin_elementwise_max(a4.lo, a4.hi), b2 = __builtin_elementwise_max(b4.lo, b4.hi);
+  const ushort2v even = {a2[0], b2[0]}, odd = {a2[1], b2[1]};
+  uint32_t t = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(even, odd));
+  t = dpp_top<0xb1>(t);   // lanes ^ 1, ^ 2, then mirrored halves of 8 and rows of 16
+  t = dpp_top<0x4e>(t);
+  t = dpp_top<0x141>(t);
+  if constexpr (LANES >= 16) t = dpp_top<0x140>(t);
+  if constexpr (LANES >= 32) {
+    const uint32_t y = (uint32_t)__shfl_xor((int)t, 16, 64);
+    t = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, t), __builtin_bit_cast(ushort2v, y)));
+  }
+  return t;
+}
+
+// 8 values of a row as codes, by the row's largest magnitude: one fp32 product, then
+// the code's own rounding.  A row that is not finite: codes 0, scale NaN.
+template <int TYPE>
+__device__ __forceinline__ uint2v quantise(half8v x, uint32_t top, float& scale) {
+  constexpr float kTop = TYPE == RFSN_PAGE_INT8 ? 127.f : 448.f;
+  const bool finite = top < 0x7c00u;
+  const float amax = h2f((uint16_t)top);
+  scale = finite ? amax / kTop : __builtin_nanf("");
+  const float inv = top ? kTop / amax : 0.f;
+  uint2v c;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (float)x[4 * w + e] * inv;
+    if constexpr (TYPE == RFSN_PAGE_INT8) {
+      uint32_t u[4];  // 1.5 2^23 + y rounds y to the nearest integer, which its low byte then is
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[e] = __builtin_bit_cast(uint32_t, y[e] + 12582912.f);
+      const uint32_t lo = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(u[3], u[2], 0x04000c0cu);
+      c[w] = lo | hi;
+    } else {
+      const int q = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+      c[w] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], q, true);
+    }
+    if (!finite) c[w] = 0;
+  }
+  return c;
+}
 
 // Smallest and largest keys of 8 coordinates, and their largest magnitude's bits, which are past infinity's where one is NaN.
 struct Bounds {
@@ -172,75 +212,133 @@ __device__ __forceinline__ Bounds bounds_of(half8v x) {
   return {x, x, __builtin_bit_cast(ushort8v, x) & (unsigned short)0x7fff};
 }
 
-// A wave writes RS = 64 / (D / 8) rows of one head, K and V; a lane holds 8
+// Block number of a grid of x by y blocks so that each XCD takes a contiguous range of
+// them (hardware deals consecutive blocks to the 8 XCDs in turn).
+__device__ __forceinline__ uint2 xcd_block() {
+  const uint32_t i = blockIdx.y * gridDim.x + blockIdx.x, all = gridDim.x * gridDim.y;
+  const uint32_t x = i & 7, each = all >> 3, more = all & 7;
+  const uint32_t g = x * each + min(x, more) + (i >> 3);
+  return make_uint2(g % gridDim.x, g / gridDim.x);
+}
+
+// Long appends pass the caches by: with 8,191 rows of 8 heads of 64 they take 9.7 us against 11.0, and 22.7
+// with the attention of a token behind them against 23.3; 2,048 rows, which attention finds in the
+// caches, 4.8 against 5.0 alone and 20.7 against 19.2 with it.
+template <bool PASS, typename V>
+__device__ __forceinline__ void store_page(V x, V* at) {
+  if constexpr (PASS) __builtin_nontemporal_store(x, at);
+  else *at = x;
+}
+
+// A wave writes I RS rows of one head, K and V, RS = 64 / (D / 8); a lane holds 8
 // coordinates of a row.  Bounds: the wave of a run's first row (rows of one
-// sequence in one page) reads the run's keys, eight rows of a lane in flight, and writes
-// the page's bounds, so no two waves write the same ones and no order changes them.
-template <int D, int TYPE>
+// sequence in one page) takes those of the run's keys that it holds and reads the others, and
+// writes the page's bounds, so no two waves write the same ones and no order changes them.
+template <int D, int TYPE, int I>
 __global__ void __launch_bounds__(256)
 paged_append_kernel(const rfsn_paged p, int shift, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
                     int64_t ts, int64_t hs, int64_t rows, const int32_t* __restrict__ cu) {
-  constexpr int LANES = D / 8, RS = 64 / LANES, U = 8;
+  constexpr int LANES = D / 8, RS = 64 / LANES, R = I * RS, U = 4;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int h = blockIdx.y * 4 + wave;
+  const uint2 block = xcd_block();  // the rows of a run are in the L2 of the wave that reads them for its bounds
+  const int h = block.y * 4 + wave;
   if (h >= p.kv_heads) return;
   const int slot = lane / LANES, chunk = lane % LANES;
-  const int64_t n0 = (int64_t)blockIdx.x * RS, nc = n0 + slot < rows ? n0 + slot : rows - 1;
-  const half8v kx = *reinterpret_cast<const half8v*>(k + nc * ts + h * hs + chunk * 8);
-  const half8v vx = *reinterpret_cast<const half8v*>(v + nc * ts + h * hs + chunk * 8);
-  const RowPlace at = row_place<LANES>(p, shift, cu, rows, n0, lane);
-  const bool write = at.page >= 0;
-  const int64_t off = (int64_t)(write ? at.page : 0) * p.page_stride + h * p.head_stride + (int64_t)at.row * D + chunk * 8;
-  const int64_t sc = ((int64_t)(write ? at.page : 0) * p.kv_heads + h) * p.page_size + at.row;
-  store_row<TYPE, LANES>(p, p.k, p.k_scale, off, sc, kx, chunk, write);
-  store_row<TYPE, LANES>(p, p.v, p.v_scale, off, sc, vx, chunk, write);
+  const int64_t n0 = (int64_t)block.x * R;
+  const uint16_t* const kh = k + h * hs + chunk * 8;
+  const uint16_t* const vh = v + h * hs + chunk * 8;
+  half8v kx[I], vx[I];
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    const int64_t n = n0 + i * RS + slot < rows ? n0 + i * RS + slot : rows - 1;
+    kx[i] = *reinterpret_cast<const half8v*>(kh + n * ts);
+    vx[i] = *reinterpret_cast<const half8v*>(vh + n * ts);
+  }
+  RowPlace at[I];
+  place_rows<LANES, I>(p, shift, cu, rows, n0, lane, at);
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    const bool write = at[i].page >= 0;
+    const int64_t off = (int64_t)(write ? at[i].page : 0) * p.page_stride + h * p.head_stride + (int64_t)at[i].row * D + chunk * 8;
+    if constexpr (TYPE == RFSN_PAGE_FP16) {
+      if (write) {
+        store_page<(I > 1)>(kx[i], (half8v*)((uint16_t*)p.k + off));
+        store_page<(I > 1)>(vx[i], (half8v*)((uint16_t*)p.v + off));
+      }
+    } else {
+      const int64_t sc = ((int64_t)(write ? at[i].page : 0) * p.kv_heads + h) * p.page_size + at[i].row;
+      const uint32_t tops = row_tops<LANES>(kx[i], vx[i]);
+      float ks, vs;
+      const uint2v kc = quantise<TYPE>(kx[i], tops & 0xffffu, ks), vc = quantise<TYPE>(vx[i], tops >> 16, vs);
+      if (write) {
+        store_page<(I > 1)>(kc, (uint2v*)((uint8_t*)p.k + off));
+        store_page<(I > 1)>(vc, (uint2v*)((uint8_t*)p.v + off));
+        if (chunk == 0) p.k_scale[sc] = ks, p.v_scale[sc] = vs;
+      }
+    }
+  }
   if (p.bounds == nullptr) return;
-  const bool leads = write && at.start;
   auto bounds_at = [&](int page) {
     return reinterpret_cast<half8v*>((uint16_t*)p.bounds + ((int64_t)page * p.kv_heads + h) * 2 * D + chunk * 8);
   };
-  // runs of one row: each row slot on its own; longer ones by the whole wave
-  if (leads && at.count == 1) {
-    half8v* bp = bounds_at(at.page);
-    Bounds m = bounds_of(kx);
-    if (at.row > 0) m.add(bp[0], bp[D / 8]);
-    m.store(bp, bp + D / 8);
-  }
-  uint64_t todo = __ballot(leads && at.count > 1);
-  while (todo) {
-    const int src = __ffsll((unsigned long long)todo) - 1;  // a lane of the run's first row
-    todo &= ~(((1ull << LANES) - 1) << (src / LANES * LANES));
-    const int page = __builtin_amdgcn_readlane(at.page, src), row = __builtin_amdgcn_readlane(at.row, src);
-    const int count = __builtin_amdgcn_readlane(at.count, src);
-    const uint16_t* run = k + (n0 + src / LANES) * ts + h * hs + chunk * 8;
-    half8v* bp = bounds_at(page);
-    const half8v x0 = *reinterpret_cast<const half8v*>(run + min(slot, count - 1) * ts);
-    Bounds m = bounds_of(x0);
-    if (row > 0) m.add(bp[0], bp[D / 8]);
-    for (int i = slot + RS; i - slot < count; i += U * RS) {
-      half8v x[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const half8v*>(run + min(i + u * RS, count - 1) * ts);
-#pragma unroll
-      for (int u = 0; u < U; ++u) m.add(x[u]);
+  for (int i = 0; i < I; ++i) {
+    const bool leads = at[i].page >= 0 && at[i].start;
+    // runs of one row: each row slot on its own; longer ones by the whole wave
+    if (leads && at[i].count == 1) {
+      half8v* bp = bounds_at(at[i].page);
+      Bounds m = bounds_of(kx[i]);
+      if (at[i].row > 0) m.add(bp[0], bp[D / 8]);
+      m.store(bp, bp + D / 8);
     }
+    uint64_t todo = __ballot(leads && at[i].count > 1);
+    while (todo) {
+      const int src = __ffsll((unsigned long long)todo) - 1;  // a lane of the run's first row
+      todo &= ~(((1ull << LANES) - 1) << (src / LANES * LANES));
+      const int page = __builtin_amdgcn_readlane(at[i].page, src), row = __builtin_amdgcn_readlane(at[i].row, src);
+      const int count = __builtin_amdgcn_readlane(at[i].count, src);
+      const int r0 = i * RS + src / LANES, r1 = r0 + count;  // the run's rows, from the wave's first
+      half8v* bp = bounds_at(page);
+      Bounds m = bounds_of(kx[i]);  // a lane whose row is not the run's takes the run's first instead
+      if (i * RS + slot < r0 || i * RS + slot >= r1) m = bounds_of(*reinterpret_cast<const half8v*>(kh + (n0 + r0) * ts));
+      if (row > 0) m.add(bp[0], bp[D / 8]);
 #pragma unroll
-    for (int o = LANES; o < 64; o <<= 1) m.across(o);
-    if (slot == 0) m.store(bp, bp + D / 8);
+      for (int j = i + 1; j < I; ++j)
+        if (j * RS + slot < r1) m.add(kx[j]);
+      for (int j = R + slot; j - slot < r1; j += U * RS) {
+        half8v x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const half8v*>(kh + (n0 + min(j + u * RS, r1 - 1)) * ts);
+#pragma unroll
+        for (int u = 0; u < U; ++u) m.add(x[u]);
+      }
+#pragma unroll
+      for (int o = LANES; o < 64; o <<= 1) m.across(o);
+      if (slot == 0) m.store(bp, bp + D / 8);
+    }
   }
 }
 
+// The reverse, RS rows to a wave.  Four sets of rows per wave are slower at every size
+// (8 heads of 64, fp16: 512 rows 3.5 us against 2.5, 8,192 rows 7.9 against 7.1; 16,384 rows x 32 heads of 128:
+// 128 against 124): nothing is read twice here, and fewer waves wait for their table entry.
+// Blocks in XCD ranges read a page's head in one L2 (16,384 rows x 32 heads of 128: 124 -> 99 us).
+// Non-temporal stores would take 7 % more off the read alone and cost the attention that takes the
+// rows from the caches more (8,191 rows read and attended by 128 queries: 36.8 us against 38.9).
 template <int D, int TYPE>
 __global__ void __launch_bounds__(256)
 paged_read_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ cu, int64_t rows,
                   uint16_t* __restrict__ out_k, uint16_t* __restrict__ out_v, int zero_rest) {
   constexpr int LANES = D / 8, RS = 64 / LANES;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int h = blockIdx.y * 4 + wave;
+  const uint2 block = xcd_block();
+  const int h = block.y * 4 + wave;
   if (h >= p.kv_heads) return;
   const int slot = lane / LANES, chunk = lane % LANES;
-  const int64_t n = (int64_t)blockIdx.x * RS + slot;
-  const RowPlace at = row_place<LANES>(p, shift, cu, rows, (int64_t)blockIdx.x * RS, lane);
+  const int64_t n = (int64_t)block.x * RS + slot;
+  RowPlace place[1];
+  place_rows<LANES, 1>(p, shift, cu, rows, (int64_t)block.x * RS, lane, place);
+  const RowPlace at = place[0];
   if (n >= rows || (at.rest && !zero_rest)) return;
   half8v ko = {}, vo = {};
   if (at.page >= 0) {
@@ -493,10 +591,19 @@ extern "C" int rfsn_paged_append(const rfsn_paged* p, const void* k, const void*
   const int rs = 512 / p->head_dim;
   RFSN_REQUIRE(ceil_div(rows, rs) < (1ll << 24), "paged_append: too many rows");
   const int shift = paged_shift(*p);
-  const dim3 grid((unsigned)ceil_div(rows, rs), (unsigned)ceil_div(p->kv_heads, 4));
+  // Four sets of rows per wave hold most of their pages' rows and read few again for the
+  // bounds, but leave fewer waves.  8 heads of 64, fp16 pages of 16: 512 rows (512 sets) 6.0 us
+  // against 4.1, 4,096 rows 7.1 against 7.3 (int8 7.9 against 7.4), 8,192 rows 11.1 against 11.8;
+  // 16,384 rows x 32 heads of 128: 107 us against 135.
+  const bool four = ceil_div(rows, rs) * p->kv_heads > 4096;
+  const dim3 grid((unsigned)ceil_div(rows, four ? 4 * rs : rs), (unsigned)ceil_div(p->kv_heads, 4));
   RFSN_PAGED_DISPATCH(p->head_dim, p->type, {
-    hipLaunchKernelGGL((paged_append_kernel<DD, TT>), grid, dim3(256), 0, (hipStream_t)stream, *p, shift,
-                       (const uint16_t*)k, (const uint16_t*)v, token_stride, head_stride, rows, cu);
+    if (four)
+      hipLaunchKernelGGL((paged_append_kernel<DD, TT, 4>), grid, dim3(256), 0, (hipStream_t)stream, *p, shift,
+                         (const uint16_t*)k, (const uint16_t*)v, token_stride, head_stride, rows, cu);
+    else
+      hipLaunchKernelGGL((paged_append_kernel<DD, TT, 1>), grid, dim3(256), 0, (hipStream_t)stream, *p, shift,
+                         (const uint16_t*)k, (const uint16_t*)v, token_stride, head_stride, rows, cu);
   });
   return check_launch("paged_append");
 }
