@@ -255,24 +255,33 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
   const int col = lane & 15, grp = lane >> 4;
   const int h = blockIdx.x, w = blockIdx.y, g0 = blockIdx.z * 16;
   const int heads = G - g0 < 16 ? G - g0 : 16;
-  Chunk c;
+  const int step = kWaves * kTile;
+  int b, t0;
+  int64_t t1_cut = 0;
   if (cut.per_seq) {
-    c.b = w / cut.per_seq;
-    c.t0 = (int64_t)(w % cut.per_seq) * cut.chunk;
-    const int64_t end = chosen ? (int64_t)count << shift : paged_len(p, shift, c.b);
-    c.t1 = c.t0 + cut.chunk < end ? c.t0 + cut.chunk : end;
+    b = w / cut.per_seq;
+    t0 = (int)((w - b * cut.per_seq) * cut.chunk);
   } else {
-    c = find_chunk(p, shift, cut, w, lane);
+    const Chunk c = find_chunk(p, shift, cut, w, lane);
     if (c.b < 0) return;
     if (c.j == 0 && h == 0 && g0 == 0 && threadIdx.x == 0) parts.seq[2 * c.b] = w, parts.seq[2 * c.b + 1] = c.n;
+    b = __builtin_amdgcn_readfirstlane(c.b), t0 = __builtin_amdgcn_readfirstlane((int)c.t0), t1_cut = c.t1;
   }
-  c.b = __builtin_amdgcn_readfirstlane(c.b);
-  const int t0 = __builtin_amdgcn_readfirstlane((int)c.t0), t1 = __builtin_amdgcn_readfirstlane((int)c.t1);
-  const int len = __builtin_amdgcn_readfirstlane(paged_len(p, shift, c.b));
-  const int32_t* const list = chosen ? chosen + ((int64_t)c.b * p.kv_heads + h) * count : nullptr;
-  const int32_t* const pages = table + (int64_t)c.b * p.table_stride;
-  const int64_t row0 = ((int64_t)c.b * p.kv_heads + h) * G + g0;  // of q and out
+  const int32_t* const list = chosen ? chosen + ((int64_t)b * p.kv_heads + h) * count : nullptr;
+  const int32_t* const pages = table + (int64_t)b * p.table_stride;
+  const int64_t row0 = ((int64_t)b * p.kv_heads + h) * G + g0;  // of q and out
 
+  // The pages of 64 groups of 16 positions, those of this wave's next 32 tiles, one group a lane:
+  // lane 2 k + u has group u of tile k.  Their loads wait for nothing but a list's.
+  auto ordinal = [&](int tile) {
+    const int64_t t = (int64_t)t0 + wave * kTile + (int64_t)(tile + (lane >> 1)) * step + (lane & 1) * 16;
+    const int64_t ord = t >> shift;
+    if (list == nullptr) return ord;
+    return ord < count ? (int64_t)list[ord] : -1;
+  };
+  auto entry = [&](int64_t ord) { return ord >= 0 && ord < p.table_width ? pages[ord] : -1; };
+  int64_t ord_l = ordinal(0);
+  int page_l = entry(ord_l);
   half8v qf[KS];
   {
     const uint16_t* qr = q + (row0 + (col < heads ? col : heads - 1)) * D;
@@ -280,6 +289,25 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
     for (int s = 0; s < KS; ++s)
       qf[s] = *reinterpret_cast<const half8v*>(qr + (kCodes ? (s >> 1) * 64 + grp * 16 + (s & 1) * 8 : s * 32 + grp * 8));
   }
+  const int len = __builtin_amdgcn_readfirstlane(paged_len(p, shift, b));
+  if (cut.per_seq) {
+    const int64_t end = chosen ? (int64_t)count << shift : len;
+    t1_cut = t0 + cut.chunk < end ? t0 + cut.chunk : end;
+  }
+  const int t1 = __builtin_amdgcn_readfirstlane((int)t1_cut);
+  int rows_l;  // rows of the lane's group that are attended; page_l is a page of the pool from here on
+  auto locate = [&](int tile) {
+    const int64_t t = (int64_t)t0 + wave * kTile + (int64_t)(tile + (lane >> 1)) * step + (lane & 1) * 16;
+    int64_t n = t1 - t;
+    if (list) {
+      const int64_t left = (int64_t)len - ((ord_l << shift) + (t & (p.page_size - 1)));
+      n = left < n ? left : n;
+    }
+    if (page_l < 0 || page_l >= p.pages || n <= 0) n = 0, page_l = 0;
+    rows_l = (int)(n < 16 ? n : 16);
+  };
+  locate(0);
+
   float4v o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = float4v{0.f, 0.f, 0.f, 0.f};
@@ -290,29 +318,12 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
   int n_next[2] = {0, 0};  // rows of the fetched groups that are attended
   // Rows past the last one attended re-read it: their weights are 0.  A group with none
   // reads page 0, and its V is not used.
-  auto fetch = [&](int t) {
+  auto fetch = [&](int t, int tile) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int tu = t + 16 * u;
-      int n = t1 - tu, page = 0, row = tu & (p.page_size - 1);
-      if (n > 0) {
-        int ord = tu >> shift;
-        if (list) {
-          ord = list[ord];
-          const int64_t left = (int64_t)len - (((int64_t)ord << shift) + row);
-          n = ord < 0 || left <= 0 ? 0 : left < 16 ? (int)left : 16;
-        }
-        if (n > 0 && ord < p.table_width) {
-          page = pages[ord];
-          if (page < 0 || page >= p.pages) n = 0;
-        } else {
-          n = 0;
-        }
-      }
-      n = n < 0 ? 0 : n > 16 ? 16 : n;
-      if (n == 0) page = 0;
-      page = __builtin_amdgcn_readfirstlane(page);
-      n = __builtin_amdgcn_readfirstlane(n);
+      const int page = __builtin_amdgcn_readlane(page_l, 2 * (tile & 31) + u);
+      const int n = __builtin_amdgcn_readlane(rows_l, 2 * (tile & 31) + u);
+      const int row = (t + 16 * u) & (p.page_size - 1);
       n_next[u] = n;
       const int last = n > 0 ? n - 1 : 0;
       const int64_t base = ((int64_t)page * p.page_stride + (int64_t)h * p.head_stride + (int64_t)row * D) * ES;
@@ -334,9 +345,8 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
     }
   };
   uint4w* const sv = smem + wave * kTile * CH;
-  const int step = kWaves * kTile;
-  int t = t0 + wave * kTile;
-  if (t < t1) fetch(t);
+  int t = t0 + wave * kTile, tile = 0;
+  if (t < t1) fetch(t, 0);
   for (; t < t1; t += step) {
     int n[2] = {n_next[0], n_next[1]};
     // V to LDS
@@ -383,7 +393,15 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
         }
       }
     }
-    if (t + step < t1) fetch(t + step);
+    ++tile;
+    if (t + step < t1) {
+      if ((tile & 31) == 0) {  // the next 32 tiles
+        ord_l = ordinal(tile);
+        page_l = entry(ord_l);
+        locate(tile);
+      }
+      fetch(t + step, tile);
+    }
     float pw[8], ls;
     auto weights = [&]() {
       const float mb = m_run > -__builtin_inff() ? m_run : 0.f;
@@ -475,7 +493,7 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
     for (int g = wave; g < heads; g += kWaves) {
       const int64_t row = row0 + g;
       float m, l, acc[E];
-      attend_row<D, TYPE>(p, shift, list, c.b, h, c.t0, c.t1, q + row * D, scale_log2, lane, m, l, acc);
+      attend_row<D, TYPE>(p, shift, list, b, h, t0, t1, q + row * D, scale_log2, lane, m, l, acc);
       if (parts.ml == nullptr) {
 #pragma unroll
         for (int e = 0; e < E; ++e) out[row * D + lane * E + e] = f2h(l == 0.f ? 0.f : acc[e] / l);
