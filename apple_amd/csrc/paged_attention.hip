@@ -11,21 +11,42 @@
 namespace rfsn {
 namespace {
 
-__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor((long long)v, o, 64);
-  return v;
+// Inclusive sums, or largest values, of the lanes up to each one, in data-parallel moves
+// (rows of 16, then the rows' last lanes): lane 63 has the wave's.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp0(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 15, true);
+}
+__device__ __forceinline__ uint32_t wave_upto(uint32_t x) {
+  x += dpp0<0x111, 15>(x), x += dpp0<0x112, 15>(x), x += dpp0<0x114, 15>(x), x += dpp0<0x118, 15>(x);
+  x += dpp0<0x142, 10>(x), x += dpp0<0x143, 12>(x);
+  return x;
+}
+__device__ __forceinline__ uint32_t wave_most(uint32_t x) {
+  x = max(x, dpp0<0x111, 15>(x)), x = max(x, dpp0<0x112, 15>(x)), x = max(x, dpp0<0x114, 15>(x));
+  x = max(x, dpp0<0x118, 15>(x)), x = max(x, dpp0<0x142, 10>(x)), x = max(x, dpp0<0x143, 12>(x));
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+__device__ __forceinline__ uint32_t wave_total(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)wave_upto(x), 63);
 }
 
-// How a call is cut (Plan, below): per_seq > 0 gives every sequence that many chunks of
-// `chunk` listed positions (a list of pages, or one chunk); 0 cuts by the lengths, into at
-// most `target` chunks of at least `chunk` positions over their sum and one more per sequence
-// for its last, shorter one.
+// How a call is cut (Plan, below).  per_seq > 0: every sequence into that many chunks of `chunk`
+// listed positions (a list of pages, or one chunk).  0: by the lengths, which only the device
+// knows, into chunks of at least `chunk` positions.
+constexpr int kCUs = 256, kTries = 3;
 struct Cut {
   int per_seq;
-  int target;
+  int units;                // blocks of a chunk (KV heads, and sets of 16 query heads)
   int64_t chunk;
+  float one_over[kTries];   // 1 / chunks aimed at, for so many blocks per CU
 };
+// Chunks aimed at with k blocks on each CU: each sequence adds half of one on average, and a batch
+// that fills the chip by itself is cut where a sequence is longer than the mean.
+inline int aim(int k, int units, int batch) {
+  const int n = k * kCUs / units - batch / 2;
+  return n > batch ? n : batch;
+}
 
 struct Chunk {
   int b;       // sequence, -1: none
@@ -33,35 +54,67 @@ struct Chunk {
   int64_t t0, t1;
 };
 
-// Chunk number w of a batch that is cut by the lengths, by one wave.
+// ceil(len / size) for quotients below 2^20, by a product with the reciprocal (off by less than half then)
+// and a correction of the one that its floor may be off by.
+__device__ __forceinline__ uint32_t parts_of(uint32_t len, uint32_t size) {
+  const uint32_t n = (uint32_t)((float)len * __builtin_amdgcn_rcpf((float)size));
+  const int64_t left = (int64_t)len - (int64_t)n * size;
+  if (left < 0) return left + size == 0 ? n - 1 : n;
+  return left == 0 ? n : left <= (int64_t)size ? n + 1 : n + 2;
+}
+
+// Chunk number w of a batch that is cut by the lengths, by one wave.  Of three sizes, for 2, 3 or 4
+// blocks per CU (1, 2 or 3 of many waves), the one whose fullest CU has the fewest positions: 24 x 5,000
+// positions of 8 KV heads take 51 us as 768 blocks and 57 as 576; 131,072 of one 54 as 512 and 61 as 896.
 __device__ __forceinline__ Chunk find_chunk(const rfsn_paged& p, int shift, const Cut& cut, int w, int lane) {
   const int len0 = lane < p.batch ? paged_len(p, shift, lane) : 0;  // of the first 64, which are most batches
-  int64_t total = len0;
-  for (int b = 64 + lane; b < p.batch; b += 64) total += paged_len(p, shift, b);
-  total = p.batch == 1 ? __builtin_amdgcn_readfirstlane(len0) : wave_sum64(total);
-  int64_t size = (total + cut.target - 1) / cut.target;
-  size = size <= cut.chunk ? cut.chunk : (size + 127) / 128 * 128;
+  float total = 0.f;
+  if (p.batch == 1) {
+    total = (float)__builtin_amdgcn_readfirstlane(len0);
+  } else {  // in 32 bits by wave: lengths below 2^31 in two halves
+    uint64_t sum = ((uint64_t)wave_total((uint32_t)len0 >> 16) << 16) + wave_total((uint32_t)len0 & 0xffffu);
+    for (int base = 64; base < p.batch; base += 64) {
+      const uint32_t len = base + lane < p.batch ? (uint32_t)paged_len(p, shift, base + lane) : 0u;
+      sum += ((uint64_t)wave_total(len >> 16) << 16) + wave_total(len & 0xffffu);
+    }
+    total = (float)sum;
+  }
+  auto about = [](uint32_t len, uint32_t n) { return (uint32_t)((float)len * __builtin_amdgcn_rcpf((float)max(n, 1u))); };
+  uint32_t size = 0;
+  float least = 0.f;
+#pragma unroll
+  for (int x = 0; x < kTries; ++x) {
+    if (x > 0 && p.batch == 1) break;  // of one sequence the chunks are alike: the fewest
+    const float each = total * cut.one_over[x] + 0.98f;  // rounded up, but for an excess that is fp32's
+    uint32_t s = each < 2147483520.f ? (uint32_t)each : 2147483520u;
+    s = s <= (uint32_t)cut.chunk ? (uint32_t)cut.chunk : (s + 127) & ~127u;
+    uint32_t n = parts_of((uint32_t)len0, s), most = about(len0, n);
+    for (int b = 64 + lane; b < p.batch; b += 64) {
+      const uint32_t len = (uint32_t)paged_len(p, shift, b), m = parts_of(len, s);
+      n += m, most = max(most, about(len, m));
+    }
+    if (p.batch > 1) n = wave_total(n), most = wave_most(most);
+    // positions on the fullest CU, each chunk costing as much as 128 more
+    const float cost = (float)((n * (uint32_t)cut.units + kCUs - 1) / kCUs) * ((float)most + 128.f);
+    if (x == 0 || cost < least) least = cost, size = s;
+  }
+  size = __builtin_amdgcn_readfirstlane(size);
   int seen = 0;
   for (int base = 0; base < p.batch; base += 64) {
     const int b = base + lane;
     const int len = base == 0 ? len0 : b < p.batch ? paged_len(p, shift, b) : 0;
-    const int n = (int)((len + size - 1) / size);
-    int upto = n;  // inclusive prefix over the wave
-    if (p.batch > 1) {
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(upto, o, 64);
-        if (lane >= o) upto += x;
-      }
-    }
+    const int n = (int)parts_of((uint32_t)len, size);
+    const int upto = p.batch > 1 ? (int)wave_upto((uint32_t)n) : n;
     const uint64_t in = __ballot(w < seen + upto && w >= seen + upto - n);
     if (in) {
       const int src = __ffsll((unsigned long long)in) - 1;
-      const int j = w - seen - __shfl(upto - n, src, 64);
-      const int64_t t0 = (int64_t)j * size, end = __shfl(len, src, 64);
-      return {base + src, j, __shfl(n, src, 64), t0, t0 + size < end ? t0 + size : end};
+      const int of = __builtin_amdgcn_readlane(n, src), j = w - seen - __builtin_amdgcn_readlane(upto, src) + of;
+      const int64_t end = __builtin_amdgcn_readlane(len, src);
+      // the sequence's chunks are alike
+      const int64_t part = (int64_t)(((uint32_t)end + (uint32_t)of - 1) / (uint32_t)of + 127) & ~127ll, t0 = j * part;
+      return {base + src, j, of, t0 < end ? t0 : end, t0 + part < end ? t0 + part : end};
     }
-    seen += __shfl(upto, 63, 64);
+    seen += __builtin_amdgcn_readlane(upto, 63);
   }
   return {-1, 0, 0, 0, 0};
 }
@@ -146,7 +199,7 @@ __device__ __forceinline__ void attend_row(const rfsn_paged& p, int shift, const
 
 // ---- tiles on the matrix cores
 //
-// A wave takes 32 positions at a time (two groups of 16, each inside one page), a
+// A wave takes NG groups of 16 positions at a time (each inside one page), a
 // block's waves take them in turn, and a lane's 16 columns are the query heads of the KV
 // head (the others repeat the last: the matrix cores are idle otherwise).
 //   S = K Q^T      MFMA 16x16x32, A = 16 rows of K as they lie in memory (16 bytes a
@@ -170,12 +223,11 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short short4w __attribute__((ext_vector_type(4)));
 typedef short short8w __attribute__((ext_vector_type(8)));
 
-constexpr int kTile = 32;          // positions per wave and step
-constexpr int kWideTiles = 8192;   // tiles of a call up to which blocks have many waves
+constexpr int kWideTiles = 8192;   // tiles of 32 positions of a call up to which blocks have many waves
 constexpr float kPBias = 8.f;      // a weight is kept as p 2^8
 constexpr float kPSum = 32768.f;   // a lane's sum below it: every weight is finite in fp16
 
-// 16-byte chunk c of row t of the [32][D] 16-bit tile sits at chunk c ^ v_swz(t): the
+// 16-byte chunk c of row t of a [16 NG][D] 16-bit tile sits at chunk c ^ v_swz(t): the
 // transposed reads take 32 bytes of 8 rows at once, which then lie in different banks.
 template <int D>
 __device__ __forceinline__ int v_swz(int t) { return D == 64 ? ((t >> 1) & 3) << 1 : (t & 7) << 1; }
@@ -234,8 +286,8 @@ struct Parts {
   int32_t* seq; // [batch][2]
 };
 
-template <int D, int TYPE, int kWaves>
-__global__ void __launch_bounds__(kWaves * 64, kWaves > 4 ? 1 : D == 64 ? 4 : D == 128 ? 2 : 1)
+template <int D, int TYPE, int kWaves, int NG>
+__global__ void __launch_bounds__(kWaves * 64, kWaves > 4 ? 1 : D == 64 ? (NG > 2 ? 3 : 4) : D == 128 ? 2 : 1)
 paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ table, const uint16_t* __restrict__ q, int G,
                   float scale_log2, const int32_t* __restrict__ chosen, int count, const Cut cut,
                   uint16_t* __restrict__ out, const Parts parts) {
@@ -246,7 +298,9 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
   constexpr int KL = D * ES / 64;                    // 16-byte loads of a lane's share of a K row
   constexpr int DT = D / 16;                         // 16-coordinate tiles of O^T
   constexpr int VC = D * ES / 16;                    // 16-byte chunks of a stored row
-  constexpr int VL = kTile * VC / 64;                // V loads of a lane
+  constexpr int kTile = 16 * NG;                     // positions per wave and step
+  constexpr int GT = 64 / NG;                        // tiles whose groups fill a wave's lanes
+  constexpr int VU = 16 * VC / 64;                   // V loads of a lane for a group
   constexpr int CH = D / 8;                          // 16-byte chunks of a row in LDS
   __shared__ uint4w smem[kWaves * kTile * CH];       // V tiles; then the waves' O, m, l
   __shared__ float s_ml[kWaves][2][16];
@@ -271,10 +325,10 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
   const int32_t* const pages = table + (int64_t)b * p.table_stride;
   const int64_t row0 = ((int64_t)b * p.kv_heads + h) * G + g0;  // of q and out
 
-  // The pages of 64 groups of 16 positions, those of this wave's next 32 tiles, one group a lane:
-  // lane 2 k + u has group u of tile k.  Their loads wait for nothing but a list's.
+  // The pages of 64 groups of 16 positions, those of this wave's next GT tiles, one group a lane:
+  // lane NG k + u has group u of tile k.  Their loads wait for nothing but a list's.
   auto ordinal = [&](int tile) {
-    const int64_t t = (int64_t)t0 + wave * kTile + (int64_t)(tile + (lane >> 1)) * step + (lane & 1) * 16;
+    const int64_t t = (int64_t)t0 + wave * kTile + (int64_t)(tile + lane / NG) * step + lane % NG * 16;
     const int64_t ord = t >> shift;
     if (list == nullptr) return ord;
     return ord < count ? (int64_t)list[ord] : -1;
@@ -297,7 +351,7 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
   const int t1 = __builtin_amdgcn_readfirstlane((int)t1_cut);
   int rows_l;  // rows of the lane's group that are attended; page_l is a page of the pool from here on
   auto locate = [&](int tile) {
-    const int64_t t = (int64_t)t0 + wave * kTile + (int64_t)(tile + (lane >> 1)) * step + (lane & 1) * 16;
+    const int64_t t = (int64_t)t0 + wave * kTile + (int64_t)(tile + lane / NG) * step + lane % NG * 16;
     int64_t n = t1 - t;
     if (list) {
       const int64_t left = (int64_t)len - ((ord_l << shift) + (t & (p.page_size - 1)));
@@ -313,34 +367,34 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
   for (int d = 0; d < DT; ++d) o[d] = float4v{0.f, 0.f, 0.f, 0.f};
   float m_run = -__builtin_inff(), l_run = 0.f;  // reference exponent of the head's weights, this lane's sum of them
 
-  uint4w kr[2][KL], vr[VL];
-  float4v ks[2], vs[2];
-  int n_next[2] = {0, 0};  // rows of the fetched groups that are attended
+  uint4w kr[NG][KL], vr[NG][VU];
+  float4v ks[NG], vs[NG];
+  int n_next[NG] = {};  // rows of the fetched groups that are attended
   // Rows past the last one attended re-read it: their weights are 0.  A group with none
   // reads page 0, and its V is not used.
   auto fetch = [&](int t, int tile) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int page = __builtin_amdgcn_readlane(page_l, 2 * (tile & 31) + u);
-      const int n = __builtin_amdgcn_readlane(rows_l, 2 * (tile & 31) + u);
+    for (int u = 0; u < NG; ++u) {
+      const int page = __builtin_amdgcn_readlane(page_l, NG * (tile % GT) + u);
+      const int n = __builtin_amdgcn_readlane(rows_l, NG * (tile % GT) + u);
       const int row = (t + 16 * u) & (p.page_size - 1);
       n_next[u] = n;
       const int last = n > 0 ? n - 1 : 0;
       const int64_t base = ((int64_t)page * p.page_stride + (int64_t)h * p.head_stride + (int64_t)row * D) * ES;
       const uint8_t* kb = (const uint8_t*)p.k + base;
       const uint8_t* vb = (const uint8_t*)p.v + base;
-      const int kl = min(col, last) * (D * ES) + grp * 16;
+      const uint32_t kl = (uint32_t)(min(col, last) * (D * ES) + grp * 16);
 #pragma unroll
       for (int i = 0; i < KL; ++i) kr[u][i] = *reinterpret_cast<const uint4w*>(kb + kl + i * 64);
 #pragma unroll
-      for (int i = 0; i < VL / 2; ++i) {
+      for (int i = 0; i < VU; ++i) {
         const int idx = i * 64 + lane, r = idx / VC, ch = idx % VC;
-        vr[u * (VL / 2) + i] = *reinterpret_cast<const uint4w*>(vb + min(r, last) * (D * ES) + ch * 16);
+        vr[u][i] = *reinterpret_cast<const uint4w*>(vb + (uint32_t)(min(r, last) * (D * ES) + ch * 16));
       }
       if constexpr (kCodes) {
-        const int64_t sc = ((int64_t)page * p.kv_heads + h) * p.page_size + row + grp * 4;
-        ks[u] = *reinterpret_cast<const float4v*>(p.k_scale + sc);
-        vs[u] = *reinterpret_cast<const float4v*>(p.v_scale + sc);
+        const int64_t sc = ((int64_t)page * p.kv_heads + h) * p.page_size + row;
+        ks[u] = *reinterpret_cast<const float4v*>(p.k_scale + sc + (uint32_t)(grp * 4));
+        vs[u] = *reinterpret_cast<const float4v*>(p.v_scale + sc + (uint32_t)(grp * 4));
       }
     }
   };
@@ -348,24 +402,28 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
   int t = t0 + wave * kTile, tile = 0;
   if (t < t1) fetch(t, 0);
   for (; t < t1; t += step) {
-    int n[2] = {n_next[0], n_next[1]};
+    int n[NG];
+#pragma unroll
+    for (int u = 0; u < NG; ++u) n[u] = n_next[u];
     // V to LDS
 #pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      const int idx = (i % (VL / 2)) * 64 + lane, r = (i / (VL / 2)) * 16 + idx / VC, ch = idx % VC;
-      uint4w x = vr[i];
-      if (n[i / (VL / 2)] == 0) x = uint4w{0, 0, 0, 0};
-      if constexpr (!kCodes) {
-        sv[r * CH + (ch ^ v_swz<D>(r))] = x;
-      } else {
-        sv[r * CH + ((2 * ch) ^ v_swz<D>(r))] = codes_bf16<TYPE>(x[0], x[1]);
-        sv[r * CH + ((2 * ch + 1) ^ v_swz<D>(r))] = codes_bf16<TYPE>(x[2], x[3]);
-      }
-    }
-    // scores in base 2
-    float4v s[2];
+    for (int u = 0; u < NG; ++u)
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+      for (int i = 0; i < VU; ++i) {
+        const int idx = i * 64 + lane, r = u * 16 + idx / VC, ch = idx % VC;
+        uint4w x = vr[u][i];
+        if (n[u] == 0) x = uint4w{0, 0, 0, 0};
+        if constexpr (!kCodes) {
+          sv[r * CH + (ch ^ v_swz<D>(r))] = x;
+        } else {
+          sv[r * CH + ((2 * ch) ^ v_swz<D>(r))] = codes_bf16<TYPE>(x[0], x[1]);
+          sv[r * CH + ((2 * ch + 1) ^ v_swz<D>(r))] = codes_bf16<TYPE>(x[2], x[3]);
+        }
+      }
+    // scores in base 2
+    float4v s[NG];
+#pragma unroll
+    for (int u = 0; u < NG; ++u) {
       s[u] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
@@ -375,9 +433,9 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
         s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[k], s[u], 0, 0, 0);
       }
     }
-    float4v vscale[2];
+    float4v vscale[NG];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < NG; ++u) {
       if constexpr (kCodes) {
         s[u] *= ks[u];
         vscale[u] = vs[u];
@@ -395,19 +453,19 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
     }
     ++tile;
     if (t + step < t1) {
-      if ((tile & 31) == 0) {  // the next 32 tiles
+      if (tile % GT == 0) {  // the next GT tiles
         ord_l = ordinal(tile);
         page_l = entry(ord_l);
         locate(tile);
       }
       fetch(t + step, tile);
     }
-    float pw[8], ls;
+    float pw[4 * NG], ls;
     auto weights = [&]() {
       const float mb = m_run > -__builtin_inff() ? m_run : 0.f;
       ls = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 4 * NG; ++i) {
         pw[i] = __builtin_amdgcn_exp2f(s[i >> 2][i & 3] - mb);
         ls += pw[i];
       }
@@ -416,8 +474,9 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
     // The maximum is moved only when a lane's sum says that a weight may leave
     // fp16's range (or nothing was seen yet): no weight exceeds the sum.
     if (__any(!(ls < kPSum) || m_run == -__builtin_inff())) {
-      float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      float mx = s[0][0];
+#pragma unroll
+      for (int i = 1; i < 4 * NG; ++i) mx = fmaxf(mx, s[i >> 2][i & 3]);
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
       const float m_new = fmaxf(m_run, mx - kPBias);
@@ -429,9 +488,9 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
       weights();
     }
     l_run += ls;
-    uint4w bh, bl;  // 8 weights as the B operand, high and low parts
+    uint32_t bh[2 * NG], bl[2 * NG];  // weights as B operands of 8, high and low parts
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2 * NG; ++i) {
       if constexpr (!kCodes) {
         const half2w hi = {(f16)pw[2 * i], (f16)pw[2 * i + 1]};
         const half2w lo = {(f16)(pw[2 * i] - (float)hi[0]), (f16)(pw[2 * i + 1] - (float)hi[1])};
@@ -447,30 +506,36 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
     __builtin_amdgcn_wave_barrier();
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      typedef __attribute__((address_space(3))) short4w lds4;
-      short4w a[2];
+    for (int x = 0; x < NG / 2; ++x) {
+      const uint4w hi = {bh[4 * x], bh[4 * x + 1], bh[4 * x + 2], bh[4 * x + 3]};
+      const uint4w lo = {bl[4 * x], bl[4 * x + 1], bl[4 * x + 2], bl[4 * x + 3]};
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int tv = 16 * e + 4 * grp + (col >> 2), cc = 2 * d + ((col & 3) >> 1);
-        const int off = (tv * CH + (cc ^ v_swz<D>(tv))) * 16 + (col & 1) * 8;
-        a[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)((__attribute__((address_space(3))) char*)sv + off));
-      }
-      const short8w av = {a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]};
-      if constexpr (!kCodes) {
-        const half8v vf = __builtin_bit_cast(half8v, av);
-        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_bit_cast(half8v, bh), o[d], 0, 0, 0);
-        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_bit_cast(half8v, bl), o[d], 0, 0, 0);
-      } else {
-        const bf16x8 vf = __builtin_bit_cast(bf16x8, av);
-        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8, bh), o[d], 0, 0, 0);
-        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8, bl), o[d], 0, 0, 0);
+      for (int d = 0; d < DT; ++d) {
+        typedef __attribute__((address_space(3))) short4w lds4;
+        short4w a[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int tv = 32 * x + 16 * e + 4 * grp + (col >> 2), cc = 2 * d + ((col & 3) >> 1);
+          const int off = (tv * CH + (cc ^ v_swz<D>(tv))) * 16 + (col & 1) * 8;
+          a[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)((__attribute__((address_space(3))) char*)sv + off));
+        }
+        const short8w av = {a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]};
+        if constexpr (!kCodes) {
+          const half8v vf = __builtin_bit_cast(half8v, av);
+          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_bit_cast(half8v, hi), o[d], 0, 0, 0);
+          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, __builtin_bit_cast(half8v, lo), o[d], 0, 0, 0);
+        } else {
+          const bf16x8 vf = __builtin_bit_cast(bf16x8, av);
+          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8, hi), o[d], 0, 0, 0);
+          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8, lo), o[d], 0, 0, 0);
+        }
       }
     }
     __builtin_amdgcn_wave_barrier();
     asm volatile("" ::: "memory");
   }
 
+  static_assert(kTile * CH * 16 >= DT * 64 * 16, "a wave's O fits its V tile");
   float zero = l_run * 0.f;  // NaN where a sum is infinite or NaN
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -484,7 +549,7 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
   if (grp == 0) s_ml[wave][0][col] = m_run, s_ml[wave][1][col] = l_run;
   // the waves' V tiles are done with: each wave's O lies over its own
 #pragma unroll
-  for (int d = 0; d < DT; ++d) *reinterpret_cast<float4v*>(so + ((wave * DT + d) * 64 + lane) * 4) = o[d];
+  for (int d = 0; d < DT; ++d) *reinterpret_cast<float4v*>(so + wave * (kTile * CH * 4) + (d * 64 + lane) * 4) = o[d];
   __syncthreads();
   int any = s_odd[0];
 #pragma unroll
@@ -521,7 +586,7 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
   for (int d = wave; d < DT; d += kWaves) {
     float4v a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int x = 0; x < kWaves; ++x) a += f[x] * *reinterpret_cast<const float4v*>(so + ((x * DT + d) * 64 + lane) * 4);
+    for (int x = 0; x < kWaves; ++x) a += f[x] * *reinterpret_cast<const float4v*>(so + x * (kTile * CH * 4) + (d * 64 + lane) * 4);
     if (col >= heads) continue;
     if (parts.ml == nullptr) {
       const half4w r = {(f16)(a[0] * inv), (f16)(a[1] * inv), (f16)(a[2] * inv), (f16)(a[3] * inv)};
@@ -534,11 +599,11 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
 
 // out = sum_j w_j acc_j / sum_j w_j l_j over a sequence's chunks, w_j = 2^(m_j - max m).
 // The (m, l) of 64 chunks are one load of a wave, and the rows of O do not wait for them.
-template <int D>
-__global__ void __launch_bounds__(256)
+template <int D, int W>
+__global__ void __launch_bounds__(W * 64)
 paged_merge_kernel(const rfsn_paged p, int shift, int q_heads, int per_seq, const Parts parts, uint16_t* __restrict__ out) {
   constexpr int E = D / 64, U = 4;
-  __shared__ float s_l[4], s_acc[4][D];
+  __shared__ float s_acc[W][D];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = blockIdx.x, b = blockIdx.y;
   int slot0 = b * per_seq, n = per_seq;
@@ -563,19 +628,19 @@ paged_merge_kernel(const rfsn_paged p, int shift, int q_heads, int per_seq, cons
     l = l * corr + wave_sum(lane < here ? wj * lj : 0.f);
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] *= corr;
-    for (int j0 = wave; j0 < here; j0 += 4 * U) {
+    for (int j0 = wave; j0 < here; j0 += W * U) {
       float x[U][E];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int j = min(j0 + 4 * u, here - 1);
+        const int j = min(j0 + W * u, here - 1);
         const float* a = parts.acc + ((int64_t)(slot0 + base + j) * q_heads + i) * D + lane * E;
 #pragma unroll
         for (int e = 0; e < E; ++e) x[u][e] = a[e];
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (j0 + 4 * u >= here) break;
-        const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wj), j0 + 4 * u));
+        if (j0 + W * u >= here) break;
+        const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wj), j0 + W * u));
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = fmaf(w, x[u][e], acc[e]);
       }
@@ -585,8 +650,10 @@ paged_merge_kernel(const rfsn_paged p, int shift, int q_heads, int per_seq, cons
 #pragma unroll
   for (int e = 0; e < E; ++e) s_acc[wave][lane * E + e] = acc[e];
   __syncthreads();
-  for (int d = threadIdx.x; d < D; d += 256) {
-    const float a = s_acc[0][d] + s_acc[1][d] + s_acc[2][d] + s_acc[3][d];
+  for (int d = threadIdx.x; d < D; d += W * 64) {
+    float a = s_acc[0][d];
+#pragma unroll
+    for (int x = 1; x < W; ++x) a += s_acc[x][d];
     out[((int64_t)b * q_heads + i) * D + d] = f2h(l == 0.f ? 0.f : a / l);
   }
 }
@@ -601,27 +668,33 @@ struct Plan {
 int waves_of(int D, bool wide) { return !wide || D == 256 ? 4 : D == 64 ? 16 : 8; }  // (256: 8 would spill)
 Plan plan(const rfsn_paged& p, int q_heads, int count) {
   const int64_t most = (int64_t)(count ? count : p.table_width) * p.page_size;
-  const int64_t units = (int64_t)p.kv_heads * ceil_div(q_heads / p.kv_heads, 16);  // blocks of a chunk
+  const int units = (int)(p.kv_heads * ceil_div(q_heads / p.kv_heads, 16));
   Plan r;
-  r.wide = (int64_t)p.batch * units * ceil_div(most, kTile) <= kWideTiles;
-  const int per_step = waves_of(p.head_dim, r.wide) * kTile;
+  r.wide = (int64_t)p.batch * units * ceil_div(most, 32) <= kWideTiles;
+  const int per_step = waves_of(p.head_dim, r.wide) * 32;
   const int64_t least = r.wide ? per_step : 4 * per_step;  // positions of a chunk
   if (most <= 4 * per_step) {
-    r.slots = p.batch, r.cut = {1, 0, most > 0 ? most : 1};
-    return r;
-  }
-  const int64_t want = ceil_div(r.wide ? 256 : 1024, units);  // chunks that fill the chip
-  if (count) {
-    int64_t n = ceil_div(want, p.batch);
+    r.slots = p.batch, r.cut = {1, units, most > 0 ? most : 1, {}};
+  } else if (count) {
+    int64_t n = ceil_div(r.wide ? kCUs : 4 * kCUs, (int64_t)units * p.batch);
     if (n > ceil_div(most, least)) n = ceil_div(most, least);
     const int64_t chunk = ceil_div(ceil_div(most, n), per_step) * per_step;
     n = ceil_div(most, chunk);
-    r.slots = n * p.batch, r.cut = {(int)n, 0, chunk};
-    return r;
+    r.slots = n * p.batch, r.cut = {(int)n, units, chunk, {}};
+  } else {
+    const int first = r.wide ? 1 : 2;
+    r.cut = {0, units, least, {}};
+    int64_t most_chunks = 0;
+    for (int x = 0; x < kTries; ++x) {
+      const int n = aim(first + x, units, p.batch);
+      r.cut.one_over[x] = 1.f / (float)n;
+      most_chunks = n > most_chunks ? n : most_chunks;
+    }
+    // The sum of ceil(len / size) is at most total / size + batch, and size at least total / target - 0.02
+    // (find_chunk) or 128 and more, which is 32767 (0.02 / 512 + 2^-21) < 2 chunks over the target.
+    r.slots = most_chunks + 2 + p.batch;
+    if (r.slots > ceil_div(most, least) * p.batch) r.slots = ceil_div(most, least) * p.batch;
   }
-  int64_t target = want;
-  if (target > ceil_div(most, least) * p.batch) target = ceil_div(most, least) * p.batch;
-  r.slots = target + p.batch, r.cut = {0, (int)target, least};
   return r;
 }
 size_t parts_bytes(const rfsn_paged& p, const Plan& c, int q_heads) {
@@ -666,28 +739,36 @@ extern "C" int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t 
     parts.seq = (int32_t*)(parts.ml + c.slots * q_heads * 2);
   }
   const dim3 grid((unsigned)p->kv_heads, (unsigned)c.slots, (unsigned)ceil_div(G, 16));
-#define RFSN_ATTEND(DD, TT, NW)                                                                                     \
-  hipLaunchKernelGGL((paged_attn_kernel<DD, TT, NW>), grid, dim3(NW * 64), 0, s, *p, shift, p->table,               \
+#define RFSN_ATTEND(DD, TT, NW, NG)                                                                                 \
+  hipLaunchKernelGGL((paged_attn_kernel<DD, TT, NW, NG>), grid, dim3(NW * 64), 0, s, *p, shift, p->table,           \
                      (const uint16_t*)q, G, sl2, chosen, count, c.cut, (uint16_t*)out, parts)
-#define RFSN_ATTEND_D(DD, NW)                                            \
-  do {                                                                   \
-    if (p->type == RFSN_PAGE_FP16) RFSN_ATTEND(DD, RFSN_PAGE_FP16, NW);  \
-    else if (p->type == RFSN_PAGE_INT8) RFSN_ATTEND(DD, RFSN_PAGE_INT8, NW); \
-    else RFSN_ATTEND(DD, RFSN_PAGE_E4M3, NW);                            \
+#define RFSN_ATTEND_D(DD, NW, NG, NG8)                                            \
+  do {                                                                            \
+    if (p->type == RFSN_PAGE_FP16) RFSN_ATTEND(DD, RFSN_PAGE_FP16, NW, NG);       \
+    else if (p->type == RFSN_PAGE_INT8) RFSN_ATTEND(DD, RFSN_PAGE_INT8, NW, NG8); \
+    else RFSN_ATTEND(DD, RFSN_PAGE_E4M3, NW, NG8);                                \
   } while (0)
-  if (p->head_dim == 64 && c.wide) RFSN_ATTEND_D(64, 16);
-  else if (p->head_dim == 64) RFSN_ATTEND_D(64, 4);
-  else if (p->head_dim == 128 && c.wide) RFSN_ATTEND_D(128, 8);
-  else if (p->head_dim == 128) RFSN_ATTEND_D(128, 4);
-  else RFSN_ATTEND_D(256, 4);
+  if (p->head_dim == 64 && c.wide) RFSN_ATTEND_D(64, 16, 2, 2);
+  else if (p->head_dim == 64) RFSN_ATTEND_D(64, 4, 2, 2);
+  else if (p->head_dim == 128 && c.wide) RFSN_ATTEND_D(128, 8, 2, 2);
+  else if (p->head_dim == 128) RFSN_ATTEND_D(128, 4, 2, 2);
+  else RFSN_ATTEND_D(256, 4, 2, 2);
 #undef RFSN_ATTEND_D
 #undef RFSN_ATTEND
   if (int st = check_launch("paged_attention")) return st;
   if (c.split()) {
     const dim3 rows((unsigned)q_heads, (unsigned)p->batch);
-#define RFSN_MERGE(DD)                                                                                           \
-  hipLaunchKernelGGL(paged_merge_kernel<DD>, rows, dim3(256), 0, s, *p, shift, q_heads, c.cut.per_seq, parts, \
-                     (uint16_t*)out)
+    // chunks a sequence may have: with few, four waves a row, with many a wave for each of 16
+    const bool many = (c.cut.per_seq ? c.cut.per_seq : c.slots - p->batch + 1) > 16 && (int64_t)q_heads * p->batch <= 256;
+#define RFSN_MERGE(DD)                                                                                              \
+  do {                                                                                                              \
+    if (many)                                                                                                       \
+      hipLaunchKernelGGL((paged_merge_kernel<DD, 16>), rows, dim3(1024), 0, s, *p, shift, q_heads, c.cut.per_seq,   \
+                         parts, (uint16_t*)out);                                                                    \
+    else                                                                                                            \
+      hipLaunchKernelGGL((paged_merge_kernel<DD, 4>), rows, dim3(256), 0, s, *p, shift, q_heads, c.cut.per_seq,     \
+                         parts, (uint16_t*)out);                                                                    \
+  } while (0)
     if (p->head_dim == 64) RFSN_MERGE(64);
     else if (p->head_dim == 128) RFSN_MERGE(128);
     else RFSN_MERGE(256);
