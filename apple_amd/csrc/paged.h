@@ -62,4 +62,24 @@ __device__ __forceinline__ int paged_page(const rfsn_paged& p, int b, int64_t or
   return n >= 0 && n < p.pages ? n : -1;
 }
 
+// Inclusive sums, or largest values, of the lanes up to each one, in data-parallel moves
+// (rows of 16, then the rows' last lanes): lane 63 has the wave's.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp0(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 15, true);
+}
+__device__ __forceinline__ uint32_t wave_upto(uint32_t x) {
+  x += dpp0<0x111, 15>(x), x += dpp0<0x112, 15>(x), x += dpp0<0x114, 15>(x), x += dpp0<0x118, 15>(x);
+  x += dpp0<0x142, 10>(x), x += dpp0<0x143, 12>(x);
+  return x;
+}
+__device__ __forceinline__ uint32_t wave_most(uint32_t x) {
+  x = max(x, dpp0<0x111, 15>(x)), x = max(x, dpp0<0x112, 15>(x)), x = max(x, dpp0<0x114, 15>(x));
+  x = max(x, dpp0<0x118, 15>(x)), x = max(x, dpp0<0x142, 10>(x)), x = max(x, dpp0<0x143, 12>(x));
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+__device__ __forceinline__ uint32_t wave_total(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)wave_upto(x), 63);
+}
+
 }  // namespace rfsn

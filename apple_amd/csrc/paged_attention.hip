@@ -11,26 +11,6 @@
 namespace rfsn {
 namespace {
 
-// Inclusive sums, or largest values, of the lanes up to each one, in data-parallel moves
-// (rows of 16, then the rows' last lanes): lane 63 has the wave's.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp0(uint32_t x) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 15, true);
-}
-__device__ __forceinline__ uint32_t wave_upto(uint32_t x) {
-  x += dpp0<0x111, 15>(x), x += dpp0<0x112, 15>(x), x += dpp0<0x114, 15>(x), x += dpp0<0x118, 15>(x);
-  x += dpp0<0x142, 10>(x), x += dpp0<0x143, 12>(x);
-  return x;
-}
-__device__ __forceinline__ uint32_t wave_most(uint32_t x) {
-  x = max(x, dpp0<0x111, 15>(x)), x = max(x, dpp0<0x112, 15>(x)), x = max(x, dpp0<0x114, 15>(x));
-  x = max(x, dpp0<0x118, 15>(x)), x = max(x, dpp0<0x142, 10>(x)), x = max(x, dpp0<0x143, 12>(x));
-  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
-}
-__device__ __forceinline__ uint32_t wave_total(uint32_t x) {
-  return (uint32_t)__builtin_amdgcn_readlane((int)wave_upto(x), 63);
-}
-
 // How a call is cut (Plan, below).  per_seq > 0: every sequence into that many chunks of `chunk`
 // listed positions (a list of pages, or one chunk).  0: by the lengths, which only the device
 // knows, into chunks of at least `chunk` positions.

@@ -731,13 +731,15 @@ def _paged(what: str, pages: KVPages, table: torch.Tensor, lens: torch.Tensor) -
     """The checked parameter block of a pool, a block table [B, W] int32 and
     lengths [B] int32: (block, (B, Hkv, D, S, W), device index)."""
     k, v, ks, vs, bounds = pages
-    dev = _dev(k, what).get_device()
-    if k.dim() != 4 or v.dim() != 4:
+    dev = k.get_device()
+    if dev < 0:
+        L.require_device(k, what)
+    shape, strides, dtype = k.shape, k.stride(), k.dtype
+    if len(shape) != 4:
         raise ValueError(f"{what}: k and v pages must be [pages, kv_heads, page_size, head_dim]")
-    shape, (sp, sh, ss, sd), dtype = k.shape, k.stride(), k.dtype
-    if v.shape != shape or v.dtype is not dtype or v.stride() != (sp, sh, ss, sd):
+    if v.shape != shape or v.dtype is not dtype or v.stride() != strides:
         raise ValueError(f"{what}: k and v pages must be of one shape, type and stride")
-    P, H, S, D = shape
+    (P, H, S, D), (sp, sh, ss, sd) = shape, strides
     kind = PAGE_TYPES.get(dtype)
     if kind is None:
         raise ValueError(f"{what}: pages of {dtype}; float16, int8 and float8_e4m3fn are served")
@@ -759,9 +761,10 @@ def _paged(what: str, pages: KVPages, table: torch.Tensor, lens: torch.Tensor) -
             raise ValueError(f"{what}: bounds must be contiguous fp16 {[P, H, 2, D]}")
         apart = apart or bounds.get_device() != dev
         bounds = bounds.data_ptr()
-    if table.dim() != 2 or table.dtype is not torch.int32:
+    shape = table.shape
+    if len(shape) != 2 or table.dtype is not torch.int32:
         raise ValueError(f"{what}: the block table must be int32 [batch, pages per sequence]")
-    (B, W), (st, sw) = table.shape, table.stride()
+    (B, W), (st, sw) = shape, table.stride()
     if sw != 1 and W > 1:
         raise ValueError(f"{what}: the block table's rows must be dense")
     if lens.dtype is not torch.int32 or lens.shape != (B,) or not lens.is_contiguous():
@@ -776,11 +779,14 @@ def _paged(what: str, pages: KVPages, table: torch.Tensor, lens: torch.Tensor) -
 
 def _paged_call(device: int, name: str, *args) -> None:
     """The call on the device's current stream, whichever device is current."""
-    if device == torch.cuda.current_device():
-        L.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+    fn = getattr(L.load(), name)
+    if device == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            L.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        L.check(status, name)
 
 
 def _cu(what: str, cu: torch.Tensor, batch: int, device: int) -> int:
@@ -790,7 +796,8 @@ def _cu(what: str, cu: torch.Tensor, batch: int, device: int) -> int:
 
 
 def _paged_query(what: str, q: torch.Tensor, batch: int, head_dim: int, device: int) -> torch.Tensor:
-    if q.dim() != 3 or q.dtype is not torch.float16 or q.shape[0] != batch or q.shape[2] != head_dim \
+    shape = q.shape
+    if len(shape) != 3 or q.dtype is not torch.float16 or shape[0] != batch or shape[2] != head_dim \
             or q.get_device() != device:
         raise ValueError(f"{what}: q must be fp16 [batch, q_heads, head_dim] = [{batch}, *, {head_dim}] "
                          "on the pages' device")
@@ -814,19 +821,20 @@ def paged_append(pages: KVPages, table: torch.Tensor, lens: torch.Tensor, k: tor
     behind cu[B] are ignored, as is what the table has no page for; ``lens`` is
     not changed.  No two sequences of a call may append to one page."""
     block, (B, H, D, _, _), dev = _paged("paged_append", pages, table, lens)
-    if k.dim() != 3 or k.shape[1:] != (H, D) or v.shape != k.shape or k.dtype is not torch.float16 \
+    shape = k.shape
+    if len(shape) != 3 or shape[1] != H or shape[2] != D or v.shape != shape or k.dtype is not torch.float16 \
             or v.dtype is not torch.float16 or k.get_device() != dev or v.get_device() != dev:
         raise ValueError(f"paged_append: k and v must be fp16 [rows, {H}, {D}] on the pages' device")
-    n = k.shape[0]
+    n = shape[0]
     if cu is not None:
         cu = _cu("paged_append", cu, B, dev)
     elif n != B:
         raise ValueError(f"paged_append: without cu there is one row per sequence ({B}), got {n}")
     if n == 0:
         return
-    ts, hs, cs = k.stride()
+    strides = ts, hs, cs = k.stride()
     kp, vp = k.data_ptr(), v.data_ptr()
-    if v.stride() != (ts, hs, cs) or cs != 1 or ts % 8 or hs % 8 or kp % 16 or vp % 16:
+    if v.stride() != strides or cs != 1 or ts % 8 or hs % 8 or kp % 16 or vp % 16:
         k, v = k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format)
         (ts, hs, _), kp, vp = k.stride(), k.data_ptr(), v.data_ptr()
     _paged_call(dev, "rfsn_paged_append", block, kp, vp, ts, hs, n, cu)
