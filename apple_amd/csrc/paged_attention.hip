@@ -650,7 +650,13 @@ Plan plan(const rfsn_paged& p, int q_heads, int count) {
   const int64_t most = (int64_t)(count ? count : p.table_width) * p.page_size;
   const int units = (int)(p.kv_heads * ceil_div(q_heads / p.kv_heads, 16));
   Plan r;
-  r.wide = (int64_t)p.batch * units * ceil_div(most, 32) <= kWideTiles;
+  const int64_t tiles = (int64_t)p.batch * units * ceil_div(most, 32);
+  // Blocks of many waves have all of a short call's loads in flight (8,192 positions x 8 KV heads of 64: 17 us in
+  // blocks of 4 waves, 12 so; 8 x 8,000: 31 in blocks of 4 and 37 so), and take up to 2,048 positions without a
+  // merge, where 4 waves take 512 (fp16, 8 KV heads: 32 x 2,000 30.4 -> 26.2 us, 256 x 2,000 206 -> 195;
+  // 1,024 x 300, which 4 waves take without one as well, 117 in blocks of 4 and 193 so).  With head_dim 128 they are 8
+  // waves, and 32 x 1,000 positions take 34 us without a merge and 31 with it.
+  r.wide = tiles <= kWideTiles || (p.head_dim == 64 && most > 512 && most <= 2048);
   const int per_step = waves_of(p.head_dim, r.wide) * 32;
   const int64_t least = r.wide ? per_step : 4 * per_step;  // positions of a chunk
   if (most <= 4 * per_step) {

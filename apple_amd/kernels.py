@@ -880,10 +880,9 @@ def page_select(q: torch.Tensor, pages: KVPages, table: torch.Tensor, lens: torc
     count, first, last = int(count), int(first), int(last)
     if count <= 0 or first < 0 or last < 0 or first + last > count:
         raise ValueError("page_select: count must be positive and have room for the first and last pages")
-    device = pages.k.device
-    chosen = torch.empty((B, H, count), dtype=torch.int32, device=device)
+    chosen = lens.new_empty((B, H, count))
     wsb = _paged_workspace("rfsn_page_select_workspace_bytes", *sizes)
-    ws = torch.empty(wsb, dtype=torch.uint8, device=device)
+    ws = lens.new_empty(wsb // 4)
     _paged_call(dev, "rfsn_page_select", block, q.data_ptr(), q.shape[1], count, first, last, chosen.data_ptr(),
                 ws.data_ptr(), wsb)
     return chosen
@@ -910,7 +909,7 @@ def paged_attention(q: torch.Tensor, pages: KVPages, table: torch.Tensor, lens: 
         return out.zero_()
     Hq = q.shape[1]
     wsb = _paged_workspace("rfsn_paged_attention_workspace_bytes", *sizes, Hq, count)
-    ws = torch.empty(wsb, dtype=torch.uint8, device=q.device) if wsb else None
+    ws = lens.new_empty(wsb // 4) if wsb else None
     _paged_call(dev, "rfsn_paged_attention", block, q.data_ptr(), Hq, float(scale), listed, count, out.data_ptr(),
                 None if ws is None else ws.data_ptr(), wsb)
     return out
