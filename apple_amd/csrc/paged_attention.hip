@@ -706,8 +706,9 @@ extern "C" int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t 
                "paged_attention: q_heads must be a multiple of kv_heads");
   RFSN_REQUIRE((chosen == nullptr) == (count == 0) && count >= 0, "paged_attention: chosen and count go together");
   RFSN_REQUIRE((int64_t)count * p->page_size <= (1ll << 31) - 1024, "paged_attention: too many chosen pages");
-  RFSN_REQUIRE(scale == scale && scale < __builtin_inff() && scale > -__builtin_inff(),
-               "paged_attention: scale must be finite");
+  const float sl2 = scale * 1.44269504088896340736f;
+  RFSN_REQUIRE(sl2 == sl2 && sl2 < __builtin_inff() && sl2 > -__builtin_inff(),
+               "paged_attention: scale must be finite, in base 2 as well");
   if (p->batch == 0) return RFSN_OK;
   RFSN_REQUIRE(q && out && ((uintptr_t)q & 15) == 0 && ((uintptr_t)out & 15) == 0,
                "paged_attention: q and out must be 16-byte aligned");
@@ -717,7 +718,6 @@ extern "C" int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t 
   RFSN_REQUIRE(c.slots <= 65535, "paged_attention: too many sequences");
   const hipStream_t s = (hipStream_t)stream;
   const int shift = paged_shift(*p), G = q_heads / p->kv_heads;
-  const float sl2 = scale * 1.44269504088896340736f;
   Parts parts = {nullptr, nullptr, nullptr};
   if (c.split()) {
     parts.acc = (float*)workspace;

@@ -300,6 +300,63 @@ def test_infinities_and_nan(device, dim, where):
     R.check(got, *R.attention(pool, table, lens, q, dim ** -0.5), where)
 
 
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_every_code(device, kind):
+    """All 256 codes as K and V: int8 from -128, e4m3 with its subnormal numbers; a NaN code makes its heads NaN."""
+    pool = R.Pool(kind, 40, 2, 16, 64, seed=21, bounds=False)
+    lens = [600]
+    table = pool.tables(lens)
+    codes = torch.arange(40 * 2 * 16 * 64).view(40, 2, 16, 64) * 37 % 256
+    if kind == "e4m3":
+        codes = torch.where(codes % 128 == 127, codes - 1, codes)
+    pool.k.view(torch.uint8).copy_(codes)
+    pool.v.view(torch.uint8).copy_(codes.flip(3))
+    q = pool.randn((1, 8, 64), 0.3)
+    R.check(attend(device, pool, table, lens, q, 0.125), *R.attention(pool, table, lens, q, 0.125))
+    if kind == "e4m3":
+        for name, at in (("k", 70), ("v", 599)):
+            kept = getattr(pool, name).clone()
+            getattr(pool, name).view(torch.uint8)[int(table[0, at // 16]), 1, at % 16, 5] = 0xff
+            got = attend(device, pool, table, lens, q, 0.125)
+            R.check(got, *R.attention(pool, table, lens, q, 0.125), name)
+            assert torch.isnan(got[0, 4:]).any() and not torch.isnan(got[0, :4]).any()
+            setattr(pool, name, kept)
+
+
+@pytest.mark.parametrize("kind", ["fp16", "int8"])
+@pytest.mark.parametrize("batch, heads, tokens, count, size", [(1, 200, 10007, 0, 16), (8, 128, 9000, 80, 64),
+                                                               (2, 100, 20000, 0, 128)])
+def test_chunks_of_many_tiles(device, kind, batch, heads, tokens, count, size):
+    """So many heads that a wave takes more tiles than it looks pages up for at once (against 64 bits on the device)."""
+    K = kernels()
+    dim = 64
+    pool = R.Pool(kind, 30, heads, size, dim, seed=heads, bounds=False)
+    width = -(-tokens // size)
+    table = torch.randint(0, 30, (batch, width), generator=pool.g, dtype=torch.int32)
+    q = pool.randn((batch, heads * 2, dim), 2.0).to(device)
+    lens = [tokens - 7 * b for b in range(batch)]
+    chosen = None
+    if count:
+        chosen = torch.stack([torch.randperm(width, generator=pool.g)[:count].sort().values
+                              for _ in range(batch * heads)]).view(batch, heads, count).int()
+    got = K.paged_attention(q, pool.pages(device), table.to(device), i32(lens, device), 0.125,
+                            None if chosen is None else chosen.to(device)).double()
+    kk, vv = pool.values("k").to(device), pool.values("v").to(device)
+    for b in range(batch):
+        for h in range(0, heads, 7):
+            ords = torch.arange(width) if chosen is None else chosen[b, h].long()
+            pos = (ords[:, None] * size + torch.arange(size)).reshape(-1).to(device) < lens[b]
+            page = table[b].long()[ords].to(device)
+            k, v = (x[page, h].reshape(-1, dim)[pos] for x in (kk, vv))
+            for g in range(2):
+                x = q[b, 2 * h + g].double()
+                want = torch.softmax((k * x).sum(-1) * 0.125, 0) @ v
+                size_qk = float(((k * x).abs().sum(-1) * 0.125).max())
+                tol = want.abs() * 2.0 ** -11 + 2.0 ** -25 + float(v.abs().max()) * (
+                    2 * 68 * 2.0 ** -24 * size_qk + 2 * len(k) * 2.0 ** -24 + 2.0 ** -16)  # as in R.attention
+                assert ((got[b, 2 * h + g] - want).abs() <= tol).all(), (b, h, g)
+
+
 # ------------------------------------------------------------------ page choice
 
 @pytest.mark.parametrize("dim, heads, group, size, count, first, last", [
@@ -526,7 +583,7 @@ def test_wrappers_refuse(device):
         lambda: K.paged_attention(q, pages, t.long(), n, 0.1), lambda: K.paged_attention(q, pages, t, n.long(), 0.1),
         lambda: K.paged_attention(q, pages, t, n[:1], 0.1), lambda: K.paged_attention(q, pages, t[:1], n, 0.1),
         lambda: K.paged_attention(q, pages, t.t().contiguous().t(), n, 0.1),
-        lambda: K.paged_attention(q, pages, t, n, math.inf),
+        lambda: K.paged_attention(q, pages, t, n, math.inf), lambda: K.paged_attention(q, pages, t, n, 3e38),
         lambda: K.paged_attention(q, pages._replace(k_scale=s), t, n, 0.1),
         lambda: K.paged_attention(q, pages._replace(v=pages.v.to(torch.int8)), t, n, 0.1),
         lambda: K.paged_attention(q, pages._replace(k=pages.k.bfloat16(), v=pages.v.bfloat16()), t, n, 0.1),
