@@ -3,9 +3,19 @@
 //
 //   out_i = sum_t e^(s_t - m) v_t / sum_t e^(s_t - m),  s_t = scale q_i . k_t
 //
-// A block takes a chunk of positions of one (sequence, KV head) with all of its
-// query heads; chunks are cut by the sum of the lengths, which only the device
-// knows (find_chunk), and a second kernel joins their (m, l, acc).
+// in one pass over K and V with a running maximum.  A block takes a chunk of
+// positions of one (sequence, KV head) with up to 16 of its query heads, so K and
+// V are read once for the group; chunks are cut by the lengths, which only the
+// device knows (find_chunk), and a second kernel joins their (m, l, O).
+//
+// Bound: the HBM read of K and V where there is enough of it (32 x 32,768
+// positions, 8 KV heads of 64: fp16 2.15 GB in 350 to 358 us, 6.0 TB/s, 1.001 of the bytes
+// that there are, the matrix cores 6 % busy, VALU 15 %, no LDS conflicts; int8 214 to
+// 220 us, 5.2 TB/s; 4 x 8,001, 32 KV heads of 128: 90 to 92 us, 5.7 TB/s).  Below some
+// 50 MB the chain of dependent loads (length, page, rows), the launch and the merge:
+// 1,021 positions x 8 KV heads 8.8 to 9.4 us, 8,192 of int8 8.5 us and 3 to 4 for the merge.
+// One wave per head and chunk with fp32 FMAs (attend_row, now for sums that are not
+// finite alone) took 4,104 us for the first and 88 us for 1,021 positions.
 #include "paged.h"
 
 namespace rfsn {
@@ -179,7 +189,8 @@ __device__ __forceinline__ void attend_row(const rfsn_paged& p, int shift, const
 
 // ---- tiles on the matrix cores
 //
-// A wave takes NG groups of 16 positions at a time (each inside one page), a
+// A wave takes two groups of 16 positions at a time (each inside one page; four groups, with half
+// the waves' registers, changed no time by more than 3 % where they fit and cost 8 % with 8-bit rows of 128), a
 // block's waves take them in turn, and a lane's 16 columns are the query heads of the KV
 // head (the others repeat the last: the matrix cores are idle otherwise).
 //   S = K Q^T      MFMA 16x16x32, A = 16 rows of K as they lie in memory (16 bytes a
@@ -189,9 +200,10 @@ __device__ __forceinline__ void attend_row(const rfsn_paged& p, int shift, const
 //                  (lane group g, j) is position 16 (j >> 2) + 4 g + (j & 3).  V passes
 //                  through LDS of the wave's own, and ds_read_b64_tr_b16 reads V^T from it
 //                  in that order.
-// Weights are kept to 2^-22 of themselves (fp16 pages: p 2^8 as fp16 hi + lo) or 2^-16
-// (8-bit pages: p times the row's scale as bf16 hi + lo, which has fp32's range; codes
-// are exact in bf16).  Scores, maxima, sums and O are fp32.
+// Weights are rounded twice, which leaves them off by 2^-22 of themselves (fp16 pages: p 2^8 as
+// fp16 hi + lo) or 2^-16 (8-bit pages: p times the row's scale as bf16 hi + lo, which has fp32's range;
+// codes are exact in bf16), both well under the 2^-11 of the result's own rounding; the second product
+// costs matrix-core time that is idle.  Scores, maxima, sums and O are fp32.
 // Where V or a score is infinite or NaN, hi, lo and weights of 0 meet it apart; a block that
 // finds a sum that is not finite takes its chunk again by attend_row.
 
@@ -203,11 +215,12 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short short4w __attribute__((ext_vector_type(4)));
 typedef short short8w __attribute__((ext_vector_type(8)));
 
+constexpr int NG = 2;              // groups of a wave's step
 constexpr int kWideTiles = 8192;   // tiles of 32 positions of a call up to which blocks have many waves
 constexpr float kPBias = 8.f;      // a weight is kept as p 2^8
 constexpr float kPSum = 32768.f;   // a lane's sum below it: every weight is finite in fp16
 
-// 16-byte chunk c of row t of a [16 NG][D] 16-bit tile sits at chunk c ^ v_swz(t): the
+// 16-byte chunk c of row t of a [32][D] 16-bit tile sits at chunk c ^ v_swz(t): the
 // transposed reads take 32 bytes of 8 rows at once, which then lie in different banks.
 template <int D>
 __device__ __forceinline__ int v_swz(int t) { return D == 64 ? ((t >> 1) & 3) << 1 : (t & 7) << 1; }
@@ -266,8 +279,8 @@ struct Parts {
   int32_t* seq; // [batch][2]
 };
 
-template <int D, int TYPE, int kWaves, int NG>
-__global__ void __launch_bounds__(kWaves * 64, kWaves > 4 ? 1 : D == 64 ? (NG > 2 ? 3 : 4) : D == 128 ? 2 : 1)
+template <int D, int TYPE, int kWaves>
+__global__ void __launch_bounds__(kWaves * 64, kWaves > 4 ? 1 : D == 64 ? 4 : D == 128 ? 2 : 1)
 paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ table, const uint16_t* __restrict__ q, int G,
                   float scale_log2, const int32_t* __restrict__ chosen, int count, const Cut cut,
                   uint16_t* __restrict__ out, const Parts parts) {
@@ -578,7 +591,9 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
 }
 
 // out = sum_j w_j acc_j / sum_j w_j l_j over a sequence's chunks, w_j = 2^(m_j - max m).
-// The (m, l) of 64 chunks are one load of a wave, and the rows of O do not wait for them.
+// The (m, l) of 64 chunks are one load of a wave.  W waves share a row's chunks: 16 where few rows
+// have many (131,072 positions of one sequence, 128 chunks: the call 64 -> 59 us), 4 for the rows of
+// a batch (48 sequences x 32 heads: 25 us, and 27 with 16).
 template <int D, int W>
 __global__ void __launch_bounds__(W * 64)
 paged_merge_kernel(const rfsn_paged p, int shift, int q_heads, int per_seq, const Parts parts, uint16_t* __restrict__ out) {
@@ -650,16 +665,19 @@ Plan plan(const rfsn_paged& p, int q_heads, int count) {
   const int64_t most = (int64_t)(count ? count : p.table_width) * p.page_size;
   const int units = (int)(p.kv_heads * ceil_div(q_heads / p.kv_heads, 16));
   Plan r;
-  const int64_t tiles = (int64_t)p.batch * units * ceil_div(most, 32);
   // Blocks of many waves have all of a short call's loads in flight (8,192 positions x 8 KV heads of 64: 17 us in
-  // blocks of 4 waves, 12 so; 8 x 8,000: 31 in blocks of 4 and 37 so), and take up to 2,048 positions without a
-  // merge, where 4 waves take 512 (fp16, 8 KV heads: 32 x 2,000 30.4 -> 26.2 us, 256 x 2,000 206 -> 195;
-  // 1,024 x 300, which 4 waves take without one as well, 117 in blocks of 4 and 193 so).  With head_dim 128 they are 8
-  // waves, and 32 x 1,000 positions take 34 us without a merge and 31 with it.
-  r.wide = tiles <= kWideTiles || (p.head_dim == 64 && most > 512 && most <= 2048);
+  // blocks of 4 waves, 12 so; 8 x 8,000: 31 in blocks of 4 and 37 so).  They also take a sequence without a
+  // merge where its steps cost less than one: 8 steps (4,096 positions of 64, 2,048 of 128) with blocks for most CUs
+  // (fp16, 8 KV heads: 24 x 4,000 of 64 43.6 -> 39.7 us, 32 x 1,900 of 128 53.3 -> 47.8, while 16 x 4,000, 128
+  // blocks, goes from 31 to 34), 4 with 64 (8 x 2,000: 14.2 -> 13.7), else 3 (1,021: 10.0 -> 8.6; 2,000 as 4: 10.3 ->
+  // 12.7).  Blocks of 4 waves take 512 positions so (1,024 x 300: 117 us, in wide blocks 193).
+  const int64_t blocks = (int64_t)p.batch * units, tiles = blocks * ceil_div(most, 32);
+  const int most_steps = blocks >= 192 ? 8 : blocks >= 64 ? 4 : 3;
+  r.wide = tiles <= kWideTiles ||
+           (most > 512 && blocks >= 192 && most <= most_steps * waves_of(p.head_dim, true) * 32);
   const int per_step = waves_of(p.head_dim, r.wide) * 32;
   const int64_t least = r.wide ? per_step : 4 * per_step;  // positions of a chunk
-  if (most <= 4 * per_step) {
+  if (most <= (r.wide ? most_steps : 4) * per_step) {
     r.slots = p.batch, r.cut = {1, units, most > 0 ? most : 1, {}};
   } else if (count) {
     int64_t n = ceil_div(r.wide ? kCUs : 4 * kCUs, (int64_t)units * p.batch);
@@ -677,7 +695,8 @@ Plan plan(const rfsn_paged& p, int q_heads, int count) {
       most_chunks = n > most_chunks ? n : most_chunks;
     }
     // The sum of ceil(len / size) is at most total / size + batch, and size at least total / target - 0.02
-    // (find_chunk) or 128 and more, which is 32767 (0.02 / 512 + 2^-21) < 2 chunks over the target.
+    // (find_chunk) and `least`: below 32767 (0.02 / 512 + 2^-21) < 2 chunks over the target (wide blocks
+    // have a `least` of 128 to 512, and at most 8,192 tiles of sequences longer than it).
     r.slots = most_chunks + 2 + p.batch;
     if (r.slots > ceil_div(most, least) * p.batch) r.slots = ceil_div(most, least) * p.batch;
   }
@@ -725,26 +744,25 @@ extern "C" int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t 
     parts.seq = (int32_t*)(parts.ml + c.slots * q_heads * 2);
   }
   const dim3 grid((unsigned)p->kv_heads, (unsigned)c.slots, (unsigned)ceil_div(G, 16));
-#define RFSN_ATTEND(DD, TT, NW, NG)                                                                                 \
-  hipLaunchKernelGGL((paged_attn_kernel<DD, TT, NW, NG>), grid, dim3(NW * 64), 0, s, *p, shift, p->table,           \
+#define RFSN_ATTEND(DD, TT, NW)                                                                                     \
+  hipLaunchKernelGGL((paged_attn_kernel<DD, TT, NW>), grid, dim3(NW * 64), 0, s, *p, shift, p->table,           \
                      (const uint16_t*)q, G, sl2, chosen, count, c.cut, (uint16_t*)out, parts)
-#define RFSN_ATTEND_D(DD, NW, NG, NG8)                                            \
-  do {                                                                            \
-    if (p->type == RFSN_PAGE_FP16) RFSN_ATTEND(DD, RFSN_PAGE_FP16, NW, NG);       \
-    else if (p->type == RFSN_PAGE_INT8) RFSN_ATTEND(DD, RFSN_PAGE_INT8, NW, NG8); \
-    else RFSN_ATTEND(DD, RFSN_PAGE_E4M3, NW, NG8);                                \
+#define RFSN_ATTEND_D(DD, NW)                                                \
+  do {                                                                       \
+    if (p->type == RFSN_PAGE_FP16) RFSN_ATTEND(DD, RFSN_PAGE_FP16, NW);      \
+    else if (p->type == RFSN_PAGE_INT8) RFSN_ATTEND(DD, RFSN_PAGE_INT8, NW); \
+    else RFSN_ATTEND(DD, RFSN_PAGE_E4M3, NW);                                \
   } while (0)
-  if (p->head_dim == 64 && c.wide) RFSN_ATTEND_D(64, 16, 2, 2);
-  else if (p->head_dim == 64) RFSN_ATTEND_D(64, 4, 2, 2);
-  else if (p->head_dim == 128 && c.wide) RFSN_ATTEND_D(128, 8, 2, 2);
-  else if (p->head_dim == 128) RFSN_ATTEND_D(128, 4, 2, 2);
-  else RFSN_ATTEND_D(256, 4, 2, 2);
+  if (p->head_dim == 64 && c.wide) RFSN_ATTEND_D(64, 16);
+  else if (p->head_dim == 64) RFSN_ATTEND_D(64, 4);
+  else if (p->head_dim == 128 && c.wide) RFSN_ATTEND_D(128, 8);
+  else if (p->head_dim == 128) RFSN_ATTEND_D(128, 4);
+  else RFSN_ATTEND_D(256, 4);
 #undef RFSN_ATTEND_D
 #undef RFSN_ATTEND
   if (int st = check_launch("paged_attention")) return st;
   if (c.split()) {
     const dim3 rows((unsigned)q_heads, (unsigned)p->batch);
-    // chunks a sequence may have: with few, four waves a row, with many a wave for each of 16
     const bool many = (c.cut.per_seq ? c.cut.per_seq : c.slots - p->batch + 1) > 16 && (int64_t)q_heads * p->batch <= 256;
 #define RFSN_MERGE(DD)                                                                                              \
   do {                                                                                                              \

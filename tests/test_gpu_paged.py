@@ -220,6 +220,23 @@ def test_attention(device, kind, lens, dim, heads, group, size):
     R.check(got, *R.attention(pool, table, lens, q, dim ** -0.5))
 
 
+@pytest.mark.parametrize("kind", ["fp16", "int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("batch", [4, 12])
+def test_tables_far_wider_than_the_sequences(device, kind, dim, batch):
+    """A table for 40,000 positions a sequence, as a captured step keeps: cut by the lengths on the device, in
+    chunks and rows of few and of many."""
+    lens = ([2100, 0, 33, 700] * 3)[:batch]
+    pool = R.Pool(kind, sum(-(-n // 16) for n in lens) + 1, 8, 16, dim, seed=dim + batch, bounds=False)
+    narrow = pool.tables(lens)
+    poison(pool, narrow, lens)
+    table = torch.full((batch, 2500), -1, dtype=torch.int32)
+    table[:, :narrow.shape[1]] = narrow
+    q = pool.randn((batch, 24, dim), 2.0)
+    got = attend(device, pool, table, lens, q, dim ** -0.5)
+    R.check(got, *R.attention(pool, narrow, lens, q, dim ** -0.5))
+
+
 def test_attention_of_many_sequences(device):
     """More sequences than a wave has lanes, lengths of every order, one far longer than the others."""
     g = torch.Generator().manual_seed(9)
