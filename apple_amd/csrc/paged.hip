@@ -2,8 +2,8 @@
 // query reads.
 //
 // Append and read move each row once and are bound by HBM from some 30 MB on (16,384 rows
-// x 32 heads of 128, K and V: fp16 with bounds 537 MB in 99 us, 5.4 TB/s, and 98 us back; int8
-// 403 MB in 98 us and 80 us back); below it by the loads that wait for one another (sequence,
+// x 32 heads of 128, K and V: fp16 with bounds 537 MB in 101 us, 5.3 TB/s, and 98 us back; int8
+// 403 MB in 97 us and 84 us back); below it by the loads that wait for one another (sequence,
 // page, row): 32 rows of 8 heads 3.5 us.
 #include "paged.h"
 
@@ -239,7 +239,7 @@ __device__ __forceinline__ void store_page(V x, V* at) {
 // coordinates of a row.  Bounds: the wave of a run's first row (rows of one
 // sequence in one page) takes those of the run's keys that it holds and reads the others, and
 // writes the page's bounds, so no two waves write the same ones and no order changes them.  Bounds
-// cost 5 to 13 % of a long append (16,384 x 32 x 128: fp16 101 -> 107 us, int8 89 -> 101).
+// take 2 us of 101 for 16,384 x 32 x 128 in fp16, 14 of 97 in int8, 1.8 of 9.3 for 8,191 x 8 x 64.
 template <int D, int TYPE, int I>
 __global__ void __launch_bounds__(256)
 paged_append_kernel(const rfsn_paged p, int shift, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
@@ -621,10 +621,11 @@ extern "C" int rfsn_paged_append(const rfsn_paged* p, const void* k, const void*
                    head_stride % 8 == 0,
                "paged_append: k and v rows must be 16-byte aligned");
   const int rs = 512 / p->head_dim;
-  RFSN_REQUIRE(ceil_div(rows, rs) < (1ll << 24), "paged_append: too many rows");
+  RFSN_REQUIRE(ceil_div(rows, rs) < (1ll << 24) && ceil_div(rows, rs) * ceil_div(p->kv_heads, 4) < (1ll << 31),
+               "paged_append: too many rows");
   const int shift = paged_shift(*p);
   // Four sets of rows per wave hold most of their pages' rows and read few again for the
-  // bounds, but leave fewer waves.  8 heads of 64, fp16 pages of 16: 512 rows (512 sets) 6.0 us
+  // bounds, but leave fewer waves.  With both storing alike, 8 heads of 64, fp16 pages of 16: 512 rows (512 sets) 6.0 us
   // against 4.1, 4,096 rows 7.1 against 7.3 (int8 7.9 against 7.4), 8,192 rows 11.1 against 11.8;
   // 16,384 rows x 32 heads of 128: 107 us against 135.
   const bool four = ceil_div(rows, rs) * p->kv_heads > 4096;
@@ -649,7 +650,8 @@ extern "C" int rfsn_paged_read(const rfsn_paged* p, const int32_t* cu, int64_t r
   RFSN_REQUIRE(out_k && out_v && ((uintptr_t)out_k & 15) == 0 && ((uintptr_t)out_v & 15) == 0,
                "paged_read: outputs must be 16-byte aligned");
   const int rs = 512 / p->head_dim;
-  RFSN_REQUIRE(ceil_div(rows, rs) < (1ll << 24), "paged_read: too many rows");
+  RFSN_REQUIRE(ceil_div(rows, rs) < (1ll << 24) && ceil_div(rows, rs) * ceil_div(p->kv_heads, 4) < (1ll << 31),
+               "paged_read: too many rows");
   const int shift = paged_shift(*p);
   const dim3 grid((unsigned)ceil_div(rows, rs), (unsigned)ceil_div(p->kv_heads, 4));
   RFSN_PAGED_DISPATCH(p->head_dim, p->type, {
