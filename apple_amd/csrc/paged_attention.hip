@@ -216,6 +216,7 @@ typedef short short4w __attribute__((ext_vector_type(4)));
 typedef short short8w __attribute__((ext_vector_type(8)));
 
 constexpr int NG = 2;              // groups of a wave's step
+constexpr double kLastLevelCache = 256 * 1024 * 1024;
 constexpr int kWideTiles = 8192;   // tiles of 32 positions of a call up to which blocks have many waves
 constexpr float kPBias = 8.f;      // a weight is kept as p 2^8
 constexpr float kPSum = 32768.f;   // a lane's sum below it: every weight is finite in fp16
@@ -271,6 +272,13 @@ __device__ __forceinline__ uint4w codes_bf16(uint32_t a, uint32_t b) {
   return r;
 }
 
+// 16 bytes of a row, marked as not to be kept where the call reads more than the caches hold (Plan).
+template <bool kOnce>
+__device__ __forceinline__ uint4w load16(const uint8_t* a) {
+  if constexpr (kOnce) return __builtin_nontemporal_load(reinterpret_cast<const uint4w*>(a));
+  else return *reinterpret_cast<const uint4w*>(a);
+}
+
 // Partial results of a split call: (m, l) and O of each chunk and query head, and for each
 // sequence that has any its first chunk and their number.
 struct Parts {
@@ -279,7 +287,7 @@ struct Parts {
   int32_t* seq; // [batch][2]
 };
 
-template <int D, int TYPE, int kWaves>
+template <int D, int TYPE, int kWaves, bool kOnce>
 __global__ void __launch_bounds__(kWaves * 64, kWaves > 4 ? 1 : D == 64 ? 4 : D == 128 ? 2 : 1)
 paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ table, const uint16_t* __restrict__ q, int G,
                   float scale_log2, const int32_t* __restrict__ chosen, int count, const Cut cut,
@@ -378,11 +386,11 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
       const uint8_t* vb = (const uint8_t*)p.v + base;
       const uint32_t kl = (uint32_t)(min(col, last) * (D * ES) + grp * 16);
 #pragma unroll
-      for (int i = 0; i < KL; ++i) kr[u][i] = *reinterpret_cast<const uint4w*>(kb + kl + i * 64);
+      for (int i = 0; i < KL; ++i) kr[u][i] = load16<kOnce>(kb + kl + i * 64);
 #pragma unroll
       for (int i = 0; i < VU; ++i) {
         const int idx = i * 64 + lane, r = idx / VC, ch = idx % VC;
-        vr[u][i] = *reinterpret_cast<const uint4w*>(vb + (uint32_t)(min(r, last) * (D * ES) + ch * 16));
+        vr[u][i] = load16<kOnce>(vb + (uint32_t)(min(r, last) * (D * ES) + ch * 16));
       }
       if constexpr (kCodes) {
         const int64_t sc = ((int64_t)page * p.kv_heads + h) * p.page_size + row;
@@ -658,6 +666,7 @@ struct Plan {
   int64_t slots;  // of partial results
   Cut cut;
   bool wide;      // blocks of many waves
+  bool once;      // rows are loaded past the caches
   bool split() const { return cut.per_seq != 1; }
 };
 int waves_of(int D, bool wide) { return !wide || D == 256 ? 4 : D == 64 ? 16 : 8; }  // (256: 8 would spill)
@@ -675,6 +684,14 @@ Plan plan(const rfsn_paged& p, int q_heads, int count) {
   const int most_steps = blocks >= 192 ? 8 : blocks >= 64 ? 4 : 3;
   r.wide = tiles <= kWideTiles ||
            (most > 512 && blocks >= 192 && most <= most_steps * waves_of(p.head_dim, true) * 32);
+  // K and V of 256 MB or more, the size of the last-level cache, are gone from it before the next call reads them
+  // again: loaded as data that is used once they displace nothing and arrive sooner (32 x 32,768 positions, 8 KV heads
+  // of 64: fp16 374 -> 344 us, int8 220 -> 205; 4 x 8,000, 32 of 128: 99 -> 90, 16 x 8,192, 8 of 256: 196 -> 180).
+  // What fits stays for the next call (245 MB read again at once: 43 us, loaded so
+  // 47), blocks of many waves have less than that, and a list of pages reads few of them.
+  const double in_tables = (double)p.batch * p.table_width, pages = in_tables < p.pages ? in_tables : p.pages;
+  r.once = !r.wide && count == 0 &&
+           pages * p.page_size * p.kv_heads * p.head_dim * (p.type == RFSN_PAGE_FP16 ? 4 : 2) >= kLastLevelCache;
   const int per_step = waves_of(p.head_dim, r.wide) * 32;
   const int64_t least = r.wide ? per_step : 4 * per_step;  // positions of a chunk
   if (most <= (r.wide ? most_steps : 4) * per_step) {
@@ -744,20 +761,23 @@ extern "C" int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t 
     parts.seq = (int32_t*)(parts.ml + c.slots * q_heads * 2);
   }
   const dim3 grid((unsigned)p->kv_heads, (unsigned)c.slots, (unsigned)ceil_div(G, 16));
-#define RFSN_ATTEND(DD, TT, NW)                                                                                     \
-  hipLaunchKernelGGL((paged_attn_kernel<DD, TT, NW>), grid, dim3(NW * 64), 0, s, *p, shift, p->table,           \
+#define RFSN_ATTEND(DD, TT, NW, ONCE)                                                                               \
+  hipLaunchKernelGGL((paged_attn_kernel<DD, TT, NW, ONCE>), grid, dim3(NW * 64), 0, s, *p, shift, p->table,           \
                      (const uint16_t*)q, G, sl2, chosen, count, c.cut, (uint16_t*)out, parts)
-#define RFSN_ATTEND_D(DD, NW)                                                \
-  do {                                                                       \
-    if (p->type == RFSN_PAGE_FP16) RFSN_ATTEND(DD, RFSN_PAGE_FP16, NW);      \
-    else if (p->type == RFSN_PAGE_INT8) RFSN_ATTEND(DD, RFSN_PAGE_INT8, NW); \
-    else RFSN_ATTEND(DD, RFSN_PAGE_E4M3, NW);                                \
+#define RFSN_ATTEND_D(DD, NW, ONCE)                                                \
+  do {                                                                             \
+    if (p->type == RFSN_PAGE_FP16) RFSN_ATTEND(DD, RFSN_PAGE_FP16, NW, ONCE);      \
+    else if (p->type == RFSN_PAGE_INT8) RFSN_ATTEND(DD, RFSN_PAGE_INT8, NW, ONCE); \
+    else RFSN_ATTEND(DD, RFSN_PAGE_E4M3, NW, ONCE);                                \
   } while (0)
-  if (p->head_dim == 64 && c.wide) RFSN_ATTEND_D(64, 16);
-  else if (p->head_dim == 64) RFSN_ATTEND_D(64, 4);
-  else if (p->head_dim == 128 && c.wide) RFSN_ATTEND_D(128, 8);
-  else if (p->head_dim == 128) RFSN_ATTEND_D(128, 4);
-  else RFSN_ATTEND_D(256, 4);
+  if (p->head_dim == 64 && c.wide) RFSN_ATTEND_D(64, 16, false);
+  else if (p->head_dim == 64 && c.once) RFSN_ATTEND_D(64, 4, true);
+  else if (p->head_dim == 64) RFSN_ATTEND_D(64, 4, false);
+  else if (p->head_dim == 128 && c.wide) RFSN_ATTEND_D(128, 8, false);
+  else if (p->head_dim == 128 && c.once) RFSN_ATTEND_D(128, 4, true);
+  else if (p->head_dim == 128) RFSN_ATTEND_D(128, 4, false);
+  else if (c.once) RFSN_ATTEND_D(256, 4, true);
+  else RFSN_ATTEND_D(256, 4, false);
 #undef RFSN_ATTEND_D
 #undef RFSN_ATTEND
   if (int st = check_launch("paged_attention")) return st;
