@@ -528,6 +528,32 @@ def test_long_pools_pass_32_bit_offsets(device):
     assert chosen[0, :, 0].eq(0).all() and chosen[0, :, 1].eq(2).all()
 
 
+@pytest.mark.parametrize("kind", ["fp16", "int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lens, times", [([2100, 0, 33, 700], 1), ([16, 0, 77, 5], 300)])
+def test_pools_past_the_last_level_cache(device, kind, dim, lens, times):
+    """300 MB of pages with the sequences' scattered over them, and room for all of them in the table: their rows
+    are loaded as used once, in chunks by the lengths and in one for each of many sequences, which share pages."""
+    K = kernels()
+    heads, size = 4, 16
+    pool = R.Pool(kind, sum(-(-n // size) for n in lens) + 1, heads, size, dim, seed=dim + len(lens), bounds=False)
+    near = pool.tables(lens)
+    poison(pool, near, lens)
+    q = pool.randn((len(lens), 12, dim), 2.0)
+    count = 300_000_000 // (2 * heads * size * dim * pool.k.element_size())
+    to = torch.randperm(count, generator=pool.g)[:pool.count].int()
+    small = pool.pages(device)
+    far = [None if x is None else x.new_zeros((count, *x.shape[1:])) for x in small]
+    for big, x in zip(far, small):
+        if x is not None:
+            big.view(torch.uint8)[to.to(device).long()] = x.view(torch.uint8)
+    table = torch.full((len(lens), max(near.shape[1], -(-count // (len(lens) * times)))), -1, dtype=torch.int32)
+    table[:, :near.shape[1]] = torch.where(near >= 0, to[near.clamp(min=0).long()], near)
+    got = K.paged_attention(q.repeat(times, 1, 1).to(device), K.KVPages(*far), table.repeat(times, 1).to(device),
+                            i32(lens * times, device), dim ** -0.5)
+    R.check(got, *(x.repeat(times, 1, 1) for x in R.attention(pool, near, lens, q, dim ** -0.5)))
+
+
 def test_another_stream(device):
     K = kernels()
     pool = R.Pool("int8", 120, 2, 16, 64, seed=45)
