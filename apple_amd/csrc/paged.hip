@@ -228,7 +228,7 @@ __device__ __forceinline__ uint2 xcd_block() {
 
 // Long appends pass the caches by: with 8,191 rows of 8 heads of 64 they take 9.7 us against 11.0, and 22.7
 // with the attention of a token behind them against 23.3; 2,048 rows, which attention finds in the
-// caches, 4.8 against 5.0 alone and 20.7 against 19.2 with it.
+// caches, 4.8 against 5.0 alone and 20.7 against 19.2 with it.  (V was loaded through them then.)
 template <bool PASS, typename V>
 __device__ __forceinline__ void store_page(V x, V* at) {
   if constexpr (PASS) __builtin_nontemporal_store(x, at);
@@ -239,7 +239,9 @@ __device__ __forceinline__ void store_page(V x, V* at) {
 // coordinates of a row.  Bounds: the wave of a run's first row (rows of one
 // sequence in one page) takes those of the run's keys that it holds and reads the others, and
 // writes the page's bounds, so no two waves write the same ones and no order changes them.  Bounds
-// take 2 us of 101 for 16,384 x 32 x 128 in fp16, 14 of 97 in int8, 1.8 of 9.3 for 8,191 x 8 x 64.
+// take 2 us of 101 for 16,384 x 32 x 128 in fp16, 14 of 97 in int8, 1.8 of 8.4 for 8,191 x 8 x 64.
+// V, which no other wave reads, is loaded past the caches in rows of 64 (8,191 x 8: fp16 9.4 -> 8.4 us, int8
+// 10.8 -> 10.0; 8,192 x 8 rows of 128 or more lose 1 %: 16.3 -> 16.5).
 template <int D, int TYPE, int I>
 __global__ void __launch_bounds__(256)
 paged_append_kernel(const rfsn_paged p, int shift, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
@@ -258,7 +260,8 @@ paged_append_kernel(const rfsn_paged p, int shift, const uint16_t* __restrict__ 
   for (int i = 0; i < I; ++i) {
     const int64_t n = n0 + i * RS + slot < rows ? n0 + i * RS + slot : rows - 1;
     kx[i] = *reinterpret_cast<const half8v*>(kh + n * ts);
-    vx[i] = *reinterpret_cast<const half8v*>(vh + n * ts);
+    if constexpr (I > 1 && D == 64) vx[i] = __builtin_nontemporal_load(reinterpret_cast<const half8v*>(vh + n * ts));
+    else vx[i] = *reinterpret_cast<const half8v*>(vh + n * ts);
   }
   RowPlace at[I];
   place_rows<LANES, I>(p, shift, cu, rows, n0, lane, at);

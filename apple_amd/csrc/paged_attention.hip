@@ -9,9 +9,9 @@
 // device knows (find_chunk), and a second kernel joins their (m, l, O).
 //
 // Bound: the HBM read of K and V where there is enough of it (32 x 32,768
-// positions, 8 KV heads of 64: fp16 2.15 GB in 350 to 358 us, 6.0 TB/s, 1.001 of the bytes
-// that there are, the matrix cores 6 % busy, VALU 15 %, no LDS conflicts; int8 214 to
-// 220 us, 5.2 TB/s; 4 x 8,001, 32 KV heads of 128: 90 to 92 us, 5.7 TB/s).  Below some
+// positions, 8 KV heads of 64: fp16 2.15 GB in 324 to 331 us, 6.5 TB/s, 1.001 of the bytes
+// that there are, the matrix cores 6 % busy, VALU 15 %, no LDS conflicts; int8 205 us,
+// 5.6 TB/s; 4 x 8,001, 32 KV heads of 128: 77 to 84 us, 6.2 to 6.8 TB/s).  Below some
 // 50 MB the chain of dependent loads (length, page, rows), the launch and the merge:
 // 1,021 positions x 8 KV heads 8.8 to 9.4 us, 8,192 of int8 8.5 us and 3 to 4 for the merge.
 // One wave per head and chunk with fp32 FMAs (attend_row, now for sums that are not
