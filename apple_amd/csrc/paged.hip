@@ -676,6 +676,7 @@ extern "C" int rfsn_page_select(const rfsn_paged* p, const void* q, int32_t q_he
   RFSN_REQUIRE(q_heads > 0 && q_heads % p->kv_heads == 0, "page_select: q_heads must be a multiple of kv_heads");
   RFSN_REQUIRE(count > 0 && first >= 0 && last >= 0 && (int64_t)first + last <= count,
                "page_select: count must be positive and have room for the first and last pages");
+  RFSN_REQUIRE((int64_t)count * p->page_size <= (1ll << 31) - 1024, "page_select: too many pages");
   if (p->batch == 0) return RFSN_OK;
   RFSN_REQUIRE(q && ((uintptr_t)q & 15) == 0 && chosen, "page_select: null or misaligned q, or null output");
   RFSN_REQUIRE(workspace_bytes >= rfsn_page_select_workspace_bytes(p) && (workspace || p->table_width == 0),

@@ -777,6 +777,13 @@ def _paged(what: str, pages: KVPages, table: torch.Tensor, lens: torch.Tensor) -
                               lens.data_ptr(), sp, sh, st, P, S, H, D, kind, B, W), (B, H, D, S, W), dev)
 
 
+def _page_count(what: str, count: int, page_size: int) -> int:
+    """``count`` pages of a list, which the library takes in 32 bits."""
+    if count * page_size > (1 << 31) - 1024:
+        raise ValueError(f"{what}: {count} pages of {page_size} tokens; a list's positions must stay below 2^31")
+    return count
+
+
 def _paged_call(device: int, name: str, *args) -> None:
     """The call on the device's current stream, whichever device is current."""
     fn = getattr(L.load(), name)
@@ -880,6 +887,7 @@ def page_select(q: torch.Tensor, pages: KVPages, table: torch.Tensor, lens: torc
     count, first, last = int(count), int(first), int(last)
     if count <= 0 or first < 0 or last < 0 or first + last > count:
         raise ValueError("page_select: count must be positive and have room for the first and last pages")
+    _page_count("page_select", count, S)
     chosen = lens.new_empty((B, H, count))
     wsb = _paged_workspace("rfsn_page_select_workspace_bytes", *sizes)
     ws = lens.new_empty(wsb // 4)
@@ -895,15 +903,16 @@ def paged_attention(q: torch.Tensor, pages: KVPages, table: torch.Tensor, lens: 
     ``chosen`` [B, Hkv, n] (``page_select``) lists; zeros where there are none.
     Codes are attended as code * scale in fp32, not rounded to fp16."""
     block, sizes, dev = _paged("paged_attention", pages, table, lens)
-    B, H, D, _, _ = sizes
+    B, H, D, S, _ = sizes
     q = _paged_query("paged_attention", q, B, D, dev)
     count, listed = 0, None
     if chosen is not None:
         if chosen.dim() != 3 or chosen.shape[:2] != (B, H) or chosen.dtype is not torch.int32 \
                 or chosen.get_device() != dev:
             raise ValueError(f"paged_attention: chosen must be int32 [{B}, {H}, n] on the pages' device")
+        count = _page_count("paged_attention", chosen.shape[2], S)
         chosen = _contig(chosen)
-        count, listed = chosen.shape[2], chosen.data_ptr()
+        listed = chosen.data_ptr()
     out = torch.empty_like(q)
     if chosen is not None and count == 0:
         return out.zero_()

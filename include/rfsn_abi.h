@@ -636,7 +636,8 @@ int rfsn_paged_read(const rfsn_paged* p, const int32_t* cu, int64_t rows, void* 
  * min(q_d, 0) lo_d over the KV head's query heads g, which no q . k of the
  * page exceeds.  The sum is exact up to 64-bit rounding and rounded to fp32;
  * NaN counts as infinite, ties go to the lower ordinal.  q [batch][q_heads]
- * [head_dim] fp16. */
+ * [head_dim] fp16.  count * page_size is at most 2^31 - 1024,
+ * here and in rfsn_paged_attention. */
 size_t rfsn_page_select_workspace_bytes(const rfsn_paged* p);
 int rfsn_page_select(const rfsn_paged* p, const void* q, int32_t q_heads, int32_t count, int32_t first, int32_t last,
                      int32_t* chosen, void* workspace, size_t workspace_bytes, void* stream);

@@ -105,6 +105,31 @@ def test_selection_is_refused_before_a_launch(lib, args, says):
     assert says.encode() in lib.rfsn_last_error(), lib.rfsn_last_error()
 
 
+@pytest.mark.parametrize("size", [16, 64, 256])
+def test_page_counts_past_the_kernels_range_are_refused(lib, size):
+    """The kernels step through a row of the list in 32-bit numbers: as many pages as positions below 2^31 hold, no more."""
+    p = ctypes.byref(block(bounds=4096, page_size=size, page_stride=8 * size * 64, head_stride=size * 64))
+    for count in (2 ** 31 - 1, 2 ** 31 - 512, 2 ** 31 // size):
+        assert lib.rfsn_page_select(p, 4096, 8, count, 1, 1, 4096, 4096, 1 << 30, None) == -1
+        assert b"too many pages" in lib.rfsn_last_error(), lib.rfsn_last_error()
+        assert lib.rfsn_paged_attention(p, 4096, 8, 0.125, 4096, count, 4096, 4096, 1 << 30, None) == -1
+
+
+def test_wrappers_refuse_page_counts_past_32_bits(monkeypatch):
+    """ctypes would pass 2^32 + 4 pages on as 4."""
+    from apple_amd import kernels as K
+
+    monkeypatch.setattr(K, "_paged", lambda what, pages, table, lens: (b"", (2, 2, 64, 16, 4), -1))
+    monkeypatch.setattr(K, "_paged_call", lambda *a: pytest.fail("the call was made"))
+    pages, table, lens = tensors()
+    q = torch.zeros((2, 4, 64), dtype=torch.float16)
+    for count in ((1 << 32) + 4, 1 << 31, (1 << 31) // 16):
+        with pytest.raises(ValueError, match="pages of 16"):
+            K.page_select(q, pages, table, torch.zeros(2, dtype=torch.int32, device="meta"), count)
+        with pytest.raises(ValueError, match="pages of 16"):
+            K.paged_attention(q, pages, table, lens, 0.1, torch.zeros((1, 1, 1), dtype=torch.int32).expand(2, 2, count))
+
+
 def test_workspace_sizes(lib):
     size = lib.rfsn_paged_attention_workspace_bytes
     assert size(None, 8, 0) == 0
