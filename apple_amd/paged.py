@@ -67,6 +67,7 @@ class RFSNPagedKVCache:
         self.num_tokens: List[int] = [0] * batch
         self._held: List[List[int]] = [[] for _ in range(batch)]
         self._free = list(range(pages - 1, -1, -1))
+        self._ended = set()  # released, and without tokens since
 
     @property
     def free_pages(self) -> int:
@@ -105,12 +106,17 @@ class RFSNPagedKVCache:
 
     def append(self, keys: torch.Tensor, values: torch.Tensor, counts: Optional[Sequence[int]] = None) -> None:
         """New rows [N, Hkv, D] of all sequences, ``counts[b]`` of sequence b in
-        the order of the batch (default: one each, a decode step)."""
+        the order of the batch (default: one each, a decode step).  While a
+        released sequence has no successor and others go on, ``counts`` has to be
+        given (0 for it): one more token each would start a sequence there."""
         k, v = self._rows(keys, "keys"), self._rows(values, "values")
         each = [1] * self.batch if counts is None else [int(c) for c in counts]
         if len(each) != self.batch or min(each) < 0 or sum(each) != k.shape[0] or v.shape != k.shape:
             raise ValueError(f"{k.shape[0]} key and {v.shape[0]} value rows do not match the counts of "
                              f"{self.batch} sequences")
+        if counts is None and self._ended and any(self.num_tokens):
+            raise ValueError(f"sequences {sorted(self._ended)} were released: append takes counts until they hold "
+                             "tokens again")
         self._reserve(each)
         if counts is None:
             K.paged_append(self.pages, self.table, self.lens, k, v)
@@ -123,6 +129,8 @@ class RFSNPagedKVCache:
             K.paged_append(self.pages, self.table, self.lens, k, v, on[0])
             self.lens.add_(on[1, :-1])
         self.num_tokens = [n + c for n, c in zip(self.num_tokens, each)]
+        if self._ended:
+            self._ended = {b for b in self._ended if not self.num_tokens[b]}
 
     def prefill(self, b: int, keys: torch.Tensor, values: torch.Tensor) -> None:
         """Rows [T, Hkv, D] behind what sequence b holds (a prompt, or a chunk of one)."""
@@ -139,6 +147,7 @@ class RFSNPagedKVCache:
         self.num_tokens[b] = 0
         self.table[b].fill_(-1)
         self.lens[b:b + 1].zero_()
+        self._ended.add(b)
 
     def _live_table(self) -> torch.Tensor:
         """The table's columns that some sequence uses."""

@@ -223,6 +223,44 @@ def test_cache_page_bookkeeping(monkeypatch):
     assert use["in_use"] * 5 == use["pool"] * 2 > 0
 
 
+def test_cache_steps_after_a_release(monkeypatch):
+    """A step without counts gives a released sequence no token: it is refused until a successor holds some, and takes
+    no page; a step of a batch that is released as a whole starts all of it again."""
+    from apple_amd import kernels as K
+    from apple_amd.paged import RFSNPagedKVCache
+
+    monkeypatch.setattr(K, "paged_append", lambda pages, table, lens, k, v, cu=None: None)
+    c = RFSNPagedKVCache(config(), batch=3, pages=6, page_size=16, device="cpu")
+    rows = lambda n: torch.zeros((n, 2, 64), dtype=torch.float16)
+    step = lambda *counts: c.append(rows(sum(counts) if counts else 3), rows(sum(counts) if counts else 3), counts or None)
+    step(5, 0, 7)
+    step()  # the second was never begun: it starts here
+    assert c.num_tokens == [6, 1, 8]
+    c.release(1)
+    for held in ([6, 0, 8], [7, 0, 9]):
+        with pytest.raises(ValueError, match=r"sequences \[1\] were released"):
+            step()
+        assert c.num_tokens == held == c.lens.tolist() and c.free_pages == 4 and c.table[1].tolist() == [-1] * 6
+        step(1, 0, 1)
+    c.prefill(1, rows(4), rows(4))
+    step()
+    assert c.num_tokens == [9, 5, 11]
+    for b in range(3):
+        c.release(b)
+    step()  # all of them begin
+    assert c.num_tokens == [1, 1, 1]
+    c.release(2)
+    c.release(0)
+    with pytest.raises(ValueError, match=r"\[0, 2\]"):
+        step()
+    step(1, 1, 0)
+    with pytest.raises(ValueError, match=r"\[2\]"):
+        step()
+    step(0, 0, 1)
+    step()
+    assert c.num_tokens == [2, 3, 2]
+
+
 def test_reference_quantiser_round_trip():
     """The host restatement itself: a value comes back within half a code step."""
     from tests.paged_reference import quantise
