@@ -17,26 +17,10 @@
 // One wave per head and chunk with fp32 FMAs (attend_row, now for sums that are not
 // finite alone) took 4,104 us for the first and 88 us for 1,021 positions.
 #include "paged.h"
+#include "paged_plan.h"
 
 namespace rfsn {
 namespace {
-
-// How a call is cut (Plan, below).  per_seq > 0: every sequence into that many chunks of `chunk`
-// listed positions (a list of pages, or one chunk).  0: by the lengths, which only the device
-// knows, into chunks of at least `chunk` positions.
-constexpr int kCUs = 256, kTries = 3;
-struct Cut {
-  int per_seq;
-  int units;                // blocks of a chunk (KV heads, and sets of 16 query heads)
-  int64_t chunk;
-  float one_over[kTries];   // 1 / chunks aimed at, for so many blocks per CU
-};
-// Chunks aimed at with k blocks on each CU: each sequence adds half of one on average, and a batch
-// that fills the chip by itself is cut where a sequence is longer than the mean.
-inline int aim(int k, int units, int batch) {
-  const int n = k * kCUs / units - batch / 2;
-  return n > batch ? n : batch;
-}
 
 struct Chunk {
   int b;       // sequence, -1: none
@@ -216,8 +200,6 @@ typedef short short4w __attribute__((ext_vector_type(4)));
 typedef short short8w __attribute__((ext_vector_type(8)));
 
 constexpr int NG = 2;              // groups of a wave's step
-constexpr double kLastLevelCache = 256 * 1024 * 1024;
-constexpr int kWideTiles = 8192;   // tiles of 32 positions of a call up to which blocks have many waves
 constexpr float kPBias = 8.f;      // a weight is kept as p 2^8
 constexpr float kPSum = 32768.f;   // a lane's sum below it: every weight is finite in fp16
 
@@ -661,64 +643,6 @@ paged_merge_kernel(const rfsn_paged p, int shift, int q_heads, int per_seq, cons
   }
 }
 
-// How a call is cut, by what the host knows: the sequences' capacity.
-struct Plan {
-  int64_t slots;  // of partial results
-  Cut cut;
-  bool wide;      // blocks of many waves
-  bool once;      // rows are loaded past the caches
-  bool split() const { return cut.per_seq != 1; }
-};
-int waves_of(int D, bool wide) { return !wide || D == 256 ? 4 : D == 64 ? 16 : 8; }  // (256: 8 would spill)
-Plan plan(const rfsn_paged& p, int q_heads, int count) {
-  const int64_t most = (int64_t)(count ? count : p.table_width) * p.page_size;
-  const int units = (int)(p.kv_heads * ceil_div(q_heads / p.kv_heads, 16));
-  Plan r;
-  // Blocks of many waves have all of a short call's loads in flight (8,192 positions x 8 KV heads of 64: 17 us in
-  // blocks of 4 waves, 12 so; 8 x 8,000: 31 in blocks of 4 and 37 so).  They also take a sequence without a
-  // merge where its steps cost less than one: 8 steps (4,096 positions of 64, 2,048 of 128) with blocks for most CUs
-  // (fp16, 8 KV heads: 24 x 4,000 of 64 43.6 -> 39.7 us, 32 x 1,900 of 128 53.3 -> 47.8, while 16 x 4,000, 128
-  // blocks, goes from 31 to 34), 4 with 64 (8 x 2,000: 14.2 -> 13.7), else 3 (1,021: 10.0 -> 8.6; 2,000 as 4: 10.3 ->
-  // 12.7).  Blocks of 4 waves take 512 positions so (1,024 x 300: 117 us, in wide blocks 193).
-  const int64_t blocks = (int64_t)p.batch * units, tiles = blocks * ceil_div(most, 32);
-  const int most_steps = blocks >= 192 ? 8 : blocks >= 64 ? 4 : 3;
-  r.wide = tiles <= kWideTiles ||
-           (most > 512 && blocks >= 192 && most <= most_steps * waves_of(p.head_dim, true) * 32);
-  // K and V of 256 MB or more, the size of the last-level cache, are gone from it before the next call reads them
-  // again: loaded as data that is used once they displace nothing and arrive sooner (32 x 32,768 positions, 8 KV heads
-  // of 64: fp16 374 -> 344 us, int8 220 -> 205; 4 x 8,000, 32 of 128: 99 -> 90, 16 x 8,192, 8 of 256: 196 -> 180).
-  // What fits stays for the next call (245 MB read again at once: 43 us, loaded so
-  // 47), blocks of many waves have less than that, and a list of pages reads few of them.
-  const double in_tables = (double)p.batch * p.table_width, pages = in_tables < p.pages ? in_tables : p.pages;
-  r.once = !r.wide && count == 0 &&
-           pages * p.page_size * p.kv_heads * p.head_dim * (p.type == RFSN_PAGE_FP16 ? 4 : 2) >= kLastLevelCache;
-  const int per_step = waves_of(p.head_dim, r.wide) * 32;
-  const int64_t least = r.wide ? per_step : 4 * per_step;  // positions of a chunk
-  if (most <= (r.wide ? most_steps : 4) * per_step) {
-    r.slots = p.batch, r.cut = {1, units, most > 0 ? most : 1, {}};
-  } else if (count) {
-    int64_t n = ceil_div(r.wide ? kCUs : 4 * kCUs, (int64_t)units * p.batch);
-    if (n > ceil_div(most, least)) n = ceil_div(most, least);
-    const int64_t chunk = ceil_div(ceil_div(most, n), per_step) * per_step;
-    n = ceil_div(most, chunk);
-    r.slots = n * p.batch, r.cut = {(int)n, units, chunk, {}};
-  } else {
-    const int first = r.wide ? 1 : 2;
-    r.cut = {0, units, least, {}};
-    int64_t most_chunks = 0;
-    for (int x = 0; x < kTries; ++x) {
-      const int n = aim(first + x, units, p.batch);
-      r.cut.one_over[x] = 1.f / (float)n;
-      most_chunks = n > most_chunks ? n : most_chunks;
-    }
-    // The sum of ceil(len / size) is at most total / size + batch, and size at least total / target - 0.02
-    // (find_chunk) and `least`: below 32767 (0.02 / 512 + 2^-21) < 2 chunks over the target (wide blocks
-    // have a `least` of 128 to 512, and at most 8,192 tiles of sequences longer than it).
-    r.slots = most_chunks + 2 + p.batch;
-    if (r.slots > ceil_div(most, least) * p.batch) r.slots = ceil_div(most, least) * p.batch;
-  }
-  return r;
-}
 size_t parts_bytes(const rfsn_paged& p, const Plan& c, int q_heads) {
   return (size_t)c.slots * q_heads * (p.head_dim + 2) * sizeof(float) + (size_t)p.batch * 2 * sizeof(int32_t);
 }
