@@ -89,7 +89,8 @@ class LinearParams(C.Structure):
 class Paged(C.Structure):
     _fields_ = [("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp), ("bounds", vp), ("table", vp), ("lens", vp),
                 ("page_stride", i64), ("head_stride", i64), ("table_stride", i64), ("pages", i32), ("page_size", i32),
-                ("kv_heads", i32), ("head_dim", i32), ("type", i32), ("batch", i32), ("table_width", i32)]
+                ("kv_heads", i32), ("head_dim", i32), ("type", i32), ("batch", i32), ("table_width", i32),
+                ("held_pages", i32)]
 
 
 class EncodeJob(C.Structure):

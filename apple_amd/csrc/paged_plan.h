@@ -57,7 +57,12 @@ inline Plan plan(const rfsn_paged& p, int q_heads, int count) {
   // of 64: fp16 374 -> 344 us, int8 220 -> 205; 4 x 8,000, 32 of 128: 99 -> 90, 16 x 8,192, 8 of 256: 196 -> 180).
   // What fits stays for the next call (245 MB read again at once: 43 us, loaded so
   // 47), blocks of many waves have less than that, and a list of pages reads few of them.
-  const double in_tables = (double)p.batch * p.table_width, pages = in_tables < p.pages ? in_tables : p.pages;
+  // What counts is what the call reads, as far as the host knows it: the pages that the caller says are held, else what
+  // the tables have room for, one table once, however many sequences go over it (512 queries over 8,192 positions, 2 KV
+  // heads of 256, fp16, took 650 us and 897 loaded so; 48 ragged sequences with 98 MB in a pool of 2.7 GB 24.8 and 27.0).
+  double pages = (p.table_stride == 0 ? 1.0 : (double)p.batch) * p.table_width;
+  if (pages > p.pages) pages = p.pages;
+  if (p.held_pages > 0 && pages > p.held_pages) pages = p.held_pages;
   r.once = !r.wide && count == 0 &&
            pages * p.page_size * p.kv_heads * p.head_dim * (p.type == RFSN_PAGE_FP16 ? 4 : 2) >= kLastLevelCache;
   const int per_step = waves_of(p.head_dim, r.wide) * 32;

@@ -724,10 +724,11 @@ class KVPages(NamedTuple):
     bounds: Optional[torch.Tensor] = None
 
 
-_PAGED_BLOCK = struct.Struct("7P3q7i4x")  # rfsn_paged, packed: a call's fields as they are, without a ctypes object
+_PAGED_BLOCK = struct.Struct("7P3q8i")  # rfsn_paged, packed: a call's fields as they are, without a ctypes object
 
 
-def _paged(what: str, pages: KVPages, table: torch.Tensor, lens: torch.Tensor) -> Tuple[bytes, tuple, int]:
+def _paged(what: str, pages: KVPages, table: torch.Tensor, lens: torch.Tensor,
+           held: int = 0) -> Tuple[bytes, tuple, int]:
     """The checked parameter block of a pool, a block table [B, W] int32 and
     lengths [B] int32: (block, (B, Hkv, D, S, W), device index)."""
     k, v, ks, vs, bounds = pages
@@ -774,7 +775,7 @@ def _paged(what: str, pages: KVPages, table: torch.Tensor, lens: torch.Tensor) -
     if max(P, H, S, D, B, W) >= 1 << 31:
         raise ValueError(f"{what}: sizes must stay below 2^31")
     return (_PAGED_BLOCK.pack(k.data_ptr(), v.data_ptr(), ks or 0, vs or 0, bounds or 0, table.data_ptr(),
-                              lens.data_ptr(), sp, sh, st, P, S, H, D, kind, B, W), (B, H, D, S, W), dev)
+                              lens.data_ptr(), sp, sh, st, P, S, H, D, kind, B, W, held), (B, H, D, S, W), dev)
 
 
 def _page_count(what: str, count: int, page_size: int) -> int:
@@ -897,12 +898,17 @@ def page_select(q: torch.Tensor, pages: KVPages, table: torch.Tensor, lens: torc
 
 
 def paged_attention(q: torch.Tensor, pages: KVPages, table: torch.Tensor, lens: torch.Tensor, scale: float,
-                    chosen: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    chosen: Optional[torch.Tensor] = None, held_pages: int = 0) -> torch.Tensor:
     """Exact attention of one query per sequence, q [B, Hq, D] fp16, over the
     sequence's first ``lens[b]`` positions, or over those of its pages that
     ``chosen`` [B, Hkv, n] (``page_select``) lists; zeros where there are none.
-    Codes are attended as code * scale in fp32, not rounded to fp16."""
-    block, sizes, dev = _paged("paged_attention", pages, table, lens)
+    Codes are attended as code * scale in fp32, not rounded to fp16.
+    ``held_pages``: the pages that the sequences hold together, where the caller
+    knows it; without it a call counts as reading what its table has room for,
+    which costs up to a tenth where that is far more."""
+    if not 0 <= held_pages < 1 << 31:
+        raise ValueError("paged_attention: held_pages must be a number of pages")
+    block, sizes, dev = _paged("paged_attention", pages, table, lens, held_pages)
     B, H, D, S, _ = sizes
     q = _paged_query("paged_attention", q, B, D, dev)
     count, listed = 0, None

@@ -167,7 +167,8 @@ class RFSNPagedKVCache:
             if sparse_pages < 2:
                 raise ValueError("sparse_pages must have room for the first and the newest page")
             chosen = K.page_select(qh, self.pages, table, self.lens, sparse_pages)
-        return K.paged_attention(qh, self.pages, table, self.lens, self.scale, chosen).to(q.dtype)
+        held = self.pages.k.shape[0] - len(self._free)
+        return K.paged_attention(qh, self.pages, table, self.lens, self.scale, chosen, held).to(q.dtype)
 
     def prompt_attention(self, b: int, q: torch.Tensor) -> torch.Tensor:
         """q [S, Hq, D], the newest S tokens of sequence b, each over the

@@ -611,6 +611,8 @@ typedef struct rfsn_paged {
   int32_t type;         /* RFSN_PAGE_* */
   int32_t batch;
   int32_t table_width;
+  int32_t held_pages;   /* pages that the sequences hold together, where the caller knows it, else 0: a hint of
+                         * rfsn_paged_attention's traffic, on which its speed alone depends */
 } rfsn_paged;
 
 /* Rows k, v [rows][kv_heads][head_dim] fp16 (token_stride, head_stride

@@ -554,6 +554,36 @@ def test_pools_past_the_last_level_cache(device, kind, dim, lens, times):
     R.check(got, *(x.repeat(times, 1, 1) for x in R.attention(pool, near, lens, q, dim ** -0.5)))
 
 
+@pytest.mark.parametrize("kind", ["fp16", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_what_the_caller_says_is_held_changes_no_bit(device, kind, dim):
+    """A pool of 300 MB with a few of its pages in use: the number of those, a far larger one or none; and many queries
+    over one sequence's pages, whose table is a row of stride 0."""
+    K = kernels()
+    count = 300_000_000 // (2 * 4 * 64 * dim * (2 if kind == "fp16" else 1))
+    small = R.Pool(kind, 60, 4, 64, dim, seed=dim, bounds=False)
+    lens = [3000, 0, 17, 555]
+    near = small.tables(lens)
+    poison(small, near, lens)
+    q = small.randn((4, 16, dim), 2.0)
+    far = [None if x is None else torch.cat([x.new_zeros((count - 60, *x.shape[1:])), x]) for x in
+           (None if x is None else x.view(torch.uint8) if x.element_size() == 1 else x for x in small.pages(device))]
+    pages = K.KVPages(*(x if y is None or y.element_size() > 1 else x.view(y.dtype) for x, y in zip(far, small.pages(device))))
+    table = torch.full((4, count // 4 + 1), -1, dtype=torch.int32)
+    table[:, :near.shape[1]] = torch.where(near >= 0, near + count - 60, near)
+    table, n = table.to(device), i32(lens, device)
+    got = [K.paged_attention(q.to(device), pages, table, n, dim ** -0.5, None, held) for held in (0, 60, 1 << 30)]
+    R.check(got[0], *R.attention(small, near, lens, q, dim ** -0.5))
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+    ends = [1 + 97 * i for i in range(30)]
+    q = small.randn((30, 16, dim), 2.0)
+    got = K.paged_attention(q.to(device), pages, table[:1].expand(30, -1), i32(ends, device), dim ** -0.5)
+    R.check(got, *R.attention(small, near[:1].expand(30, -1), ends, q, dim ** -0.5))
+    for held in (-1, 1 << 31):
+        with pytest.raises(ValueError, match="held_pages"):
+            K.paged_attention(q.to(device), pages, table[:1].expand(30, -1), i32(ends, device), 0.1, None, held)
+
+
 def test_another_stream(device):
     K = kernels()
     pool = R.Pool("int8", 120, 2, 16, 64, seed=45)

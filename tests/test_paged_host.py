@@ -119,7 +119,7 @@ def test_wrappers_refuse_page_counts_past_32_bits(monkeypatch):
     """ctypes would pass 2^32 + 4 pages on as 4."""
     from apple_amd import kernels as K
 
-    monkeypatch.setattr(K, "_paged", lambda what, pages, table, lens: (b"", (2, 2, 64, 16, 4), -1))
+    monkeypatch.setattr(K, "_paged", lambda *a: (b"", (2, 2, 64, 16, 4), -1))
     monkeypatch.setattr(K, "_paged_call", lambda *a: pytest.fail("the call was made"))
     pages, table, lens = tensors()
     q = torch.zeros((2, 4, 64), dtype=torch.float16)
@@ -274,3 +274,73 @@ def test_reference_quantiser_round_trip():
         half = scale[:, None] * 0.5 if step is None else torch.maximum(x.float().abs() * step, scale[:, None] * 2.0 ** -10)
         assert ((back - x.float()).abs() <= half * (1 + 1e-5)).all()
         assert (codes[7].float() == 0).all() and scale[7] == 0
+
+
+# ------------------------------------------------------------------ the plan of an attention call
+
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    """(slots, wide, once, chunks per sequence, chunk) of a call, from the host's own source."""
+    at = tmp_path_factory.mktemp("plan")
+    (at / "plan.cc").write_text('''#include "paged_plan.h"
+extern "C" void plan_of(const rfsn_paged* p, int q_heads, int count, int64_t* out, float* one_over) {
+  const rfsn::Plan r = rfsn::plan(*p, q_heads, count);
+  out[0] = r.slots, out[1] = r.wide, out[2] = r.once, out[3] = r.cut.per_seq, out[4] = r.cut.chunk;
+  for (int x = 0; x < rfsn::kTries; ++x) one_over[x] = r.cut.one_over[x];
+}
+''')
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-shared", "-fPIC", f"-I{ROOT / 'include'}",
+                    f"-I{ROOT / 'apple_amd' / 'csrc'}", str(at / "plan.cc"), "-o", str(at / "plan.so")], check=True)
+    fn = ctypes.CDLL(str(at / "plan.so")).plan_of
+
+    def call(q_heads, count=0, **kw):
+        out, one_over = (ctypes.c_int64 * 5)(), (ctypes.c_float * 3)()
+        fn(ctypes.byref(block(**kw)), q_heads, count, out, one_over)
+        return dict(zip(("slots", "wide", "once", "per_seq", "chunk"), out), one_over=list(one_over))
+
+    return call
+
+
+def test_rows_count_as_used_once_by_what_is_read(plan):
+    """256 MB of pages that a call reads, not of pages that there are or that wide tables could name."""
+    # a pool of 4 GB: 2 MB of K and V a page with 8 heads of 256
+    pool = dict(pages=2048, page_size=256, kv_heads=8, head_dim=256)
+    for batch, width, held, once in ((64, 5, 0, True), (65, 2, 0, True), (64, 8, 127, False), (64, 8, 128, True),
+                                     (64, 8, 1 << 30, True), (64, 2048, 100, False), (64, 2048, 0, True)):
+        assert plan(32, batch=batch, table_width=width, table_stride=width, held_pages=held, **pool)["once"] == once
+    # many queries over one sequence's pages: one row of the table for all of them
+    for width, once in ((32, False), (127, False), (128, True)):
+        assert plan(32, batch=512, table_width=width, table_stride=0, **pool)["once"] == once
+        assert plan(32, batch=512, table_width=width, table_stride=width, **pool)["once"]
+    # a list of pages, and blocks of many waves, are never loaded so
+    assert not plan(32, count=16, batch=64, table_width=64, table_stride=64, **pool)["once"]
+
+
+def test_a_hint_changes_nothing_but_how_rows_are_loaded(plan, lib):
+    for kw in (dict(batch=48, table_width=250, page_size=64, kv_heads=4), dict(batch=1, table_width=4096, kv_heads=8),
+               dict(batch=600, table_width=600, kv_heads=2)):
+        a, b = (plan(32, pages=1 << 20, held_pages=n, **kw) for n in (0, 3))
+        a.pop("once"), b.pop("once")
+        assert a == b
+        sizes = [lib.rfsn_paged_attention_workspace_bytes(ctypes.byref(block(pages=1 << 20, held_pages=n, **kw)), 32, 0)
+                 for n in (0, 3)]
+        assert sizes[0] == sizes[1] > 0
+
+
+def test_cache_says_what_it_holds(monkeypatch):
+    from apple_amd import kernels as K
+    from apple_amd.paged import RFSNPagedKVCache
+
+    said = []
+    monkeypatch.setattr(K, "paged_append", lambda *a: None)
+    monkeypatch.setattr(K, "paged_attention", lambda q, pages, table, lens, scale, chosen=None, held_pages=0:
+                        said.append((held_pages, table.stride(0))) or q)
+    c = RFSNPagedKVCache(config(), batch=2, pages=20, page_size=16, device="cpu")
+    rows = torch.zeros((60, 2, 64), dtype=torch.float16)
+    c.append(rows, rows, [35, 25])
+    c.attention_forward(torch.zeros((2, 8, 64)))
+    wide = RFSNPagedKVCache(config(head_dim=256, subspace_dim=32), batch=2, pages=20, page_size=16, device="cpu")
+    rows = torch.zeros((60, 2, 256), dtype=torch.float16)
+    wide.append(rows, rows, [35, 25])
+    wide.prompt_attention(0, torch.zeros((7, 8, 256)))
+    assert said == [(5, 20), (0, 0)]  # two tables of 3 and 2 pages; one row for all queries of a chunk
