@@ -62,6 +62,7 @@ __device__ __forceinline__ Chunk find_chunk(const rfsn_paged& p, int shift, cons
     const float each = total * cut.one_over[x] + 0.98f;  // rounded up, but for an excess that is fp32's
     uint32_t s = each < 2147483520.f ? (uint32_t)each : 2147483520u;
     s = s <= (uint32_t)cut.chunk ? (uint32_t)cut.chunk : (s + 127) & ~127u;
+    if (s > cut.longest) s = (uint32_t)cut.longest;
     uint32_t n = parts_of((uint32_t)len0, s), most = about(len0, n);
     for (int b = 64 + lane; b < p.batch; b += 64) {
       const uint32_t len = (uint32_t)paged_len(p, shift, b), m = parts_of(len, s);
@@ -184,10 +185,13 @@ __device__ __forceinline__ void attend_row(const rfsn_paged& p, int shift, const
 //                  (lane group g, j) is position 16 (j >> 2) + 4 g + (j & 3).  V passes
 //                  through LDS of the wave's own, and ds_read_b64_tr_b16 reads V^T from it
 //                  in that order.
-// Weights are rounded twice, which leaves them off by 2^-22 of themselves (fp16 pages: p 2^8 as
-// fp16 hi + lo) or 2^-16 (8-bit pages: p times the row's scale as bf16 hi + lo, which has fp32's range;
-// codes are exact in bf16), both well under the 2^-11 of the result's own rounding; the second product
-// costs matrix-core time that is idle.  Scores, maxima, sums and O are fp32.
+// Weights are rounded twice.  With 8-bit pages p times the row's scale is bf16 hi + lo, which has fp32's range, and
+// off by 2^-16 of itself (codes are exact in bf16).  With fp16 pages p 2^8 is fp16 hi + lo: off by 2^-22 of itself
+// or by 2^-33 of the largest weight that the wave has seen, whichever is more, because fp16 ends at 2^-24; what
+// is under 2^-33 adds nothing to O and counts in l.  N positions of a wave are then off by at most N 2^-33 of the
+// largest |v|, and no wave has more than 2^20 (kLongestChunk; tables for over 2^37 positions aside).  All of it is
+// well under the 2^-11 of the result's own rounding; the second product costs matrix-core time that is idle.
+// Scores, maxima, sums and O are fp32.
 // Where V or a score is infinite or NaN, hi, lo and weights of 0 meet it apart; a block that
 // finds a sum that is not finite takes its chunk again by attend_row.
 

@@ -17,6 +17,7 @@ struct Cut {
   int per_seq;
   int units;                // blocks of a chunk (KV heads, and sets of 16 query heads)
   int64_t chunk;
+  int64_t longest;          // positions that a chunk has at most
   float one_over[kTries];   // 1 / chunks aimed at, for so many blocks per CU
 };
 // Chunks aimed at with k blocks on each CU: each sequence adds half of one on average, and a batch
@@ -27,6 +28,10 @@ inline int aim(int k, int units, int batch) {
 }
 
 constexpr double kLastLevelCache = 256 * 1024 * 1024;
+// Of fp16 pages a wave drops weights below 2^-33 of the largest that it sees from its products with V, and
+// rounds others by as much (paged_attention.hip), so a chunk of four waves is off by at most 2^20 2^-33 of the
+// largest |v|, a quarter of fp16's half step.
+constexpr int64_t kLongestChunk = 1 << 22;
 constexpr int kWideTiles = 8192;   // tiles of 32 positions of a call up to which blocks have many waves
 
 // By sizes and the sequences' capacity; paged_attention.hip cuts by the lengths within it.
@@ -67,17 +72,20 @@ inline Plan plan(const rfsn_paged& p, int q_heads, int count) {
            pages * p.page_size * p.kv_heads * p.head_dim * (p.type == RFSN_PAGE_FP16 ? 4 : 2) >= kLastLevelCache;
   const int per_step = waves_of(p.head_dim, r.wide) * 32;
   const int64_t least = r.wide ? per_step : 4 * per_step;  // positions of a chunk
+  int64_t longest = kLongestChunk;
+  while (longest < most && div_up(most, longest) * p.batch > 32768) longest *= 2;  // the grid ends at 65,535 chunks
   if (most <= (r.wide ? most_steps : 4) * per_step) {
-    r.slots = p.batch, r.cut = {1, units, most > 0 ? most : 1, {}};
+    r.slots = p.batch, r.cut = {1, units, most > 0 ? most : 1, longest, {}};
   } else if (count) {
     int64_t n = div_up(r.wide ? kCUs : 4 * kCUs, (int64_t)units * p.batch);
     if (n > div_up(most, least)) n = div_up(most, least);
+    if (n < div_up(most, longest)) n = div_up(most, longest);
     const int64_t chunk = div_up(div_up(most, n), per_step) * per_step;
     n = div_up(most, chunk);
-    r.slots = n * p.batch, r.cut = {(int)n, units, chunk, {}};
+    r.slots = n * p.batch, r.cut = {(int)n, units, chunk, longest, {}};
   } else {
     const int first = r.wide ? 1 : 2;
-    r.cut = {0, units, least, {}};
+    r.cut = {0, units, least, longest, {}};
     int64_t most_chunks = 0;
     for (int x = 0; x < kTries; ++x) {
       const int n = aim(first + x, units, p.batch);
@@ -86,8 +94,10 @@ inline Plan plan(const rfsn_paged& p, int q_heads, int count) {
     }
     // The sum of ceil(len / size) is at most total / size + batch, and size at least total / target - 0.02
     // (find_chunk) and `least`: below 32767 (0.02 / 512 + 2^-21) < 2 chunks over the target (wide blocks
-    // have a `least` of 128 to 512, and at most 8,192 tiles of sequences longer than it).
+    // have a `least` of 128 to 512, and at most 8,192 tiles of sequences longer than it).  Chunks of `longest`
+    // positions are as many as the sequences' capacity has.
     r.slots = most_chunks + 2 + p.batch;
+    if (r.slots < div_up(most, longest) * p.batch) r.slots = div_up(most, longest) * p.batch;
     if (r.slots > div_up(most, least) * p.batch) r.slots = div_up(most, least) * p.batch;
   }
   return r;

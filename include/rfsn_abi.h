@@ -650,8 +650,10 @@ int rfsn_page_select(const rfsn_paged* p, const void* q, int32_t q_heads, int32_
  * i / (q_heads / kv_heads).  chosen (or NULL): [batch][kv_heads][count] page ordinals,
  * the only pages that are attended, one listed twice counting twice.  Nothing
  * to attend, or scores all -infinite: zeros.  Weights are fp32: one under its
- * smallest value is 0, which makes an infinite value NaN.  The workspace size depends on
- * q_heads and, with chosen, count (0: dense). */
+ * smallest value is 0, which makes an infinite value NaN.  Products with finite values take them to
+ * 2^-16 of themselves or, from fp16 pages, to 2^-22 of themselves or 2^-33 of the largest, whichever is more: at
+ * most 2^-13 of the largest |v| at any length (unless the tables have room for over 2^37 positions).
+ * The workspace size depends on q_heads and, with chosen, count (0: dense). */
 size_t rfsn_paged_attention_workspace_bytes(const rfsn_paged* p, int32_t q_heads, int32_t count);
 int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t q_heads, float scale, const int32_t* chosen,
                          int32_t count, void* out, void* workspace, size_t workspace_bytes, void* stream);

@@ -374,6 +374,30 @@ def test_chunks_of_many_tiles(device, kind, batch, heads, tokens, count, size):
                 assert ((got[b, 2 * h + g] - want).abs() <= tol).all(), (b, h, g)
 
 
+def test_small_weights_of_a_very_long_sequence(device):
+    """One position with a value of 0 and 2^24 - 1 with 2^-33.5 of its weight and a value of 2^15, in fp16 pages, and so
+    many heads that the chip is full without cutting the sequence.  The wave that sees the first position loses the
+    others' weights, which are below fp16's range there; every other wave goes by its own largest weight.
+
+    The tolerance: the wave with the first position drops up to 2^20 weights of up to 2^-33; fp16's half step of the
+    output; 2^-16 of it for the weights' exponent (a score of 33.5 in base 2 is off by 2^-18) and roundings."""
+    K = kernels()
+    heads, tokens, dim = 512, 1 << 24, 64
+    k, v = (torch.zeros((2, heads, 16, dim), dtype=D16, device=device) for _ in range(2))
+    v[:] = 32768.0
+    v[0, :, 0] = 0.0
+    k[0, :, 0, 0] = 23.21875
+    table = torch.ones((1, tokens // 16), dtype=torch.int32, device=device)
+    table[0, 0] = 0
+    q = torch.zeros((1, heads, dim), dtype=D16, device=device)
+    q[:, :, 0] = 1.0
+    got = K.paged_attention(q, K.KVPages(k, v), table, i32([tokens], device), 1.0).double()
+    w = math.exp(-23.21875)
+    want = 32768.0 * (tokens - 1) * w / (1.0 + (tokens - 1) * w)
+    off = float((got - want).abs().max())
+    assert off <= 2.0 ** 20 * 2.0 ** -33 * 32768 + want * (2.0 ** -11 + 2.0 ** -16), (off, want)
+
+
 # ------------------------------------------------------------------ page choice
 
 @pytest.mark.parametrize("dim, heads, group, size, count, first, last", [

@@ -285,7 +285,7 @@ def plan(tmp_path_factory):
     (at / "plan.cc").write_text('''#include "paged_plan.h"
 extern "C" void plan_of(const rfsn_paged* p, int q_heads, int count, int64_t* out, float* one_over) {
   const rfsn::Plan r = rfsn::plan(*p, q_heads, count);
-  out[0] = r.slots, out[1] = r.wide, out[2] = r.once, out[3] = r.cut.per_seq, out[4] = r.cut.chunk;
+  out[0] = r.slots, out[1] = r.wide, out[2] = r.once, out[3] = r.cut.per_seq, out[4] = r.cut.chunk, out[5] = r.cut.longest;
   for (int x = 0; x < rfsn::kTries; ++x) one_over[x] = r.cut.one_over[x];
 }
 ''')
@@ -294,9 +294,9 @@ extern "C" void plan_of(const rfsn_paged* p, int q_heads, int count, int64_t* ou
     fn = ctypes.CDLL(str(at / "plan.so")).plan_of
 
     def call(q_heads, count=0, **kw):
-        out, one_over = (ctypes.c_int64 * 5)(), (ctypes.c_float * 3)()
+        out, one_over = (ctypes.c_int64 * 6)(), (ctypes.c_float * 3)()
         fn(ctypes.byref(block(**kw)), q_heads, count, out, one_over)
-        return dict(zip(("slots", "wide", "once", "per_seq", "chunk"), out), one_over=list(one_over))
+        return dict(zip(("slots", "wide", "once", "per_seq", "chunk", "longest"), out), one_over=list(one_over))
 
     return call
 
@@ -325,6 +325,58 @@ def test_a_hint_changes_nothing_but_how_rows_are_loaded(plan, lib):
         sizes = [lib.rfsn_paged_attention_workspace_bytes(ctypes.byref(block(pages=1 << 20, held_pages=n, **kw)), 32, 0)
                  for n in (0, 3)]
         assert sizes[0] == sizes[1] > 0
+
+
+def chunks_by_lengths(cut, lens):
+    """Chunks of each sequence for each size that the device may choose, and the longest of them: find_chunk's arithmetic
+    in fp32."""
+    f = torch.float32
+    for one_over in cut["one_over"]:
+        each = torch.tensor(sum(lens), dtype=f) * torch.tensor(one_over, dtype=f) + torch.tensor(0.98, dtype=f)
+        size = min(int(each), 2147483520)
+        size = cut["chunk"] if size <= cut["chunk"] else (size + 127) // 128 * 128
+        size = min(size, cut["longest"])
+        n = [-(-t // size) for t in lens]
+        yield sum(n), max((-(-(-(-t // m)) // 128) * 128 for t, m in zip(lens, n) if m), default=0)
+
+
+def test_every_chunk_has_a_slot_and_none_is_too_long(plan):
+    """Batches of one to many sequences, alike and ragged, up to the capacity's limit."""
+    import random
+
+    rng = random.Random(7)
+    seen = 0
+    for i in range(600):
+        batch = rng.choice([1, 1, 2, 3, 31, 64, 65, 500, 4000, 32000])
+        size = rng.choice([16, 64, 256])
+        most = 2 ** 31 - 1024 if i % 4 == 0 else int(2 ** rng.uniform(7, 30.9))
+        heads, group, dim = rng.choice([1, 2, 8, 32, 512, 3000]), rng.choice([1, 4, 20]), rng.choice([64, 128, 256])
+        width = max(1, most // size)
+        cut = plan(heads * group, batch=batch, table_width=width, table_stride=width, page_size=size, kv_heads=heads, head_dim=dim)
+        assert cut["longest"] >= 1 << 22
+        assert cut["longest"] == 1 << 22 or (cut["longest"] // 2 < width * size and
+                                             -(-width * size // (cut["longest"] // 2)) * batch > 32768)
+        if cut["per_seq"]:
+            assert cut["per_seq"] == 1 and cut["slots"] == batch and cut["chunk"] == width * size <= 4096
+            continue
+        seen += 1
+        lens = [width * size if rng.random() < 0.5 else int((width * size) ** rng.random()) for _ in range(min(batch, 500))]
+        lens = (lens * -(-batch // len(lens)))[:batch]
+        for all_of in (lens, [width * size] * batch, [0] * (batch - 1) + [width * size]):
+            for chunks, longest in chunks_by_lengths(cut, all_of):
+                assert chunks <= cut["slots"] and longest <= max(cut["longest"], cut["chunk"]), (cut, chunks, longest)
+        if batch <= 4000:
+            assert cut["slots"] <= 65535
+    assert seen > 200
+
+
+def test_lists_of_pages_are_cut_below_the_longest_chunk(plan):
+    for batch, heads, count, size in ((1, 512, 1 << 19, 64), (3, 700, (1 << 31) // 16 - 64, 16), (1, 1, 1 << 22, 256), (64, 8, 128, 16),
+                                      (2000, 4, 1 << 18, 256), (40000, 1, 1 << 20, 64), (512, 8, 1 << 16, 256)):
+        cut = plan(heads, count, batch=batch, table_width=1 << 20, page_size=size, kv_heads=heads)
+        assert cut["per_seq"] * cut["chunk"] >= count * size and cut["slots"] == cut["per_seq"] * batch <= 65535
+        assert (cut["per_seq"] - 1) * cut["chunk"] < count * size
+        assert cut["chunk"] <= cut["longest"] and (cut["longest"] == 1 << 22 or batch > 64)
 
 
 def test_cache_says_what_it_holds(monkeypatch):
