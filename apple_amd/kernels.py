@@ -879,7 +879,9 @@ def page_select(q: torch.Tensor, pages: KVPages, table: torch.Tensor, lens: torc
     sequence's: int32 [B, Hkv, count] page ordinals, ascending, then -1.  The
     ``first`` and ``last`` ones are always among them, the others those with the
     largest upper bound of q . k by the pages' bounds, over the KV head's query
-    heads (``rfsn_page_select``)."""
+    heads (``rfsn_page_select``).  The bounds are of the keys as they were
+    appended: of 8-bit pages, whose values differ by their rounding, the score is
+    an estimate."""
     block, sizes, dev = _paged("page_select", pages, table, lens)
     B, H, D, S, W = sizes
     if pages.bounds is None:

@@ -157,7 +157,8 @@ class RFSNPagedKVCache:
         """q [B, Hq, D], each sequence's newest token, over the sequence's
         positions -> [B, Hq, D] in q's dtype; an empty sequence gives zeros.
         ``sparse_pages``: over that many of its pages per KV head, the first, the
-        newest and those whose bounds promise the largest scores."""
+        newest and those whose bounds promise the largest scores (of keys before
+        their rounding to 8 bits)."""
         if q.dim() != 3 or q.shape[0] != self.batch or q.shape[2] != self.D:
             raise ValueError(f"q must be [{self.batch}, heads, {self.D}]")
         qh = q.to(device=self.device, dtype=torch.float16)

@@ -635,9 +635,12 @@ int rfsn_paged_read(const rfsn_paged* p, const int32_t* cu, int64_t rows, void* 
 /* The pages that a query reads, [batch][kv_heads][count] page ordinals of the
  * sequence (not page numbers of the pool), ascending, then -1: the first and last
  * ones, then those of the highest score max_g sum_d max(q_d, 0) hi_d +
- * min(q_d, 0) lo_d over the KV head's query heads g, which no q . k of the
- * page exceeds.  The sum is exact up to 64-bit rounding and rounded to fp32;
- * NaN counts as infinite, ties go to the lower ordinal.  q [batch][q_heads]
+ * min(q_d, 0) lo_d over the KV head's query heads g.  The sum is exact up to
+ * 64-bit rounding and rounded to fp32; but for these roundings no q . k exceeds
+ * it, k a key of the page as it was appended.  What is attended of an 8-bit page,
+ * code * scale, may: by sum_d |q_d| e_d, e_d = scale / 2 of the row (int8) or the larger of
+ * 2^-4 |k_d| and 2^-10 scale (e4m3), so there the score is an estimate.  NaN
+ * counts as infinite, ties go to the lower ordinal.  q [batch][q_heads]
  * [head_dim] fp16.  count * page_size is at most 2^31 - 1024,
  * here and in rfsn_paged_attention. */
 size_t rfsn_page_select_workspace_bytes(const rfsn_paged* p);

@@ -276,6 +276,43 @@ def test_reference_quantiser_round_trip():
         assert (codes[7].float() == 0).all() and scale[7] == 0
 
 
+@pytest.mark.parametrize("kind", ["fp16", "int8", "e4m3"])
+def test_what_a_page_s_score_says_of_its_keys(kind):
+    """No q . k of the keys as they were appended exceeds the page's score; what is attended of an 8-bit page may, by half a
+    code step per coordinate: int8 stores 0.6 beside 127 as 1."""
+    from tests import paged_reference as R
+
+    g = torch.Generator().manual_seed(5)
+    over = 0
+    for trial in range(60):
+        rows = 1 if trial % 2 else 16
+        k = torch.randn((rows, 64), generator=g).half()
+        q = torch.randn(64, generator=g).half()
+        if trial == 1:  # values that round up: 0.6 to 1, and 1.07 to 1.125 (e4m3 turns at 1.0625)
+            k[0], q[:] = 0, 0
+            k[0, 0], k[0, 1], q[1] = (127.0, 0.6, 8.0) if kind == "int8" else (448.0, 1.07, 8.0)
+        pool = R.Pool(kind, 1, 1, 16, 64, seed=1)
+        pool.append(torch.zeros((1, 1), dtype=torch.int32), [0], k[:, None], k[:, None], [0, rows])
+        lo, hi = pool.bounds[0, 0].double()
+        x = q.double()
+        score = float((x.clamp(min=0) * hi + x.clamp(max=0) * lo).sum().float())
+        slack = 2.0 ** -24 * abs(score)  # the score's rounding to fp32
+        assert float((k.double() @ x).max()) <= score + slack
+        held = pool.values("k")[0, 0, :rows]
+        if kind == "fp16":
+            assert torch.equal(held, k.double())
+            continue
+        scale = pool.k_scale[0, 0, :rows].double()[:, None]
+        half = scale / 2 if kind == "int8" else torch.maximum(k.double().abs() * 2.0 ** -4, scale * 2.0 ** -10)
+        # the quantiser's own product and reciprocal are off by 2^-22 of the value
+        more = ((half + k.double().abs() * 2.0 ** -22) * x.abs()).sum(-1)
+        assert (held @ x <= score + slack + more).all()
+        over += bool((held @ x > score + slack).any())
+        if trial == 1:
+            assert float((held @ x)[0]) > score + 0.1
+    assert over > 0 or kind == "fp16"
+
+
 # ------------------------------------------------------------------ the plan of an attention call
 
 @pytest.fixture(scope="module")
