@@ -202,6 +202,55 @@ def test_pages_outside_the_pool_and_rows_past_the_table(device):
         assert len(before) == len([t for t in pages if t is not None])
 
 
+@pytest.mark.parametrize("kind", ["fp16", "int8", "e4m3"])
+@pytest.mark.parametrize("batch", [3, 70])
+def test_row_offsets_that_are_no_prefix_write_nothing(device, kind, batch):
+    """``cu`` that no row n has a sequence in (cu[b] <= n < cu[b + 1]): the pool stays as it is, and zeros are read."""
+    K = kernels()
+    pool = R.Pool(kind, 2 * batch, 2, 16, 64, seed=batch)
+    table = torch.randperm(2 * batch, generator=pool.g).int().view(batch, 2).to(device)
+    k, v = (pool.randn((90, 2, 64)).to(device) for _ in range(2))
+    falling = [90 - 90 * i // batch for i in range(batch + 1)]
+    for cu in ([5] * (batch + 1), falling, [100] * (batch + 1), [-7] * (batch + 1), [100 + i for i in range(batch + 1)],
+               [-100 + i for i in range(batch + 1)]):
+        for starts in ([0] * batch, [2147483647, -5, 31] + [9] * (batch - 3)):
+            pages = pool.pages(device)
+            K.paged_append(pages, table, i32(starts, device), k, v, i32(cu, device))
+            for name, got in pages._asdict().items():
+                want = getattr(pool, name)
+                if want is not None:
+                    assert torch.equal(got.cpu().view(torch.uint8), want.view(torch.uint8)), (name, cu[:4])
+            for x in K.paged_read(pages, table, i32(starts, device), i32(cu, device), 90):
+                assert not x.any(), cu[:4]
+            out = tuple(torch.full((90, 2, 64), 3.0, dtype=D16, device=device) for _ in range(2))
+            K.paged_read(pages, table, i32(starts, device), i32(cu, device), 90, out)
+            assert (out[0] == 3.0).all() and (out[1] == 3.0).all()
+
+
+@pytest.mark.parametrize("kind", ["fp16", "int8"])
+@pytest.mark.parametrize("batch", [5, 63, 64, 130])
+def test_any_row_offsets_stay_in_the_tables_pages(device, kind, batch):
+    """``cu`` of any numbers and lengths past every table: only pages that a table names are written."""
+    K = kernels()
+    pool = R.Pool(kind, 3 * batch + 40, 2, 16, 64, seed=batch)
+    order = torch.randperm(pool.count, generator=pool.g).int()
+    table, rest = order[:2 * batch].view(batch, 2).clone(), order[2 * batch:].long()
+    table[1, 0], table[2, 1] = -1, pool.count
+    k, v = (pool.randn((300, 2, 64)).to(device) for _ in range(2))
+    pages = pool.pages(device)
+    for trial in range(12):
+        cu = torch.randint(-50, 400, (batch + 1,), generator=pool.g, dtype=torch.int32)
+        if trial % 3 == 0:
+            cu[::2], cu[1::2] = -4, 300 + trial
+        starts = torch.randint(-5, 60, (batch,), generator=pool.g, dtype=torch.int32)
+        starts[trial % batch] = 2147483647
+        K.paged_append(pages, table.to(device), starts.to(device), k, v, cu.to(device))
+        for name, got in pages._asdict().items():
+            want = getattr(pool, name)
+            if want is not None:
+                assert torch.equal(got.cpu()[rest].view(torch.uint8), want[rest].view(torch.uint8)), (name, trial)
+
+
 # ------------------------------------------------------------------ attention
 
 LENGTHS = [[0], [1], [15, 16, 17], [31, 0, 33, 64], [129, 1, 500, 511], [513, 2, 1200], [3001]]
