@@ -240,8 +240,9 @@ __device__ __forceinline__ void store_page(V x, V* at) {
 // sequence in one page) takes those of the run's keys that it holds and reads the others, and
 // writes the page's bounds, so no two waves write the same ones and no order changes them.  Bounds
 // take 2 us of 101 for 16,384 x 32 x 128 in fp16, 14 of 97 in int8, 1.8 of 8.4 for 8,191 x 8 x 64.
-// V, which no other wave reads, is loaded past the caches in rows of 64 (8,191 x 8: fp16 9.4 -> 8.4 us, int8
-// 10.8 -> 10.0; 8,192 x 8 rows of 128 or more lose 1 %: 16.3 -> 16.5).
+// V, which no other wave reads, is loaded past the caches in rows of 64 (32,768 x 8: fp16 30.7 -> 28.3 us, int8
+// 29.4 -> 27.7, e4m3 29.2 -> 27.4; 65,536 x 32: 202 alike, 173 -> 171, 173 -> 172; 5,000 to 16,384 x 8 lose or gain 1 %:
+// 8,191 fp16 9.15 -> 9.10, int8 10.5 -> 10.6; 8,192 x 8 rows of 128 or more lose 1 %: 16.3 -> 16.5).
 template <int D, int TYPE, int I>
 __global__ void __launch_bounds__(256)
 paged_append_kernel(const rfsn_paged p, int shift, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
@@ -393,8 +394,9 @@ __device__ __forceinline__ double group_sum(double x) {
 // bounds, D / 8 lanes a page, a wave U sets of pages, whose loads are all in flight together.
 // Sums are held in 64 bits; the bounds are converted once for all query heads, which leaves two
 // fused multiply-adds per coordinate and head.  2,048 pages x 4 KV heads of 64, 8 query heads each:
-// 5.3 us, latency; 32 x 2,048 pages x 8 KV heads, 4 query heads: 44 us for 134 MB, the 64-bit
-// operations and HBM about alike.
+// 5.3 us, latency; 32 x 2,048 pages x 8 KV heads, 4 query heads: 44 us for 134 MB, 63 % of the copy rate, with vector
+// instructions in some 60 % of the SIMDs' issue cycles; 32 ragged sequences of up to 2,048 pages: 11.8 us for 17 MB,
+// a third of them, and waves that wait in 56 % of their cycles.
 constexpr int kScoreSets = 2;
 template <int D>
 __global__ void __launch_bounds__(256)

@@ -173,7 +173,9 @@ class RFSNPagedKVCache:
 
     def prompt_attention(self, b: int, q: torch.Tensor) -> torch.Tensor:
         """q [S, Hq, D], the newest S tokens of sequence b, each over the
-        positions up to its own -> [S, Hq, D] in q's dtype."""
+        positions up to its own -> [S, Hq, D] in q's dtype.  Rows of 8-bit pages
+        are read back as fp16 first at head sizes 64 and 128, while
+        ``attention_forward`` takes code * scale as it is."""
         n = self.num_tokens[self._index(b)]
         if q.dim() != 3 or q.shape[2] != self.D or q.shape[0] > n:
             raise ValueError(f"q must be [S, heads, {self.D}] of at most the {n} tokens held")
