@@ -90,7 +90,14 @@ class Paged(C.Structure):
     _fields_ = [("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp), ("bounds", vp), ("table", vp), ("lens", vp),
                 ("page_stride", i64), ("head_stride", i64), ("table_stride", i64), ("pages", i32), ("page_size", i32),
                 ("kv_heads", i32), ("head_dim", i32), ("type", i32), ("batch", i32), ("table_width", i32),
-                ("held_pages", i32)]
+                ("held_pages", i32), ("weight", vp)]
+
+
+class RotaryParams(C.Structure):
+    _fields_ = [("x", vp * 2), ("out", vp * 2), ("row_stride", i64 * 2), ("head_stride", i64 * 2),
+                ("out_row_stride", i64 * 2), ("out_head_stride", i64 * 2), ("positions", vp), ("inv_freq", vp),
+                ("rows", i64), ("heads", i32 * 2), ("head_dim", i32), ("rotary_dim", i32), ("layout", i32),
+                ("type", i32), ("wide_positions", i32), ("factor", f32)]
 
 
 class EncodeJob(C.Structure):
@@ -145,6 +152,9 @@ SIGNATURES = {
     "rfsn_page_select": (i32, [vp, vp, i32, i32, i32, i32, vp, vp, sz, vp]),
     "rfsn_paged_attention_workspace_bytes": (sz, [C.POINTER(Paged), i32, i32]),
     "rfsn_paged_attention": (i32, [vp, vp, i32, f32, vp, i32, vp, vp, sz, vp]),
+    "rfsn_paged_evict_workspace_bytes": (sz, [C.POINTER(Paged), i32]),
+    "rfsn_paged_evict": (i32, [vp, i32, i32, i32, vp, vp, sz, vp]),
+    "rfsn_rotary": (i32, [C.POINTER(RotaryParams), vp]),
     "rfsn_kmeans_workspace_bytes": (sz, [i32, i32, i32]),
     "rfsn_kmeans_update": (i32, [vp, i64, i32, i64, vp, i32, i32, vp, vp, sz, vp]),
     "rfsn_host_alloc": (i32, [sz, C.POINTER(vp)]),
@@ -177,7 +187,7 @@ def load(path: Optional[os.PathLike] = None) -> C.CDLL:
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
-    if lib.rfsn_abi_version() != 8:
+    if lib.rfsn_abi_version() != 9:
         raise RuntimeError("librfsn_hip.so ABI version mismatch")
     if path is None:
         _lib = lib

@@ -1,0 +1,172 @@
+// Eviction from a paged KV cache by accumulated attention weight: per sequence and KV head the positions that
+// stay, then their rows to the front of the sequence's own pages, then the pages' bounds.
+#include "choose.h"
+#include "paged.h"
+
+namespace rfsn {
+namespace {
+
+constexpr int kEvictKeys = 8192;
+
+// The positions that (sequence, head) keeps, ascending, and the sequences' new lengths.  A block a (sequence, head).
+__global__ void __launch_bounds__(kChooseWaves * 64)
+evict_choose_kernel(const rfsn_paged p, int shift, int keep, int first, int last, int32_t* __restrict__ kept,
+                    int32_t* __restrict__ new_lens) {
+  constexpr int T = kChooseWaves * 64;
+  __shared__ ChooseRoom<kEvictKeys> room;
+  const int tid = threadIdx.x;
+  const int h = blockIdx.x, b = blockIdx.y;
+  const int len = paged_len(p, shift, b);
+  if (h == 0 && tid == 0) new_lens[b] = min(len, keep);
+  if (len <= keep) return;
+  int32_t* out = kept + ((int64_t)b * p.kv_heads + h) * keep;
+  const int end = len - last;
+  auto weight = [&](int n) {
+    const int page = paged_page(p, b, n >> shift);
+    return page < 0 ? -__builtin_inff() : p.weight[((int64_t)page * p.kv_heads + h) * p.page_size + (n & (p.page_size - 1))];
+  };
+  choose_largest(room, first, end, (uint32_t)(keep - first - last), first, weight, out);
+  for (int i = tid; i < first; i += T) out[i] = i;
+  for (int i = tid; i < last; i += T) out[keep - last + i] = end + i;
+}
+
+// Row kept[j] to row j for j = 0, 1, ..., in place.  kept ascends and kept[j] >= j, so rows that are read later lie
+// behind all that is written now, and a set of rows may be written once all of its reads and those
+// of the sets before it are done: each set is loaded while the one before it waits for the block and is stored.
+// A thread moves `lanes`-th parts of T / lanes rows of a set, U of them.
+template <typename V, int T, int U>
+__device__ __forceinline__ void move_rows(const rfsn_paged& p, int shift, int b, int h, const int32_t* __restrict__ kept, int keep,
+                                          uint8_t* base, int64_t page_bytes, int row_bytes, int lanes) {
+  const int slot = threadIdx.x / lanes, rows = T / lanes, set = rows * U;
+  uint8_t* const at = base + (threadIdx.x % lanes) * sizeof(V);
+  V x[2][U];
+  uint8_t* to[2][U];
+  auto load = [&](int j0, V (&v)[U], uint8_t* (&d)[U]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + u * rows + slot;
+      d[u] = nullptr, v[u] = V{};
+      if (j >= keep || slot >= rows) continue;
+      const int from = kept[j];
+      if (from == j) continue;
+      const int src = paged_page(p, b, from >> shift), dst = paged_page(p, b, j >> shift);
+      if (src >= 0) v[u] = *reinterpret_cast<const V*>(at + src * page_bytes + (int64_t)(from & (p.page_size - 1)) * row_bytes);
+      if (dst >= 0) d[u] = at + dst * page_bytes + (int64_t)(j & (p.page_size - 1)) * row_bytes;
+    }
+  };
+  auto store = [&](const V (&v)[U], uint8_t* const (&d)[U]) {
+    // the loads that this set is of have returned to every wave before any wave writes
+#pragma unroll
+    for (int u = 0; u < U; ++u) asm volatile("" ::"v"(v[u]) : "memory");
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (d[u]) *reinterpret_cast<V*>(d[u]) = v[u];
+  };
+  load(0, x[0], to[0]);
+  for (int j0 = 0; j0 < keep; j0 += 2 * set) {
+    load(j0 + set, x[1], to[1]);
+    store(x[0], to[0]);
+    load(j0 + 2 * set, x[0], to[0]);
+    store(x[1], to[1]);
+  }
+}
+
+// Blocks of a (sequence, head): `parts` slices of K rows, as many of V rows, and one of scales and weights.
+constexpr int kMoveThreads = 256;
+template <int RB, int SB>  // bytes of a row and of its scale
+__global__ void __launch_bounds__(kMoveThreads)
+evict_move_kernel(const rfsn_paged p, int shift, int parts, const int32_t* __restrict__ kept_of, int keep) {
+  const int x = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  if (paged_len(p, shift, b) <= keep) return;
+  const int32_t* kept = kept_of + ((int64_t)b * p.kv_heads + h) * keep;
+  if (x < 2 * parts) {
+    const int width = RB / parts;
+    uint8_t* base = (uint8_t*)(x < parts ? p.k : p.v);
+    const int64_t page_bytes = p.page_stride * RB / p.head_dim, head_bytes = p.head_stride * RB / p.head_dim;
+    move_rows<uint4w, kMoveThreads, 4>(p, shift, b, h, kept, keep, base + h * head_bytes + (x % parts) * width, page_bytes, RB, width / 16);
+    return;
+  }
+  auto words = [&](void* base, int row) {
+    const int64_t head = (int64_t)p.page_size * row;
+    move_rows<uint32_t, kMoveThreads, 4>(p, shift, b, h, kept, keep, (uint8_t*)base + h * head, head * p.kv_heads, row, row / 4);
+  };
+  words(p.weight, 4);
+  if constexpr (SB > 0) {
+    words(p.k_scale, SB);
+    words(p.v_scale, SB);
+  }
+}
+
+// Bounds of the pages that hold the kept rows, from the keys as they are read back.  A wave a (page, head).
+template <int D, int TYPE>
+__global__ void __launch_bounds__(64)
+evict_bounds_kernel(const rfsn_paged p, int shift, int keep) {
+  constexpr int LANES = D / 8, RS = 64 / LANES;
+  const int lane = threadIdx.x, slot = lane / LANES, chunk = lane % LANES;
+  const int o = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  if (paged_len(p, shift, b) <= keep) return;
+  const int page = paged_page(p, b, o);
+  if (page < 0) return;
+  const int rows = min(p.page_size, keep - (o << shift));
+  half8v x = read_page8<D, TYPE>(p, p.k, p.k_scale, page, h, min(slot, rows - 1), chunk);
+  Bounds m = bounds_of(x);
+  for (int r = RS + slot; r - slot < rows; r += RS) m.add(read_page8<D, TYPE>(p, p.k, p.k_scale, page, h, min(r, rows - 1), chunk));
+#pragma unroll
+  for (int w = LANES; w < 64; w <<= 1) m.across(w);
+  half8v* bp = reinterpret_cast<half8v*>((uint16_t*)p.bounds + ((int64_t)page * p.kv_heads + h) * 2 * D + chunk * 8);
+  if (slot == 0) m.store(bp, bp + D / 8);
+}
+
+}  // namespace
+}  // namespace rfsn
+
+using namespace rfsn;
+
+extern "C" size_t rfsn_paged_evict_workspace_bytes(const rfsn_paged* p, int32_t keep) {
+  if (p == nullptr || p->batch <= 0 || p->kv_heads <= 0 || keep <= 0) return 0;
+  return (size_t)p->batch * p->kv_heads * keep * sizeof(int32_t);
+}
+
+extern "C" int rfsn_paged_evict(const rfsn_paged* p, int32_t keep, int32_t first, int32_t last, int32_t* new_lens,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  if (int st = paged_check(p, "paged_evict")) return st;
+  RFSN_REQUIRE(p->weight != nullptr, "paged_evict: the pages hold no weights");
+  RFSN_REQUIRE(keep > 0 && first >= 0 && last >= 0 && (int64_t)first + last <= keep,
+               "paged_evict: keep must be positive and have room for the first and last positions");
+  if (p->batch == 0) return RFSN_OK;
+  RFSN_REQUIRE(new_lens != nullptr, "paged_evict: null output");
+  RFSN_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= rfsn_paged_evict_workspace_bytes(p, keep),
+               "paged_evict: workspace too small or misaligned");
+  const hipStream_t s = (hipStream_t)stream;
+  const int shift = paged_shift(*p), D = p->head_dim;
+  int32_t* kept = (int32_t*)workspace;
+  hipLaunchKernelGGL(evict_choose_kernel, dim3((unsigned)p->kv_heads, (unsigned)p->batch), dim3(kChooseWaves * 64), 0, s, *p,
+                     shift, keep, first, last, kept, new_lens);
+  if (int st = check_launch("paged_evict")) return st;
+  if ((int64_t)p->table_width * p->page_size <= keep) return RFSN_OK;  // nothing can be longer
+#define RFSN_EVICT(RB, SB)                                                                                          \
+  do {                                                                                                              \
+    const int parts = RB > 128 ? RB / 128 : 1;                                                                      \
+    hipLaunchKernelGGL((evict_move_kernel<RB, SB>), dim3(2 * parts + 1, (unsigned)p->kv_heads, (unsigned)p->batch), \
+                       dim3(kMoveThreads), 0, s, *p, shift, parts, kept, keep);                                     \
+  } while (0)
+#define RFSN_EVICT_D(DD)                                    \
+  do {                                                      \
+    if (p->type == RFSN_PAGE_FP16) RFSN_EVICT(2 * DD, 0);   \
+    else if (p->type == RFSN_PAGE_E2M1) RFSN_EVICT(DD / 2, DD / 16); \
+    else RFSN_EVICT(DD, 4);                                 \
+  } while (0)
+  if (D == 64) RFSN_EVICT_D(64);
+  else if (D == 128) RFSN_EVICT_D(128);
+  else RFSN_EVICT_D(256);
+#undef RFSN_EVICT_D
+#undef RFSN_EVICT
+  if (int st = check_launch("paged_evict")) return st;
+  if (p->bounds == nullptr) return RFSN_OK;
+  const dim3 grid((unsigned)ceil_div(keep, p->page_size), (unsigned)p->kv_heads, (unsigned)p->batch);
+  RFSN_PAGED_DISPATCH(D, p->type, {
+    hipLaunchKernelGGL((evict_bounds_kernel<DD, TT>), grid, dim3(64), 0, s, *p, shift, keep);
+  });
+  return check_launch("paged_evict");
+}

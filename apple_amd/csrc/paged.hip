@@ -5,6 +5,7 @@
 // x 32 heads of 128, K and V: fp16 with bounds 537 MB in 101 us, 5.3 TB/s, and 98 us back; int8
 // 403 MB in 97 us and 84 us back); below it by the loads that wait for one another (sequence,
 // page, row): 32 rows of 8 heads 3.5 us.
+#include "choose.h"
 #include "paged.h"
 
 namespace rfsn {
@@ -16,7 +17,8 @@ int paged_check(const rfsn_paged* p, const char* what) {
   RFSN_REQUIRE(p->page_size == 16 || p->page_size == 32 || p->page_size == 64 || p->page_size == 128 ||
                    p->page_size == 256,
                w + ": page_size must be 16, 32, 64, 128 or 256");
-  RFSN_REQUIRE(p->type == RFSN_PAGE_FP16 || p->type == RFSN_PAGE_INT8 || p->type == RFSN_PAGE_E4M3,
+  RFSN_REQUIRE(p->type == RFSN_PAGE_FP16 || p->type == RFSN_PAGE_INT8 || p->type == RFSN_PAGE_E4M3 ||
+                   p->type == RFSN_PAGE_E2M1,
                w + ": unknown page type");
   RFSN_REQUIRE(p->kv_heads > 0 && p->kv_heads <= 65535, w + ": kv_heads out of range");
   RFSN_REQUIRE(p->batch >= 0 && p->batch <= 65535, w + ": batch out of range");
@@ -27,14 +29,16 @@ int paged_check(const rfsn_paged* p, const char* what) {
   RFSN_REQUIRE(p->batch == 0 || p->lens != nullptr, w + ": null lens");
   RFSN_REQUIRE(p->k && p->v && ((uintptr_t)p->k & 15) == 0 && ((uintptr_t)p->v & 15) == 0,
                w + ": k and v must be 16-byte aligned");
-  RFSN_REQUIRE(p->head_stride % 16 == 0 && p->page_stride % 16 == 0 &&
+  const int unit = p->type == RFSN_PAGE_E2M1 ? 32 : 16;
+  RFSN_REQUIRE(p->head_stride % unit == 0 && p->page_stride % unit == 0 &&
                    (p->kv_heads == 1 || p->head_stride >= (int64_t)p->page_size * p->head_dim) && p->page_stride >= 0,
-               w + ": page and head strides must be multiples of 16 that leave room for a head's rows");
+               w + ": page and head strides must be multiples of 16 (4-bit pages: 32) that leave room for a head's rows");
   RFSN_REQUIRE((p->type == RFSN_PAGE_FP16) == (p->k_scale == nullptr) &&
                    (p->type == RFSN_PAGE_FP16) == (p->v_scale == nullptr),
-               w + ": 8-bit pages need both scales, fp16 pages none");
+               w + ": 8-bit and 4-bit pages need both scales, fp16 pages none");
   RFSN_REQUIRE(((uintptr_t)p->bounds & 15) == 0 && ((uintptr_t)p->k_scale & 15) == 0 && ((uintptr_t)p->v_scale & 15) == 0,
                w + ": scales and bounds must be 16-byte aligned");
+  RFSN_REQUIRE(((uintptr_t)p->weight & 15) == 0, w + ": weights must be 16-byte aligned");
   return RFSN_OK;
 }
 
@@ -123,16 +127,13 @@ __device__ __forceinline__ void place_rows(const rfsn_paged& p, int shift, const
   }
 }
 
-typedef unsigned short ushort8v __attribute__((ext_vector_type(8)));
-typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
-typedef unsigned short ushort4v __attribute__((ext_vector_type(4)));
-
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_top(uint32_t x) {
   const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 15, 15, true);
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, x), __builtin_bit_cast(ushort2v, y)));
 }
 // The largest |x| of a K and a V row as bits, K's in the low half: infinity and NaN are the largest.
+// (over LANES lanes: 2 where 16 coordinates share a scale)
 template <int LANES>
 __device__ __forceinline__ uint32_t row_tops(half8v k, half8v v) {
   const ushort8v a = __builtin_bit_cast(ushort8v, k) & (unsigned short)0x7fff;
@@ -142,6 +143,7 @@ __device__ __forceinline__ uint32_t row_tops(half8v k, half8v v) {
   const ushort2v even = {a2[0], b2[0]}, odd = {a2[1], b2[1]};
   uint32_t t = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(even, odd));
   t = dpp_top<0xb1>(t);   // lanes ^ 1, ^ 2, then mirrored halves of 8 and rows of 16
+  if constexpr (LANES == 2) return t;
   t = dpp_top<0x4e>(t);
   t = dpp_top<0x141>(t);
   if constexpr (LANES >= 16) t = dpp_top<0x140>(t);
@@ -182,39 +184,34 @@ __device__ __forceinline__ uint2v quantise(half8v x, uint32_t top, float& scale)
   return c;
 }
 
-// Smallest and largest keys of 8 coordinates, and their largest magnitude's bits, which are past infinity's where one is NaN.
-struct Bounds {
-  half8v lo, hi;
-  ushort8v top;
-  __device__ __forceinline__ void add(half8v x) {
-    lo = __builtin_elementwise_min(lo, x), hi = __builtin_elementwise_max(hi, x);
-    top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort8v, x) & (unsigned short)0x7fff);
+// 8 values of a row as 4-bit codes, by the largest magnitude (as bits) of the 16 coordinates that share
+// the scale.  The scale has 4 significant bits, so x / scale is a midpoint of two codes or at least 2^-11 of
+// itself away from it: a quotient that is right to the last bit or two would do but for the midpoints, and the
+// step after the product with the reciprocal makes those exact.
+__device__ __forceinline__ uint32_t quantise_e2m1(half8v x, uint32_t top, uint32_t& byte) {
+  if (top >= 0x7c00u) {  // not finite
+    byte = 255;
+    return 0;
   }
-  // what a page holds already
-  __device__ __forceinline__ void add(half8v l, half8v h) { add(l), add(h); }
-  __device__ __forceinline__ void across(int o) {  // with the lanes o apart
-    const uint4w l = __builtin_bit_cast(uint4w, lo), h = __builtin_bit_cast(uint4w, hi), t = __builtin_bit_cast(uint4w, top);
-    uint4w l2, h2, t2;
+  const float s = h2f((uint16_t)top) / 6.f;
+  // to 3 mantissa bits: of fp32's from fp16's normal range on, to 2^-17 below it
+  const uint32_t u = __builtin_bit_cast(uint32_t, s);
+  float r = __builtin_bit_cast(float, (u + 0x7ffffu + ((u >> 20) & 1)) & 0xfff00000u);
+  if (s < 0x1p-14f) r = rintf(s * 0x1p17f) * 0x1p-17f;
+  r = fminf(r, 10240.f);
+  byte = (uint32_t)(f2h(r) >> 7);
+  if (r == 0.f) return 0;
+  const float inv = 1.f / r;
+  float y[8];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      l2[w] = (uint32_t)__shfl_xor((int)l[w], o, 64);
-      h2[w] = (uint32_t)__shfl_xor((int)h[w], o, 64);
-      t2[w] = (uint32_t)__shfl_xor((int)t[w], o, 64);
-    }
-    lo = __builtin_elementwise_min(lo, __builtin_bit_cast(half8v, l2));
-    hi = __builtin_elementwise_max(hi, __builtin_bit_cast(half8v, h2));
-    top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort8v, t2));
+  for (int e = 0; e < 8; ++e) {
+    const float v = (float)x[e], z = v * inv;
+    y[e] = __builtin_copysignf(fmaf(fmaf(-z, r, v), inv, z), v);  // (-0 as well)
   }
-  __device__ __forceinline__ void store(half8v* l, half8v* h) const {
-    ushort8v a = __builtin_bit_cast(ushort8v, lo), b = __builtin_bit_cast(ushort8v, hi);
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (top[e] > 0x7c00) a[e] = b[e] = 0x7e00;
-    *l = __builtin_bit_cast(half8v, a), *h = __builtin_bit_cast(half8v, b);
-  }
-};
-__device__ __forceinline__ Bounds bounds_of(half8v x) {
-  return {x, x, __builtin_bit_cast(ushort8v, x) & (unsigned short)0x7fff};
+  uint32_t c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, y[0], y[1], 1.f, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[2], y[3], 1.f, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[4], y[5], 1.f, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[6], y[7], 1.f, 3);
 }
 
 // Block number of a grid of x by y blocks so that each XCD takes a contiguous range of
@@ -270,20 +267,33 @@ paged_append_kernel(const rfsn_paged p, int shift, const uint16_t* __restrict__ 
   for (int i = 0; i < I; ++i) {
     const bool write = at[i].page >= 0;
     const int64_t off = (int64_t)(write ? at[i].page : 0) * p.page_stride + h * p.head_stride + (int64_t)at[i].row * D + chunk * 8;
+    const int64_t sc = ((int64_t)(write ? at[i].page : 0) * p.kv_heads + h) * p.page_size + at[i].row;
+    if (p.weight != nullptr && write && chunk == 0) p.weight[sc] = 0.f;
     if constexpr (TYPE == RFSN_PAGE_FP16) {
       if (write) {
         store_page<(I > 1)>(kx[i], (half8v*)((uint16_t*)p.k + off));
         store_page<(I > 1)>(vx[i], (half8v*)((uint16_t*)p.v + off));
       }
+    } else if constexpr (TYPE == RFSN_PAGE_E2M1) {
+      const uint32_t tops = row_tops<2>(kx[i], vx[i]);
+      uint32_t ks, vs;
+      const uint32_t kc = quantise_e2m1(kx[i], tops & 0xffffu, ks), vc = quantise_e2m1(vx[i], tops >> 16, vs);
+      if (write) {
+        store_page<(I > 1)>(kc, (uint32_t*)((uint8_t*)p.k + off / 2));
+        store_page<(I > 1)>(vc, (uint32_t*)((uint8_t*)p.v + off / 2));
+        if (chunk % 2 == 0) {
+          ((uint8_t*)p.k_scale)[sc * (D / 16) + chunk / 2] = (uint8_t)ks;
+          ((uint8_t*)p.v_scale)[sc * (D / 16) + chunk / 2] = (uint8_t)vs;
+        }
+      }
     } else {
-      const int64_t sc = ((int64_t)(write ? at[i].page : 0) * p.kv_heads + h) * p.page_size + at[i].row;
       const uint32_t tops = row_tops<LANES>(kx[i], vx[i]);
       float ks, vs;
       const uint2v kc = quantise<TYPE>(kx[i], tops & 0xffffu, ks), vc = quantise<TYPE>(vx[i], tops >> 16, vs);
       if (write) {
         store_page<(I > 1)>(kc, (uint2v*)((uint8_t*)p.k + off));
         store_page<(I > 1)>(vc, (uint2v*)((uint8_t*)p.v + off));
-        if (chunk == 0) p.k_scale[sc] = ks, p.v_scale[sc] = vs;
+        if (chunk == 0) ((float*)p.k_scale)[sc] = ks, ((float*)p.v_scale)[sc] = vs;
       }
     }
   }
@@ -352,17 +362,8 @@ paged_read_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ cu,
   if (n >= rows || (at.rest && !zero_rest)) return;
   half8v ko = {}, vo = {};
   if (at.page >= 0) {
-    const int64_t off = (int64_t)at.page * p.page_stride + h * p.head_stride + (int64_t)at.row * D + chunk * 8;
-    if constexpr (TYPE == RFSN_PAGE_FP16) {
-      ko = *reinterpret_cast<const half8v*>((const uint16_t*)p.k + off);
-      vo = *reinterpret_cast<const half8v*>((const uint16_t*)p.v + off);
-    } else {
-      const int64_t sc = ((int64_t)at.page * p.kv_heads + h) * p.page_size + at.row;
-      const float ks = p.k_scale[sc], vs = p.v_scale[sc];
-      const float8v kf = load_page8<TYPE>(p.k, off), vf = load_page8<TYPE>(p.v, off);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ko[e] = (f16)(kf[e] * ks), vo[e] = (f16)(vf[e] * vs);
-    }
+    ko = read_page8<D, TYPE>(p, p.k, p.k_scale, at.page, h, at.row, chunk);
+    vo = read_page8<D, TYPE>(p, p.v, p.v_scale, at.page, h, at.row, chunk);
   }
   const int64_t o = (n * p.kv_heads + h) * D + chunk * 8;
   *reinterpret_cast<half8v*>(out_k + o) = ko;
@@ -482,29 +483,13 @@ page_score_kernel(const rfsn_paged p, int shift, const uint16_t* __restrict__ q,
   }
 }
 
-// Order of the scores as unsigned keys: NaN as +infinity, -0 as +0.
-__device__ __forceinline__ uint32_t page_key(float s) {
-  if (s != s) s = __builtin_inff();
-  const uint32_t u = __builtin_bit_cast(uint32_t, s + 0.f);
-  return u >> 31 ? ~u : u | 0x80000000u;
-}
-
-// The pages of a row's largest keys besides the kept ones, all in ascending order.  A block a row.
-// The smallest key to keep is found by narrowing [lo, hi], at first the smallest and largest key: a histogram of
-// 2,048 equal parts of it says which part holds the key wanted.  Scores share their exponent mostly, so parts
-// of their range spread over the counters where their leading bits would meet in one; two rounds are the rule,
-// three the most (leading bits as counters: 50 us for 128 of 2,048 pages, 256 rows; so 6.3, latency of
-// some ten block barriers).  Then each of 16 waves counts what it keeps of its own run of pages and writes it
-// behind the waves before it.  Keys past the LDS copy are read again from the scores.
-constexpr int kChooseWaves = 16, kChooseBins = 2048, kChooseKeys = 8192;
+// The pages of a row's largest scores besides the kept ones, all in ascending order.  A block a row.
 __global__ void __launch_bounds__(kChooseWaves * 64)
 page_choose_kernel(const rfsn_paged p, int shift, const float* __restrict__ score, int count, int first, int last,
                    int32_t* __restrict__ chosen) {
-  constexpr int T = kChooseWaves * 64, PER = kChooseBins / T;
-  __shared__ uint32_t s_key[kChooseKeys];
-  __shared__ uint32_t hist[kChooseBins];
-  __shared__ uint32_t s_wave[2][kChooseWaves], s_found[3];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int T = kChooseWaves * 64;
+  __shared__ ChooseRoom<8192> room;
+  const int tid = threadIdx.x;
   const int h = blockIdx.x, b = blockIdx.y;
   const int64_t row = (int64_t)b * p.kv_heads + h;
   const float* s = score + row * p.table_width;
@@ -516,100 +501,10 @@ page_choose_kernel(const rfsn_paged p, int shift, const float* __restrict__ scor
   }
   // held > count >= first + last: the kept pages are apart, the others lie between them
   const int begin = first, end = held - last;
-  uint32_t left = (uint32_t)(count - first - last);
-  auto key = [&](int n) { return n - begin < kChooseKeys ? s_key[n - begin] : page_key(s[n]); };
-  uint32_t lo = 0xffffffffu, hi = 0;
-#pragma unroll 4
-  for (int n = begin + tid; n < end; n += T) {
-    const uint32_t k = page_key(s[n]);
-    if (n - begin < kChooseKeys) s_key[n - begin] = k;
-    lo = min(lo, k), hi = max(hi, k);
-  }
-  lo = ~wave_most(~lo), hi = wave_most(hi);
-  if (lane == 0) s_wave[0][wave] = lo, s_wave[1][wave] = hi;
-  __syncthreads();
-  lo = ~wave_most(lane < kChooseWaves ? ~s_wave[0][lane] : 0u), hi = wave_most(lane < kChooseWaves ? s_wave[1][lane] : 0u);
-  // what the waves before this one have of s_wave[i]
-  auto before_wave = [&](int i) { return wave_total(lane < wave ? s_wave[i][lane] : 0u); };
-  uint32_t over = 0xffffffffu, tie = 0xffffffffu;  // keys from `over` on are kept, and `left` of those equal to `tie`
-  while (left > 0) {
-    if (lo == hi) {
-      over = lo + 1, tie = lo;
-      break;
-    }
-    const int bits = 32 - __builtin_clz(hi - lo), sh = bits > 11 ? bits - 11 : 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) hist[tid + i * T] = 0;
-    __syncthreads();
-    for (int n = begin + tid; n < end; n += T) {
-      const uint32_t k = key(n);
-      if (k >= lo && k <= hi) atomicAdd(&hist[(k - lo) >> sh], 1u);
-    }
-    __syncthreads();
-    // keys in the parts above each thread's PER parts, from the top down
-    uint32_t c[PER], mine = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) mine += c[i] = hist[kChooseBins - 1 - (tid * PER + i)];
-    const uint32_t upto = wave_upto(mine);
-    if (lane == 63) s_wave[0][wave] = upto;
-    __syncthreads();
-    uint32_t above = upto - mine + before_wave(0);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      if (above < left && above + c[i] >= left) {
-        s_found[0] = (uint32_t)(kChooseBins - 1 - (tid * PER + i));
-        s_found[1] = left - above;
-        s_found[2] = c[i];
-      }
-      above += c[i];
-    }
-    __syncthreads();
-    lo += s_found[0] << sh;
-    hi = min(hi, lo + ((1u << sh) - 1u));
-    left = s_found[1];
-    if (s_found[2] == left) {  // the whole part
-      over = lo, left = 0;
-    }
-  }
-  __syncthreads();  // s_wave is written again
-  const int seg = ((end - begin + kChooseWaves - 1) / kChooseWaves + 63) / 64 * 64;
-  const int n0 = begin + wave * seg, n1 = min(end, n0 + seg);
-  uint32_t kept = 0, ties = 0;
-  for (int n = n0 + lane; n - lane < n1; n += 64) {
-    const uint32_t k = n < n1 ? key(n) : 0;
-    kept += (uint32_t)__popcll(__ballot(n < n1 && k >= over));
-    ties += (uint32_t)__popcll(__ballot(n < n1 && left && k == tie));
-  }
-  if (lane == 0) s_wave[0][wave] = kept, s_wave[1][wave] = ties;
-  __syncthreads();
-  uint32_t before = before_wave(1), at = (uint32_t)first + before_wave(0);
-  at += min(before, left);
-  const uint64_t below = (1ull << lane) - 1;
-  for (int n = n0 + lane; n - lane < n1; n += 64) {
-    const uint32_t k = n < n1 ? key(n) : 0;
-    const bool is_tie = n < n1 && left && k == tie;
-    const uint64_t bt = __ballot(is_tie);
-    const bool keep = (n < n1 && k >= over) || (is_tie && before + (uint32_t)__popcll(bt & below) < left);
-    const uint64_t bk = __ballot(keep);
-    if (keep) out[at + (uint32_t)__popcll(bk & below)] = n;
-    at += (uint32_t)__popcll(bk), before += (uint32_t)__popcll(bt);
-  }
+  choose_largest(room, begin, end, (uint32_t)(count - first - last), first, [&](int n) { return s[n]; }, out);
   for (int i = tid; i < first; i += T) out[i] = i;
   for (int i = tid; i < last; i += T) out[count - last + i] = end + i;
 }
-
-#define RFSN_PAGED_DISPATCH(D, TYPE, ...)                                                       \
-  do {                                                                                          \
-    if (D == 64 && TYPE == RFSN_PAGE_FP16) { constexpr int DD = 64, TT = RFSN_PAGE_FP16; __VA_ARGS__ }        \
-    else if (D == 64 && TYPE == RFSN_PAGE_INT8) { constexpr int DD = 64, TT = RFSN_PAGE_INT8; __VA_ARGS__ }   \
-    else if (D == 64) { constexpr int DD = 64, TT = RFSN_PAGE_E4M3; __VA_ARGS__ }                             \
-    else if (D == 128 && TYPE == RFSN_PAGE_FP16) { constexpr int DD = 128, TT = RFSN_PAGE_FP16; __VA_ARGS__ } \
-    else if (D == 128 && TYPE == RFSN_PAGE_INT8) { constexpr int DD = 128, TT = RFSN_PAGE_INT8; __VA_ARGS__ } \
-    else if (D == 128) { constexpr int DD = 128, TT = RFSN_PAGE_E4M3; __VA_ARGS__ }                           \
-    else if (TYPE == RFSN_PAGE_FP16) { constexpr int DD = 256, TT = RFSN_PAGE_FP16; __VA_ARGS__ }             \
-    else if (TYPE == RFSN_PAGE_INT8) { constexpr int DD = 256, TT = RFSN_PAGE_INT8; __VA_ARGS__ }             \
-    else { constexpr int DD = 256, TT = RFSN_PAGE_E4M3; __VA_ARGS__ }                                         \
-  } while (0)
 
 }  // namespace
 }  // namespace rfsn

@@ -69,7 +69,8 @@ inline Plan plan(const rfsn_paged& p, int q_heads, int count) {
   if (pages > p.pages) pages = p.pages;
   if (p.held_pages > 0 && pages > p.held_pages) pages = p.held_pages;
   r.once = !r.wide && count == 0 &&
-           pages * p.page_size * p.kv_heads * p.head_dim * (p.type == RFSN_PAGE_FP16 ? 4 : 2) >= kLastLevelCache;
+           pages * p.page_size * p.kv_heads * p.head_dim *
+                   (p.type == RFSN_PAGE_FP16 ? 4.0 : p.type == RFSN_PAGE_E2M1 ? 1.125 : 2.0) >= kLastLevelCache;
   const int per_step = waves_of(p.head_dim, r.wide) * 32;
   const int64_t least = r.wide ? per_step : 4 * per_step;  // positions of a chunk
   int64_t longest = kLongestChunk;

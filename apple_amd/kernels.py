@@ -708,13 +708,15 @@ def fused_attention(q: torch.Tensor, fmt: WarmFormat, *, kv_heads: int, scale: f
 # --------------------------------------------------------------------------
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
-PAGE_TYPES = {torch.float16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
+PAGE_TYPES = {torch.float16: 0, torch.int8: 1, torch.float8_e4m3fn: 2, torch.uint8: 4}
 
 
 class KVPages(NamedTuple):
     """A pool of pages (``rfsn_paged``): k, v [P, Hkv, S, D] fp16, int8 or
-    float8_e4m3fn, of one stride each, rows dense; with 8-bit codes the rows'
-    scales [P, Hkv, S] fp32; bounds [P, Hkv, 2, D] fp16, each page's smallest and
+    float8_e4m3fn, or [P, Hkv, S, D / 2] uint8 with two e2m1 codes each, of one
+    stride each, rows dense; with 8-bit codes the rows'
+    scales [P, Hkv, S] fp32, with 4-bit ones [P, Hkv, S, D / 16] uint8, a scale
+    per row and 16 coordinates; bounds [P, Hkv, 2, D] fp16, each page's smallest and
     largest key per coordinate, where pages are to be selected by them."""
 
     k: torch.Tensor
@@ -724,13 +726,13 @@ class KVPages(NamedTuple):
     bounds: Optional[torch.Tensor] = None
 
 
-_PAGED_BLOCK = struct.Struct("7P3q8i")  # rfsn_paged, packed: a call's fields as they are, without a ctypes object
+_PAGED_BLOCK = struct.Struct("7P3q8iP")  # rfsn_paged, packed: a call's fields as they are, without a ctypes object
 
 
 def _paged(what: str, pages: KVPages, table: torch.Tensor, lens: torch.Tensor,
-           held: int = 0) -> Tuple[bytes, tuple, int]:
-    """The checked parameter block of a pool, a block table [B, W] int32 and
-    lengths [B] int32: (block, (B, Hkv, D, S, W), device index)."""
+           held: int = 0, weight: Optional[torch.Tensor] = None) -> Tuple[bytes, tuple, int]:
+    """The checked parameter block of a pool, a block table [B, W] int32,
+    lengths [B] int32 and accumulated weights [P, Hkv, S] fp32 (or None): (block, (B, Hkv, D, S, W), device index)."""
     k, v, ks, vs, bounds = pages
     dev = k.get_device()
     if dev < 0:
@@ -743,16 +745,21 @@ def _paged(what: str, pages: KVPages, table: torch.Tensor, lens: torch.Tensor,
     (P, H, S, D), (sp, sh, ss, sd) = shape, strides
     kind = PAGE_TYPES.get(dtype)
     if kind is None:
-        raise ValueError(f"{what}: pages of {dtype}; float16, int8 and float8_e4m3fn are served")
+        raise ValueError(f"{what}: pages of {dtype}; float16, int8, float8_e4m3fn and uint8 (e2m1) are served")
     if sd != 1 or ss != D:
         raise ValueError(f"{what}: a head's rows must be dense")
+    rows = (P, H, S)
+    if kind == 4:
+        D, sp, sh, rows, scale_type = 2 * D, 2 * sp, 2 * sh, (P, H, S, D // 8), torch.uint8
+    else:
+        scale_type = torch.float32
     apart = v.get_device() != dev or table.get_device() != dev or lens.get_device() != dev
     if kind:
         if ks is None or vs is None:
-            raise ValueError(f"{what}: 8-bit pages need k_scale and v_scale")
+            raise ValueError(f"{what}: 8-bit and 4-bit pages need k_scale and v_scale")
         for t in (ks, vs):
-            if t.shape != (P, H, S) or t.dtype is not torch.float32 or not t.is_contiguous():
-                raise ValueError(f"{what}: scales must be contiguous fp32 {[P, H, S]}")
+            if t.shape != rows or t.dtype is not scale_type or not t.is_contiguous():
+                raise ValueError(f"{what}: scales must be contiguous {scale_type} {list(rows)}")
             apart = apart or t.get_device() != dev
         ks, vs = ks.data_ptr(), vs.data_ptr()
     elif ks is not None or vs is not None:
@@ -762,6 +769,11 @@ def _paged(what: str, pages: KVPages, table: torch.Tensor, lens: torch.Tensor,
             raise ValueError(f"{what}: bounds must be contiguous fp16 {[P, H, 2, D]}")
         apart = apart or bounds.get_device() != dev
         bounds = bounds.data_ptr()
+    if weight is not None:
+        if weight.shape != (P, H, S) or weight.dtype is not torch.float32 or not weight.is_contiguous():
+            raise ValueError(f"{what}: weights must be contiguous fp32 {[P, H, S]}")
+        apart = apart or weight.get_device() != dev
+        weight = weight.data_ptr()
     shape = table.shape
     if len(shape) != 2 or table.dtype is not torch.int32:
         raise ValueError(f"{what}: the block table must be int32 [batch, pages per sequence]")
@@ -775,7 +787,7 @@ def _paged(what: str, pages: KVPages, table: torch.Tensor, lens: torch.Tensor,
     if max(P, H, S, D, B, W) >= 1 << 31:
         raise ValueError(f"{what}: sizes must stay below 2^31")
     return (_PAGED_BLOCK.pack(k.data_ptr(), v.data_ptr(), ks or 0, vs or 0, bounds or 0, table.data_ptr(),
-                              lens.data_ptr(), sp, sh, st, P, S, H, D, kind, B, W, held), (B, H, D, S, W), dev)
+                              lens.data_ptr(), sp, sh, st, P, S, H, D, kind, B, W, held, weight or 0), (B, H, D, S, W), dev)
 
 
 def _page_count(what: str, count: int, page_size: int) -> int:
@@ -815,20 +827,23 @@ def _paged_query(what: str, q: torch.Tensor, batch: int, head_dim: int, device: 
 
 
 @functools.lru_cache(maxsize=1024)
-def _paged_workspace(name: str, batch: int, kv_heads: int, head_dim: int, page_size: int, width: int, *more: int) -> int:
-    """A call's workspace, which its sizes alone determine."""
+def _paged_workspace(name: str, batch: int, kv_heads: int, head_dim: int, page_size: int, width: int, *more: int,
+                     weigh: bool = False) -> int:
+    """A call's workspace, which its sizes (and whether it accumulates weights) alone determine."""
     p = L.Paged(kv_heads=kv_heads, head_dim=head_dim, page_size=page_size, batch=batch, table_width=width)
+    p.weight = 16 if weigh else None  # asked for, never followed
     return getattr(L.load(), name)(C.byref(p), *more)
 
 
 def paged_append(pages: KVPages, table: torch.Tensor, lens: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
-                 cu: Optional[torch.Tensor] = None) -> None:
+                 cu: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None) -> None:
     """New rows k, v [N, Hkv, D] fp16 into the pages, quantised where they hold
     codes, with the pages' bounds: rows cu[b] .. cu[b + 1] - 1 (``cu`` [B + 1]
     int32; None: row b) follow the ``lens[b]`` tokens of sequence b.  Rows
     behind cu[B] are ignored, as is what the table has no page for; ``lens`` is
-    not changed.  No two sequences of a call may append to one page."""
-    block, (B, H, D, _, _), dev = _paged("paged_append", pages, table, lens)
+    not changed.  No two sequences of a call may append to one page.
+    ``weight`` [P, Hkv, S] fp32: accumulated weights, those of the new rows set to 0."""
+    block, (B, H, D, _, _), dev = _paged("paged_append", pages, table, lens, 0, weight)
     shape = k.shape
     if len(shape) != 3 or shape[1] != H or shape[2] != D or v.shape != shape or k.dtype is not torch.float16 \
             or v.dtype is not torch.float16 or k.get_device() != dev or v.get_device() != dev:
@@ -900,17 +915,23 @@ def page_select(q: torch.Tensor, pages: KVPages, table: torch.Tensor, lens: torc
 
 
 def paged_attention(q: torch.Tensor, pages: KVPages, table: torch.Tensor, lens: torch.Tensor, scale: float,
-                    chosen: Optional[torch.Tensor] = None, held_pages: int = 0) -> torch.Tensor:
+                    chosen: Optional[torch.Tensor] = None, held_pages: int = 0,
+                    weight: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Exact attention of one query per sequence, q [B, Hq, D] fp16, over the
     sequence's first ``lens[b]`` positions, or over those of its pages that
     ``chosen`` [B, Hkv, n] (``page_select``) lists; zeros where there are none.
-    Codes are attended as code * scale in fp32, not rounded to fp16.
+    Codes are attended as code * scale in fp32, not rounded to fp16 (in which those of 4 bits are exact).
+    ``weight`` [P, Hkv, S] fp32 (without ``chosen``): each position's softmax
+    weight, summed over the KV head's query heads, is added to its row's; no two
+    sequences may hold one page then.
     ``held_pages``: the pages that the sequences hold together, where the caller
     knows it; without it a call counts as reading what its table has room for,
     which costs up to a tenth where that is far more."""
     if not 0 <= held_pages < 1 << 31:
         raise ValueError("paged_attention: held_pages must be a number of pages")
-    block, sizes, dev = _paged("paged_attention", pages, table, lens, held_pages)
+    if weight is not None and chosen is not None:
+        raise ValueError("paged_attention: weights are of whole sequences, not of chosen pages")
+    block, sizes, dev = _paged("paged_attention", pages, table, lens, held_pages, weight)
     B, H, D, S, _ = sizes
     q = _paged_query("paged_attention", q, B, D, dev)
     count, listed = 0, None
@@ -925,11 +946,116 @@ def paged_attention(q: torch.Tensor, pages: KVPages, table: torch.Tensor, lens: 
     if chosen is not None and count == 0:
         return out.zero_()
     Hq = q.shape[1]
-    wsb = _paged_workspace("rfsn_paged_attention_workspace_bytes", *sizes, Hq, count)
+    wsb = _paged_workspace("rfsn_paged_attention_workspace_bytes", *sizes, Hq, count, weigh=weight is not None)
     ws = lens.new_empty(wsb // 4) if wsb else None
     _paged_call(dev, "rfsn_paged_attention", block, q.data_ptr(), Hq, float(scale), listed, count, out.data_ptr(),
                 None if ws is None else ws.data_ptr(), wsb)
     return out
+
+
+def paged_evict(pages: KVPages, table: torch.Tensor, lens: torch.Tensor, weight: torch.Tensor, keep: int, *,
+                first: int = 4, last: int = 64) -> torch.Tensor:
+    """Sequences of more than ``keep`` positions give up the others, each KV
+    head its own: kept are the ``first`` oldest and ``last`` newest and those of the largest
+    ``weight`` [P, Hkv, S] (``paged_attention``; ties go to the older).  Their
+    rows, scales and weights move, in their order, to the sequence's positions 0
+    .. keep - 1; bounds follow, rows behind stay as they are (``rfsn_paged_evict``).  Returns
+    the new lengths [B] int32; ``table`` and ``lens`` are not changed.  No two sequences of
+    a call may hold one page."""
+    block, sizes, dev = _paged("paged_evict", pages, table, lens, 0, weight)
+    if weight is None:
+        raise ValueError("paged_evict: weights are needed")
+    keep, first, last = int(keep), int(first), int(last)
+    if keep <= 0 or first < 0 or last < 0 or first + last > keep:
+        raise ValueError("paged_evict: keep must be positive and have room for the first and last positions")
+    new_lens = torch.empty_like(lens)
+    if sizes[0] == 0:
+        return new_lens
+    if keep >= sizes[3] * sizes[4]:  # no sequence is longer: a list of what the table holds will do
+        keep, first, last = max(1, sizes[3] * sizes[4]), 0, 0
+    wsb = _paged_workspace("rfsn_paged_evict_workspace_bytes", *sizes, keep)
+    ws = lens.new_empty(wsb // 4)
+    _paged_call(dev, "rfsn_paged_evict", block, keep, first, last, new_lens.data_ptr(), ws.data_ptr() or None, wsb)
+    return new_lens
+
+
+# --------------------------------------------------------------------------
+# rotary positions (llama32_adapter.py:555-568)
+# --------------------------------------------------------------------------
+
+ROTARY_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
+
+
+def _apart(x: torch.Tensor) -> bool:
+    """Whether no two elements of x [N, H, D] (D dense) share memory, as far as its strides say."""
+    dims = sorted((s, n) for s, n in zip(x.stride()[:2], x.shape[:2]) if n > 1)
+    reach = x.shape[2]
+    for s, n in dims:
+        if s < reach:
+            return False
+        reach += s * (n - 1)
+    return True
+
+
+def _clear_of(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether a and b [N, H, D] share no memory: apart as a whole, or parts of the same rows (a projection's output)."""
+    size = a.element_size()
+    span = lambda x: (x.data_ptr(), x.data_ptr() + (sum(s * (n - 1) for s, n in zip(x.stride(), x.shape)) + 1) * size)
+    (a0, a1), (b0, b1) = span(a), span(b)
+    if a1 <= b0 or b1 <= a0:
+        return True
+    step = a.stride(0) * size
+    if a.stride(0) != b.stride(0) or a.shape[0] != b.shape[0]:
+        return False
+    row = lambda x: ((x.shape[1] - 1) * x.stride(1) + x.shape[2]) * size
+    if a0 > b0:
+        a, b, a0, b0 = b, a, b0, a0
+    return a0 + row(a) <= b0 and b0 + row(b) <= a0 + step
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor, *,
+           layout: str = "half", factor: float = 1.0, inplace: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Rotary positions of q [N, Hq, D] and k [N, Hkv, D] (or None), fp16, bf16
+    or fp32: the first R = 2 * len(inv_freq) coordinates of every head are turned in pairs
+    (i, i + R / 2) (``layout`` "half") or (2 i, 2 i + 1) ("interleaved") by
+    positions[n] * inv_freq[i] and scaled by ``factor`` (``rfsn_rotary``); the
+    others are copied.  ``positions`` [N] int32 or int64, ``inv_freq`` float64
+    (``layer.rope_inv_freq``).  New contiguous tensors, or with ``inplace`` q and k themselves."""
+    _dev(q, "rotary")
+    kind = ROTARY_TYPES.get(q.dtype)
+    if q.dim() != 3 or kind is None:
+        raise ValueError("rotary: q must be [rows, heads, head_dim] of float16, bfloat16 or float32")
+    N, Hq, D = q.shape
+    if k is not None and (k.dim() != 3 or k.shape[0] != N or k.shape[2] != D or k.dtype is not q.dtype or k.device != q.device):
+        raise ValueError(f"rotary: k must be [{N}, heads, {D}] of q's type and device")
+    if layout not in ROTARY_LAYOUTS:
+        raise ValueError(f"rotary: layout must be one of {tuple(ROTARY_LAYOUTS)}")
+    if positions.shape != (N,) or positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device:
+        raise ValueError(f"rotary: positions must be int32 or int64 [{N}] on q's device")
+    if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float64 or inv_freq.device != q.device \
+            or not 2 <= 2 * inv_freq.shape[0] <= D:
+        raise ValueError(f"rotary: inv_freq must be float64 of 1 to {D // 2} frequencies on q's device")
+    xs = [q] if k is None else [q, k]
+    if any(t.requires_grad for t in xs) and torch.is_grad_enabled():
+        raise RuntimeError("rotary has no gradients: call it under torch.no_grad()")
+    if inplace:
+        if any(t.stride(2) != 1 or not _apart(t) for t in xs) or k is not None and N and Hq and k.shape[1] and not _clear_of(q, k):
+            raise ValueError("rotary: in place, the coordinates must be dense and no two elements share memory")
+        outs = xs
+    else:
+        xs = [t if t.stride(2) == 1 else t.contiguous() for t in xs]
+        outs = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in xs]
+    positions, inv_freq = _contig(positions), _contig(inv_freq)
+    p = L.RotaryParams()
+    for i, (x, o) in enumerate(zip(xs, outs)):
+        p.x[i], p.out[i], p.heads[i] = x.data_ptr(), o.data_ptr(), x.shape[1]
+        p.row_stride[i], p.head_stride[i], p.out_row_stride[i], p.out_head_stride[i] = *x.stride()[:2], *o.stride()[:2]
+    p.positions, p.inv_freq, p.rows = positions.data_ptr(), inv_freq.data_ptr(), N
+    p.head_dim, p.rotary_dim, p.layout, p.type = D, 2 * inv_freq.shape[0], ROTARY_LAYOUTS[layout], kind
+    p.wide_positions, p.factor = int(positions.dtype is torch.int64), float(factor)
+    _paged_call(q.get_device(), "rfsn_rotary", C.byref(p))
+    return outs[0], None if k is None else outs[1]
 
 
 # --------------------------------------------------------------------------

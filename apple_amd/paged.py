@@ -6,11 +6,16 @@ The reference keeps one cache per sequence (cache.py:33-57), and
 pages of ``page_size`` tokens from a pool as it grows and returns them when it
 ends, so that what is held is what the sequences have, whatever their lengths.
 
-* ``append`` / ``prefill`` write new rows (fp16, or int8 / e4m3 codes with a
-  scale per row) and each page's key bounds in one launch;
+* ``append`` / ``prefill`` write new rows (fp16, int8 / e4m3 codes with a
+  scale per row, or e2m1 codes of 4 bits with a scale per 16 coordinates) and
+  each page's key bounds in one launch;
+* ``rotary`` turns a step's queries and keys to the positions that ``append``
+  will give them;
 * ``attention_forward`` attends the newest token of every sequence over all of
   its positions, or over the pages whose bounds promise the largest scores;
 * ``prompt_attention`` attends a chunk of one sequence's prompt;
+* ``evict`` gives up the positions that have had the least attention weight
+  (``weights=True``: ``attention_forward`` adds it up);
 * ``sequence_window`` reads one sequence back.
 
 Rows of K/V heads are as in the other caches: ``num_kv_heads`` heads are stored
@@ -28,16 +33,17 @@ from . import kernels as K
 from .attention import _blockwise_exact_attention
 from .storage import RFSNConfig
 
-PAGE_DTYPES = {"fp16": torch.float16, "int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+PAGE_DTYPES = {"fp16": torch.float16, "int8": torch.int8, "e4m3": torch.float8_e4m3fn, "e2m1": torch.uint8}
 
 
 class RFSNPagedKVCache:
     """``pages`` pages of ``page_size`` tokens for up to ``batch`` sequences of up to ``max_tokens`` tokens (default:
-    the whole pool).  ``page_type``: "fp16", "int8" or "e4m3".  ``bounds``: keep what page selection needs (4 bytes
-    per page, KV head and coordinate)."""
+    the whole pool).  ``page_type``: "fp16", "int8", "e4m3" or "e2m1" (4.5 bits a value).  ``bounds``: keep what page
+    selection needs (4 bytes per page, KV head and coordinate).  ``weights``: add up each row's attention weight, which
+    ``evict`` goes by (4 bytes per row and KV head)."""
 
     def __init__(self, config: RFSNConfig, batch: int, pages: int, page_size: int = 64, page_type: str = "fp16",
-                 max_tokens: Optional[int] = None, bounds: bool = True, device=None):
+                 max_tokens: Optional[int] = None, bounds: bool = True, device=None, weights: bool = False):
         if batch <= 0 or pages <= 0:
             raise ValueError("batch and pages must be positive")
         if page_size not in K.PAGE_SIZES:
@@ -59,7 +65,12 @@ class RFSNPagedKVCache:
         self.max_tokens = width * page_size if max_tokens is None else min(max_tokens, width * page_size)
         shape, dtype = (pages, self.H, page_size, self.D), PAGE_DTYPES[page_type]
         new = lambda s, d: torch.zeros(s, dtype=d, device=self.device)
-        scales = (None, None) if page_type == "fp16" else (new(shape[:3], torch.float32), new(shape[:3], torch.float32))
+        if page_type == "e2m1":  # two codes a byte, a scale byte per 16 coordinates
+            shape = (*shape[:3], self.D // 2)
+            scales = tuple(new((*shape[:3], self.D // 16), torch.uint8) for _ in range(2))
+        else:
+            scales = (None, None) if page_type == "fp16" else (new(shape[:3], torch.float32), new(shape[:3], torch.float32))
+        self.weight = new(shape[:3], torch.float32) if weights else None
         self.pages = K.KVPages(new(shape, dtype), new(shape, dtype), *scales,
                                new((pages, self.H, 2, self.D), torch.float16) if bounds else None)
         self.table = torch.full((batch, width), -1, dtype=torch.int32, device=self.device)
@@ -68,6 +79,8 @@ class RFSNPagedKVCache:
         self._held: List[List[int]] = [[] for _ in range(batch)]
         self._free = list(range(pages - 1, -1, -1))
         self._ended = set()  # released, and without tokens since
+        self._given_up = new((batch,), torch.int32)  # tokens that the sequences hold no longer
+        self._gaps: List[int] = [0] * batch          # rows at the front of each that may not be neighbours' any more
 
     @property
     def free_pages(self) -> int:
@@ -118,15 +131,16 @@ class RFSNPagedKVCache:
             raise ValueError(f"sequences {sorted(self._ended)} were released: append takes counts until they hold "
                              "tokens again")
         self._reserve(each)
+        kept = {} if self.weight is None else {"weight": self.weight}
         if counts is None:
-            K.paged_append(self.pages, self.table, self.lens, k, v)
+            K.paged_append(self.pages, self.table, self.lens, k, v, **kept)
             self.lens.add_(1)
         else:
             cu = [0]
             for c in each:
                 cu.append(cu[-1] + c)
             on = torch.tensor([cu, each + [0]], dtype=torch.int32).to(self.device)
-            K.paged_append(self.pages, self.table, self.lens, k, v, on[0])
+            K.paged_append(self.pages, self.table, self.lens, k, v, on[0], **kept)
             self.lens.add_(on[1, :-1])
         self.num_tokens = [n + c for n, c in zip(self.num_tokens, each)]
         if self._ended:
@@ -147,7 +161,52 @@ class RFSNPagedKVCache:
         self.num_tokens[b] = 0
         self.table[b].fill_(-1)
         self.lens[b:b + 1].zero_()
+        self._given_up[b:b + 1].zero_()
+        self._gaps[b] = 0
         self._ended.add(b)
+
+    def positions(self, counts: Optional[Sequence[int]] = None) -> torch.Tensor:
+        """Positions [N] int32 of the tokens that the next ``append`` of these
+        counts writes: those after all that the sequences were ever given, evicted ones
+        included."""
+        begin = self.lens + self._given_up
+        if counts is None:
+            return begin
+        each = [int(c) for c in counts]
+        if len(each) != self.batch or min(each) < 0:
+            raise ValueError(f"counts must be {self.batch} numbers of tokens")
+        on = torch.tensor([[b, i] for b, c in enumerate(each) for i in range(c)], dtype=torch.int32)
+        b, i = on.reshape(-1, 2).t().to(self.device)
+        return begin[b.long()] + i
+
+    def rotary(self, q: torch.Tensor, k: torch.Tensor, inv_freq: torch.Tensor, counts: Optional[Sequence[int]] = None, *,
+               layout: str = "half", factor: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+        """q [N, Hq, D] and k [N, Hkv, D] of the tokens that ``append(k, v, counts)``
+        is to write, at their positions (``kernels.rotary``)."""
+        pos = self.positions(counts)
+        return K.rotary(q.to(self.device), k.to(self.device), pos, inv_freq, layout=layout, factor=factor)
+
+    def evict(self, keep: int, first: int = 4, last: int = 64) -> None:
+        """Sequences of more than ``keep`` tokens give up the others, each KV
+        head its own: kept are the ``first`` oldest, the ``last`` newest and those with the most attention
+        weight (``kernels.paged_evict``).  Pages that are not needed any more return to the pool."""
+        if self.weight is None:
+            raise ValueError("evict goes by attention weights: the cache keeps none (weights=True)")
+        if keep <= 0 or first < 0 or last < 0 or first + last > keep:
+            raise ValueError("keep must be positive and have room for the first and last tokens")
+        long = [b for b, n in enumerate(self.num_tokens) if n > keep]
+        if not long:
+            return
+        new = K.paged_evict(self.pages, self._live_table(), self.lens, self.weight, keep, first=first, last=last)
+        self._given_up.add_(self.lens - new)
+        self.lens.copy_(new)
+        need = -(-keep // self.page_size)
+        for b in long:
+            self._free.extend(reversed(self._held[b][need:]))
+            del self._held[b][need:]
+            whole = min(last, self.num_tokens[b] - self._gaps[b])  # newest tokens without a gap
+            self.num_tokens[b], self._gaps[b] = keep, keep - whole
+        self.table[torch.tensor(long, device=self.device), need:] = -1
 
     def _live_table(self) -> torch.Tensor:
         """The table's columns that some sequence uses."""
@@ -158,7 +217,8 @@ class RFSNPagedKVCache:
         positions -> [B, Hq, D] in q's dtype; an empty sequence gives zeros.
         ``sparse_pages``: over that many of its pages per KV head, the first, the
         newest and those whose bounds promise the largest scores (of keys before
-        their rounding to 8 bits)."""
+        their rounding to 8 or 4 bits).  A cache with ``weights`` adds up those of whole
+        sequences, not of ``sparse_pages``."""
         if q.dim() != 3 or q.shape[0] != self.batch or q.shape[2] != self.D:
             raise ValueError(f"q must be [{self.batch}, heads, {self.D}]")
         qh = q.to(device=self.device, dtype=torch.float16)
@@ -169,16 +229,21 @@ class RFSNPagedKVCache:
                 raise ValueError("sparse_pages must have room for the first and the newest page")
             chosen = K.page_select(qh, self.pages, table, self.lens, sparse_pages)
         held = self.pages.k.shape[0] - len(self._free)
-        return K.paged_attention(qh, self.pages, table, self.lens, self.scale, chosen, held).to(q.dtype)
+        kept = {} if self.weight is None or chosen is not None else {"weight": self.weight}
+        return K.paged_attention(qh, self.pages, table, self.lens, self.scale, chosen, held, **kept).to(q.dtype)
 
     def prompt_attention(self, b: int, q: torch.Tensor) -> torch.Tensor:
         """q [S, Hq, D], the newest S tokens of sequence b, each over the
         positions up to its own -> [S, Hq, D] in q's dtype.  Rows of 8-bit pages
         are read back as fp16 first at head sizes 64 and 128, while
-        ``attention_forward`` takes code * scale as it is."""
+        ``attention_forward`` takes code * scale as it is.  Weights are not added up.
+        After an ``evict`` the S newest tokens have to be among those that are held
+        without a gap: its ``last`` and those appended since."""
         n = self.num_tokens[self._index(b)]
         if q.dim() != 3 or q.shape[2] != self.D or q.shape[0] > n:
             raise ValueError(f"q must be [S, heads, {self.D}] of at most the {n} tokens held")
+        if q.shape[0] > n - self._gaps[b]:
+            raise ValueError(f"the newest {n - self._gaps[b]} tokens are held without a gap, not {q.shape[0]}")
         if q.shape[0] == 0:
             return torch.zeros_like(q)
         if self.D == 256:  # the blockwise entry serves 64 and 128: each query as a sequence of its own over the same pages
@@ -193,7 +258,7 @@ class RFSNPagedKVCache:
                                           causal=True, query_positions=torch.arange(n - q.shape[0], n))
 
     def sequence_window(self, b: int) -> Tuple[torch.Tensor, torch.Tensor]:
-        """K and V [T, Hkv, D] fp16 of sequence b."""
+        """K and V [T, Hkv, D] fp16 of sequence b (after an ``evict``: of what each KV head has kept, in order)."""
         n = self.num_tokens[self._index(b)]
         at = torch.tensor([0, 0, n], dtype=torch.int32).to(self.device)
         return K.paged_read(self.pages, self.table[b:b + 1], at[:1], at[1:], n)
@@ -203,5 +268,6 @@ class RFSNPagedKVCache:
         size = lambda t: 0 if t is None else t.numel() * t.element_size()
         pool = sum(size(t) for t in self.pages)
         total = self.pages.k.shape[0]
-        return {"pool": pool, "in_use": pool // total * (total - len(self._free)),
-                "table": size(self.table) + size(self.lens)}
+        use = {"pool": pool, "in_use": pool // total * (total - len(self._free)),
+               "table": size(self.table) + size(self.lens)}
+        return use if self.weight is None else use | {"weights": size(self.weight)}

@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define RFSN_ABI_VERSION 8
+#define RFSN_ABI_VERSION 9
 
 #define RFSN_OK 0
 #define RFSN_ERR_INVALID (-1)     /* shape / contract violation -> ValueError   */
@@ -579,7 +579,14 @@ int rfsn_ref_table_stats(const rfsn_ref_params* p, float* stats_dev, void* strea
  * reference, which keeps one cache per sequence, cache.py:33-57).  Position t
  * of sequence b is row t % page_size of page table[b][t / page_size].
  * K/V rows are fp16, or 8-bit codes with one fp32 scale per row (value =
- * code * scale): int8 (scale = amax / 127) or OCP e4m3 (amax / 448).  bounds
+ * code * scale): int8 (scale = amax / 127) or OCP e4m3 (amax / 448), or 4-bit
+ * OCP e2m1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives; two a byte, the
+ * earlier coordinate in the low half) with one 8-bit scale per row and 16
+ * coordinates, the fp16 number whose bits are byte << 7 (5 exponent and 3
+ * mantissa bits): scale = min(amax / 6 rounded to such a number, 10240), code =
+ * x / scale rounded to nearest, ties to the even code; a group with a value that
+ * is not finite has scale byte 255 (NaN) and codes 0.  code * scale is exact in
+ * fp16.  bounds
  * holds, per page and KV head, the smallest and the largest key of each
  * coordinate, as fp16 of the rows before they are quantised; a NaN key makes
  * both NaN.
@@ -589,15 +596,17 @@ int rfsn_ref_table_stats(const rfsn_ref_params* p, float* stats_dev, void* strea
  *  - lens below 0 count as 0, lens past table_width * page_size as that.
  *  - Device values are never trusted for addressing: every page, row and
  *    sequence index is checked by the kernels.
- *  - k, v, bounds 16-byte aligned, strides multiples of 16 elements. */
+ *  - k, v, bounds 16-byte aligned, strides multiples of 16 elements (32 with
+ *    4-bit pages, whose elements are coordinates too). */
 #define RFSN_PAGE_FP16 0
 #define RFSN_PAGE_INT8 1
 #define RFSN_PAGE_E4M3 2
+#define RFSN_PAGE_E2M1 4
 typedef struct rfsn_paged {
   void* k;              /* [pages][kv_heads][page_size][head_dim]; page_stride and     */
   void* v;              /*   head_stride elements between pages and heads, rows dense  */
-  float* k_scale;       /* [pages][kv_heads][page_size], NULL with fp16 pages          */
-  float* v_scale;
+  void* k_scale;        /* fp32 [pages][kv_heads][page_size], NULL with fp16 pages;    */
+  void* v_scale;        /*   4-bit pages: bytes [pages][kv_heads][page_size][head_dim / 16] */
   void* bounds;         /* fp16 [pages][kv_heads][2][head_dim], or NULL                */
   const int32_t* table; /* [batch][table_width], table_stride entries between rows     */
   const int32_t* lens;  /* [batch] tokens of each sequence (append, read: the first position) */
@@ -613,6 +622,9 @@ typedef struct rfsn_paged {
   int32_t table_width;
   int32_t held_pages;   /* pages that the sequences hold together, where the caller knows it, else 0: a hint of
                          * rfsn_paged_attention's traffic, on which its speed alone depends */
+  float* weight;        /* [pages][kv_heads][page_size] accumulated attention weight of each row, or NULL:
+                         * rfsn_paged_append sets a new row's to 0, rfsn_paged_attention adds to it,
+                         * rfsn_paged_evict goes by it; the other calls do not look at it */
 } rfsn_paged;
 
 /* Rows k, v [rows][kv_heads][head_dim] fp16 (token_stride, head_stride
@@ -656,10 +668,63 @@ int rfsn_page_select(const rfsn_paged* p, const void* q, int32_t q_heads, int32_
  * smallest value is 0, which makes an infinite value NaN.  Products with finite values take them to
  * 2^-16 of themselves or, from fp16 pages, to 2^-22 of themselves or 2^-33 of the largest, whichever is more: at
  * most 2^-13 of the largest |v| at any length (unless the tables have room for over 2^37 positions).
- * The workspace size depends on q_heads and, with chosen, count (0: dense). */
+ * With p->weight each position's softmax weight, summed over the query heads of
+ * the KV head, is added to its row's (nothing to attend: nothing is added; a head
+ * whose weights are NaN adds NaN to all of the sequence's positions); chosen has to be NULL
+ * then, and no two sequences of the call may hold one page.
+ * The workspace size depends on q_heads, whether there are weights and, with chosen, count (0: dense). */
 size_t rfsn_paged_attention_workspace_bytes(const rfsn_paged* p, int32_t q_heads, int32_t count);
 int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t q_heads, float scale, const int32_t* chosen,
                          int32_t count, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Sequences that hold more than `keep` positions give up the others, each KV
+ * head its own: kept are the `first` oldest and `last` newest positions and
+ * those of the largest p->weight (NaN counts as infinite, ties go to the older
+ * position; a position without a page as of the smallest), `keep` in all.  Their
+ * rows, with scales and weights, move to positions 0 .. keep - 1 of the sequence in
+ * their order; the rows behind stay as they are, as does the table.  A position without a
+ * page moves as a row of zeros.  Bounds of all of the sequence's pages up to position keep - 1
+ * become those of the keys that lie there then, as rfsn_paged_read gives them.
+ * Sequences with at most `keep` positions stay as they are.  new_lens
+ * [batch]: min(lens, keep).  No two sequences of the call, nor two entries of a sequence's
+ * table, may name one page. */
+size_t rfsn_paged_evict_workspace_bytes(const rfsn_paged* p, int32_t keep);
+int rfsn_paged_evict(const rfsn_paged* p, int32_t keep, int32_t first, int32_t last, int32_t* new_lens,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- rotary positions
+ * The rotary embedding of llama32_adapter.py:555-568 for rows at positions of their
+ * own, in either layout, of all or the first rotary_dim coordinates of each
+ * head: a pair (x1, x2) becomes factor (x1 cos a - x2 sin a, x2 cos a + x1 sin a),
+ * a = position * inv_freq[i].  Pair i is (i, i + rotary_dim / 2) with
+ * RFSN_ROTARY_HALF and (2 i, 2 i + 1) with RFSN_ROTARY_INTERLEAVED.
+ * The other coordinates are copied.  a and its turns are held in 64 bits, sine, cosine and
+ * products in 32; one rounding at the end.  An output may be its input (same address and strides);
+ * outputs overlap nothing else.  Coordinates are dense, strides count elements. */
+#define RFSN_ROTARY_HALF 0
+#define RFSN_ROTARY_INTERLEAVED 1
+#define RFSN_ROTARY_FP16 0
+#define RFSN_ROTARY_BF16 1
+#define RFSN_ROTARY_FP32 2
+typedef struct rfsn_rotary_params {
+  const void* x[2];        /* [rows][heads[i]][head_dim]: queries, keys (heads 0: none) */
+  void* out[2];
+  int64_t row_stride[2];
+  int64_t head_stride[2];
+  int64_t out_row_stride[2];
+  int64_t out_head_stride[2];
+  const void* positions;   /* [rows] int32, or int64 with wide_positions */
+  const double* inv_freq;  /* [rotary_dim / 2] */
+  int64_t rows;
+  int32_t heads[2];
+  int32_t head_dim;        /* 2 .. 1024 */
+  int32_t rotary_dim;      /* even, 2 .. head_dim */
+  int32_t layout;          /* RFSN_ROTARY_HALF, RFSN_ROTARY_INTERLEAVED */
+  int32_t type;            /* RFSN_ROTARY_FP16, _BF16, _FP32 */
+  int32_t wide_positions;
+  float factor;
+} rfsn_rotary_params;
+int rfsn_rotary(const rfsn_rotary_params* p, void* stream);
 
 /* ---------------------------------------------------------------- k-means
  * One Lloyd update of PQ codebooks (rfsn_v10_mlx_ane_complete.py:197-207):
