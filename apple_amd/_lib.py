@@ -154,7 +154,7 @@ SIGNATURES = {
     "rfsn_paged_attention": (i32, [vp, vp, i32, f32, vp, i32, vp, vp, sz, vp]),
     "rfsn_paged_evict_workspace_bytes": (sz, [C.POINTER(Paged), i32]),
     "rfsn_paged_evict": (i32, [vp, i32, i32, i32, vp, vp, sz, vp]),
-    "rfsn_rotary": (i32, [C.POINTER(RotaryParams), vp]),
+    "rfsn_rotary": (i32, [vp, vp]),
     "rfsn_kmeans_workspace_bytes": (sz, [i32, i32, i32]),
     "rfsn_kmeans_update": (i32, [vp, i64, i32, i64, vp, i32, i32, vp, vp, sz, vp]),
     "rfsn_host_alloc": (i32, [sz, C.POINTER(vp)]),

@@ -985,6 +985,7 @@ def paged_evict(pages: KVPages, table: torch.Tensor, lens: torch.Tensor, weight:
 
 ROTARY_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}
+_ROTARY_BLOCK = struct.Struct("4P8q2Pq7if")  # rfsn_rotary_params, packed
 
 
 def _apart(x: torch.Tensor) -> bool:
@@ -1022,40 +1023,50 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     positions[n] * inv_freq[i] and scaled by ``factor`` (``rfsn_rotary``); the
     others are copied.  ``positions`` [N] int32 or int64, ``inv_freq`` float64
     (``layer.rope_inv_freq``).  New contiguous tensors, or with ``inplace`` q and k themselves."""
-    _dev(q, "rotary")
-    kind = ROTARY_TYPES.get(q.dtype)
-    if q.dim() != 3 or kind is None:
+    dev = q.get_device()
+    if dev < 0:
+        L.require_device(q, "rotary")
+    dtype, shape = q.dtype, q.shape
+    kind = ROTARY_TYPES.get(dtype)
+    if len(shape) != 3 or kind is None:
         raise ValueError("rotary: q must be [rows, heads, head_dim] of float16, bfloat16 or float32")
-    N, Hq, D = q.shape
-    if k is not None and (k.dim() != 3 or k.shape[0] != N or k.shape[2] != D or k.dtype is not q.dtype or k.device != q.device):
-        raise ValueError(f"rotary: k must be [{N}, heads, {D}] of q's type and device")
+    N, Hq, D = shape
     if layout not in ROTARY_LAYOUTS:
         raise ValueError(f"rotary: layout must be one of {tuple(ROTARY_LAYOUTS)}")
-    if positions.shape != (N,) or positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device:
+    if positions.shape != (N,) or positions.dtype not in (torch.int32, torch.int64) or positions.get_device() != dev:
         raise ValueError(f"rotary: positions must be int32 or int64 [{N}] on q's device")
-    if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float64 or inv_freq.device != q.device \
+    if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float64 or inv_freq.get_device() != dev \
             or not 2 <= 2 * inv_freq.shape[0] <= D:
         raise ValueError(f"rotary: inv_freq must be float64 of 1 to {D // 2} frequencies on q's device")
-    xs = [q] if k is None else [q, k]
-    if any(t.requires_grad for t in xs) and torch.is_grad_enabled():
+    watched = q.requires_grad
+    (qs, qh, qc), Hk, (ks, kh, kc) = q.stride(), 0, (0, 0, 1)
+    if k is not None:
+        if k.dim() != 3 or k.shape[0] != N or k.shape[2] != D or k.dtype is not dtype or k.get_device() != dev:
+            raise ValueError(f"rotary: k must be [{N}, heads, {D}] of q's type and device")
+        watched = watched or k.requires_grad
+        Hk, (ks, kh, kc) = k.shape[1], k.stride()
+    if watched and torch.is_grad_enabled():
         raise RuntimeError("rotary has no gradients: call it under torch.no_grad()")
     if inplace:
-        if any(t.stride(2) != 1 or not _apart(t) for t in xs) or k is not None and N and Hq and k.shape[1] and not _clear_of(q, k):
+        if qc != 1 or kc != 1 or not _apart(q) or k is not None and (not _apart(k) or N and Hq and Hk and not _clear_of(q, k)):
             raise ValueError("rotary: in place, the coordinates must be dense and no two elements share memory")
-        outs = xs
+        qo, ko, qos, qoh, kos, koh = q, k, qs, qh, ks, kh
     else:
-        xs = [t if t.stride(2) == 1 else t.contiguous() for t in xs]
-        outs = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in xs]
+        qo = q.new_empty(shape)
+        ko = None if k is None else q.new_empty(k.shape)
+        qos, qoh, kos, koh = Hq * D, D, Hk * D, D
+        if qc != 1:
+            q = q.contiguous()
+            qs, qh = qos, qoh
+        if kc != 1:
+            k = k.contiguous()
+            ks, kh = kos, koh
     positions, inv_freq = _contig(positions), _contig(inv_freq)
-    p = L.RotaryParams()
-    for i, (x, o) in enumerate(zip(xs, outs)):
-        p.x[i], p.out[i], p.heads[i] = x.data_ptr(), o.data_ptr(), x.shape[1]
-        p.row_stride[i], p.head_stride[i], p.out_row_stride[i], p.out_head_stride[i] = *x.stride()[:2], *o.stride()[:2]
-    p.positions, p.inv_freq, p.rows = positions.data_ptr(), inv_freq.data_ptr(), N
-    p.head_dim, p.rotary_dim, p.layout, p.type = D, 2 * inv_freq.shape[0], ROTARY_LAYOUTS[layout], kind
-    p.wide_positions, p.factor = int(positions.dtype is torch.int64), float(factor)
-    _paged_call(q.get_device(), "rfsn_rotary", C.byref(p))
-    return outs[0], None if k is None else outs[1]
+    _paged_call(dev, "rfsn_rotary", _ROTARY_BLOCK.pack(
+        q.data_ptr(), 0 if k is None else k.data_ptr(), qo.data_ptr(), 0 if k is None else ko.data_ptr(), qs, ks, qh, kh,
+        qos, kos, qoh, koh, positions.data_ptr(), inv_freq.data_ptr(), N, Hq, Hk, D, 2 * inv_freq.shape[0],
+        ROTARY_LAYOUTS[layout], kind, int(positions.dtype is torch.int64), float(factor)))
+    return qo, ko
 
 
 # --------------------------------------------------------------------------

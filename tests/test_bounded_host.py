@@ -33,6 +33,22 @@ def test_rotary_block_layout(tmp_path):
         assert int(got[f]) == getattr(_lib.RotaryParams, f).offset, f
 
 
+def test_packed_rotary_block_is_the_parameter_block():
+    from apple_amd import _lib
+    from apple_amd.kernels import _ROTARY_BLOCK
+
+    p, flat = _lib.RotaryParams(), []
+    for n, (name, t) in enumerate(_lib.RotaryParams._fields_):
+        if hasattr(t, "_length_"):
+            values = [(100 * n + i) for i in range(2)]
+            setattr(p, name, t(*values))
+            flat += values
+        else:
+            setattr(p, name, n + 1)
+            flat.append(n + 1)
+    assert _ROTARY_BLOCK.pack(*flat) == bytes(p)
+
+
 def test_four_bit_pools_are_refused_before_a_launch(lib):
     for bad, says in ((dict(k_scale=0), "scales"), (dict(v_scale=0), "scales"), (dict(head_stride=16 * 64 + 16), "strides"),
                       (dict(page_stride=8 * 16 * 64 + 16), "strides"), (dict(weight=4100), "weights must be")):
