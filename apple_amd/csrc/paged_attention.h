@@ -75,7 +75,7 @@ __device__ __forceinline__ Chunk find_chunk(const rfsn_paged& p, int shift, cons
   float least = 0.f;
 #pragma unroll
   for (int x = 0; x < kTries; ++x) {
-    if (x > 0 && p.batch == 1) break;  // of one sequence the chunks are alike: the fewest
+    if (x > 0 && p.batch == 1 && cut.alike) break;  // of one sequence the chunks are alike: the fewest
     const float each = total * cut.one_over[x] + 0.98f;  // rounded up, but for an excess that is fp32's
     uint32_t s = each < 2147483520.f ? (uint32_t)each : 2147483520u;
     s = s <= (uint32_t)cut.chunk ? (uint32_t)cut.chunk : (s + 127) & ~127u;
@@ -86,8 +86,8 @@ __device__ __forceinline__ Chunk find_chunk(const rfsn_paged& p, int shift, cons
       n += m, most = max(most, about(len, m));
     }
     if (p.batch > 1) n = wave_total(n), most = wave_most(most);
-    // positions on the fullest CU, each chunk costing as much as 128 more
-    const float cost = (float)((n * (uint32_t)cut.units + kCUs - 1) / kCUs) * ((float)most + 128.f);
+    // positions on the fullest CU, each chunk costing as much as some more
+    const float cost = (float)((n * (uint32_t)cut.units + kCUs - 1) / kCUs) * ((float)most + cut.start) * cut.each[x];
     if (x == 0 || cost < least) least = cost, size = s;
   }
   size = __builtin_amdgcn_readfirstlane(size);
@@ -288,6 +288,15 @@ __device__ __forceinline__ uint4w codes_bf16(uint32_t a, uint32_t b) {
   return r;
 }
 
+// x - y[I], exact where y[I] is x rounded: one operation that takes y as fp16.
+template <int I>
+__device__ __forceinline__ float less(float x, half2w y) {
+  float r;
+  if constexpr (I == 0) asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(y), "v"(x));
+  else asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(y), "v"(x));
+  return r;
+}
+
 // 16 or 8 bytes of a row, marked as not to be kept where the call reads more than the caches hold (Plan).
 template <bool kOnce, typename V>
 __device__ __forceinline__ V load_piece(const uint8_t* a) {
@@ -361,6 +370,11 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
       qf[s] = *reinterpret_cast<const half8v*>(qr + (kCodes   ? (s >> 1) * 64 + grp * 16 + (s & 1) * 8
                                                      : kSmall ? s / (LB / 4) * (LB * 8) + grp * (LB * 2) + s % (LB / 4) * 8
                                                               : s * 32 + grp * 8));
+    // 4 bits: columns without a head stay 0, weights too (m_run below), which spares the matrix cores' power: 32 x 32,768
+    // positions, 8 KV heads of 64, again and again 160 us, so 146
+    if (kSmall && col >= heads)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) qf[s] = half8v{};
   }
   const int len = __builtin_amdgcn_readfirstlane(paged_len(p, shift, b));
   if (cut.per_seq) {
@@ -384,15 +398,23 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
   float4v o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = float4v{0.f, 0.f, 0.f, 0.f};
-  float m_run = -__builtin_inff(), l_run = 0.f;  // reference exponent of the head's weights, this lane's sum of them
+  float m_run = kSmall && col >= heads ? 0x1p100f : -__builtin_inff(), l_run = 0.f;  // reference exponent of the head's weights, this lane's sum of them
 
   typedef std::conditional_t<LB == 16, uint4w, uint2v> piece;
   piece kr[NG][KL], vr[NG][VU];
   float4v ks[NG], vs[NG];
   uint32_t kb8[NG][KL], vb8[NG][VU];  // scale bytes of 4-bit codes
   int n_next[NG] = {};  // rows of the fetched groups that are attended
+  const int64_t page_bytes = p.page_stride * RB / D, head_bytes = p.head_stride * RB / D;
+  const uint8_t* const k0 = (const uint8_t*)p.k + h * head_bytes;
+  const uint8_t* const v0 = (const uint8_t*)p.v + h * head_bytes;
+  constexpr int kScale = kSmall ? D / 16 : 4;  // bytes of a row's scales
+  const int64_t scale_page = (int64_t)p.kv_heads * p.page_size * kScale;
+  const uint8_t* const ks0 = (const uint8_t*)p.k_scale + (int64_t)h * p.page_size * kScale;
+  const uint8_t* const vs0 = (const uint8_t*)p.v_scale + (int64_t)h * p.page_size * kScale;
   // Rows past the last one attended re-read it: their weights are 0.  A group with none
-  // reads page 0, and its V is not used.
+  // reads page 0, and its V is not used.  Of 4-bit pages all 16 rows are read, which are the
+  // page's own, and the scales of those that are not attended taken as 0.
   auto fetch = [&](int t, int tile) {
 #pragma unroll
     for (int u = 0; u < NG; ++u) {
@@ -401,36 +423,34 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
       const int row = (t + 16 * u) & (p.page_size - 1);
       n_next[u] = n;
       const int last = n > 0 ? n - 1 : 0;
-      const int64_t base = ((int64_t)page * p.page_stride + (int64_t)h * p.head_stride + (int64_t)row * D) * RB / D;
-      const uint8_t* kb = (const uint8_t*)p.k + base;
-      const uint8_t* vb = (const uint8_t*)p.v + base;
-      const uint32_t kl = (uint32_t)(min(col, last) * RB + grp * LB);
+      const int64_t base = page * page_bytes + row * RB;
+      const uint8_t* kb = k0 + base;
+      const uint8_t* vb = v0 + base;
+      const uint32_t kl = (uint32_t)((kSmall ? col : min(col, last)) * RB + grp * LB);
 #pragma unroll
       for (int i = 0; i < KL; ++i) kr[u][i] = load_piece<kOnce, piece>(kb + kl + i * (4 * LB));
 #pragma unroll
       for (int i = 0; i < VU; ++i) {
         const int idx = i * 64 + lane, r = idx / VC, ch = idx % VC;
-        vr[u][i] = load_piece<kOnce, piece>(vb + (uint32_t)(min(r, last) * RB + ch * LB));
+        vr[u][i] = load_piece<kOnce, piece>(vb + (uint32_t)((kSmall ? r : min(r, last)) * RB + ch * LB));
       }
       if constexpr (kSmall) {
-        const int64_t sc = (((int64_t)page * p.kv_heads + h) * p.page_size + row) * (D / 16);
-        const uint8_t* ksb = (const uint8_t*)p.k_scale + sc;
-        const uint8_t* vsb = (const uint8_t*)p.v_scale + sc;
+        const int64_t sc = page * scale_page + row * kScale;
 #pragma unroll
-        for (int i = 0; i < KL; ++i) kb8[u][i] = load_scales<SB>(ksb + (uint32_t)(min(col, last) * (D / 16) + (i * 4 + grp) * SB));
+        for (int i = 0; i < KL; ++i) kb8[u][i] = load_scales<SB>(ks0 + sc + (uint32_t)(col * kScale + (i * 4 + grp) * SB));
 #pragma unroll
-        for (int i = 0; i < VU; ++i) {
-          const int idx = i * 64 + lane;
-          vb8[u][i] = load_scales<SB>(vsb + (uint32_t)(min(idx / VC, last) * (D / 16) + idx % VC * SB));
-        }
+        for (int i = 0; i < VU; ++i) vb8[u][i] = load_scales<SB>(vs0 + sc + (uint32_t)((i * 64 + lane) * SB));
       }
       if constexpr (kCodes) {
-        const int64_t sc = ((int64_t)page * p.kv_heads + h) * p.page_size + row;
-        ks[u] = *reinterpret_cast<const float4v*>((const float*)p.k_scale + sc + (uint32_t)(grp * 4));
-        vs[u] = *reinterpret_cast<const float4v*>((const float*)p.v_scale + sc + (uint32_t)(grp * 4));
+        const int64_t sc = page * scale_page + row * kScale;
+        ks[u] = *reinterpret_cast<const float4v*>(ks0 + sc + (uint32_t)(grp * 16));
+        vs[u] = *reinterpret_cast<const float4v*>(vs0 + sc + (uint32_t)(grp * 16));
       }
     }
   };
+  // 4 bits: a positive scale is left to the subtraction of the maximum (another would turn a masked score's infinity)
+  const bool late = kSmall && scale_log2 > 0.f;
+  const float factor = late ? scale_log2 : 1.f;
   uint4w* const sv = smem + wave * kTile * CH;
   int t = t0 + wave * kTile, tile = 0;
   if (t < t1) fetch(t, 0);
@@ -445,9 +465,10 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
       for (int i = 0; i < VU; ++i) {
         const int idx = i * 64 + lane, r = u * 16 + idx / VC, ch = idx % VC;
         piece x = vr[u][i];
-        if (n[u] == 0) x = piece{};
+        if (!kSmall && n[u] == 0) x = piece{};
         if constexpr (kSmall) {
-          const uint32_t sb = n[u] == 0 ? 0 : vb8[u][i];
+          uint32_t sb = vb8[u][i];
+          if (n[u] < 16 && idx / VC >= n[u]) sb = 0;  // (codes are finite)
 #pragma unroll
           for (int c = 0; c < LB / 4; ++c)
             sv[r * CH + ((ch * (LB / 4) + c) ^ v_swz<D>(r))] =
@@ -480,7 +501,7 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
         s[u] *= ks[u];
         vscale[u] = vs[u];
       }
-      s[u] *= scale_log2;
+      if (!late) s[u] *= scale_log2;
       if (n[u] < 16) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -495,7 +516,8 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
 #pragma unroll
       for (int u = 0; u < NG; ++u)
         if (n[u] > 0 && col < heads)
-          *reinterpret_cast<float4v*>(parts.score + (row0 + col) * parts.positions + t + 16 * u + grp * 4) = s[u];
+          *reinterpret_cast<float4v*>(parts.score + (row0 + col) * parts.positions + t + 16 * u + grp * 4) =
+              kSmall ? s[u] * factor : s[u];
     }
     ++tile;
     if (t + step < t1) {
@@ -512,7 +534,7 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
       ls = 0.f;
 #pragma unroll
       for (int i = 0; i < 4 * NG; ++i) {
-        pw[i] = __builtin_amdgcn_exp2f(s[i >> 2][i & 3] - mb);
+        pw[i] = __builtin_amdgcn_exp2f(kSmall ? fmaf(s[i >> 2][i & 3], factor, -mb) : s[i >> 2][i & 3] - mb);
         ls += pw[i];
       }
     };
@@ -525,6 +547,7 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
       for (int i = 1; i < 4 * NG; ++i) mx = fmaxf(mx, s[i >> 2][i & 3]);
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      if constexpr (kSmall) mx *= factor;
       const float m_new = fmaxf(m_run, mx - kPBias);
       const float corr = m_run > -__builtin_inff() ? __builtin_amdgcn_exp2f(m_run - m_new) : 0.f;
       l_run *= corr;
@@ -539,7 +562,7 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
     for (int i = 0; i < 2 * NG; ++i) {
       if constexpr (!kCodes) {
         const half2w hi = {(f16)pw[2 * i], (f16)pw[2 * i + 1]};
-        const half2w lo = {(f16)(pw[2 * i] - (float)hi[0]), (f16)(pw[2 * i + 1] - (float)hi[1])};
+        const half2w lo = {(f16)less<0>(pw[2 * i], hi), (f16)less<1>(pw[2 * i + 1], hi)};
         bh[i] = __builtin_bit_cast(uint32_t, hi), bl[i] = __builtin_bit_cast(uint32_t, lo);
       } else {
         const float a = pw[2 * i] * vscale[i >> 1][(2 * i) & 3], b = pw[2 * i + 1] * vscale[i >> 1][(2 * i + 1) & 3];

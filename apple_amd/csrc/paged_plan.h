@@ -19,6 +19,9 @@ struct Cut {
   int64_t chunk;
   int64_t longest;          // positions that a chunk has at most
   float one_over[kTries];   // 1 / chunks aimed at, for so many blocks per CU
+  float start;              // positions that a chunk costs besides its own
+  float each[kTries];       // what a position costs with so many blocks per CU
+  bool alike;               // the same with any of them
 };
 // Chunks aimed at with k blocks on each CU: each sequence adds half of one on average, and a batch
 // that fills the chip by itself is cut where a sequence is longer than the mean.
@@ -76,17 +79,25 @@ inline Plan plan(const rfsn_paged& p, int q_heads, int count) {
   int64_t longest = kLongestChunk;
   while (longest < most && div_up(most, longest) * p.batch > 32768) longest *= 2;  // the grid ends at 65,535 chunks
   if (most <= (r.wide ? most_steps : 4) * per_step) {
-    r.slots = p.batch, r.cut = {1, units, most > 0 ? most : 1, longest, {}};
+    r.slots = p.batch, r.cut = {1, units, most > 0 ? most : 1, longest, {}, 0.f, {}, true};
   } else if (count) {
     int64_t n = div_up(r.wide ? kCUs : 4 * kCUs, (int64_t)units * p.batch);
     if (n > div_up(most, least)) n = div_up(most, least);
     if (n < div_up(most, longest)) n = div_up(most, longest);
     const int64_t chunk = div_up(div_up(most, n), per_step) * per_step;
     n = div_up(most, chunk);
-    r.slots = n * p.batch, r.cut = {(int)n, units, chunk, longest, {}};
+    r.slots = n * p.batch, r.cut = {(int)n, units, chunk, longest, {}, 0.f, {}, true};
   } else {
     const int first = r.wide ? 1 : 2;
-    r.cut = {0, units, least, longest, {}};
+    r.cut = {0, units, least, longest, {}, 128.f, {1.f, 1.f, 1.f}, true};
+    if (!r.wide && p.type == RFSN_PAGE_E2M1) {
+      // 4-bit rows are decoded by the vector units, which more waves keep busier: 32 x 32,768 positions, 8 KV heads of 64,
+      // take 173, 160 and 149 us as 2, 3 and 4 blocks per CU, 16 x 8,192 of 128 33.8, 32.5 and 35, of 256 82, 87 and 92.  A
+      // chunk's start weighs more beside them (131,072 positions of 4 heads of 64: 20.5, 22.4 and 24.4).
+      const float each[3][kTries] = {{1.f, 0.93f, 0.86f}, {1.f, 0.95f, 1.05f}, {1.f, 1.1f, 1.15f}};
+      r.cut.start = 300.f, r.cut.alike = false;
+      for (int x = 0; x < kTries; ++x) r.cut.each[x] = each[p.head_dim == 64 ? 0 : p.head_dim == 128 ? 1 : 2][x];
+    }
     int64_t most_chunks = 0;
     for (int x = 0; x < kTries; ++x) {
       const int n = aim(first + x, units, p.batch);
