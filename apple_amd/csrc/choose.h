@@ -6,6 +6,8 @@
 namespace rfsn {
 namespace {
 
+typedef float float4v __attribute__((ext_vector_type(4)));
+
 // Order of the scores as unsigned keys: NaN as +infinity, -0 as +0.
 __device__ __forceinline__ uint32_t score_key(float s) {
   if (s != s) s = __builtin_inff();
@@ -22,25 +24,31 @@ struct ChooseRoom {
 };
 
 // The `left` numbers of begin .. end - 1 (left below their count) with the largest score(n), ties to the lower number,
-// in ascending order to out[at], out[at + 1], ...
+// in ascending order to emit(at, n), emit(at + 1, n'), ...  score.four(n) has the scores of n .. n + 3, n a multiple of 4.
 // The smallest key to keep is found by narrowing [lo, hi], at first the smallest and largest key: a histogram of
 // 2,048 equal parts of it says which part holds the key wanted.  Scores share their exponent mostly, so parts
 // of their range spread over the counters where their leading bits would meet in one; two rounds are the rule,
 // three the most (leading bits as counters: 50 us for 128 of 2,048 pages, 256 rows; so 6.3, latency of
 // some ten block barriers).  Then each of 16 waves counts what it keeps of its own run and writes it
 // behind the waves before it.  Keys past the LDS copy are read again from the scores.
-template <int KEYS, typename Score>
-__device__ __forceinline__ void choose_largest(ChooseRoom<KEYS>& room, int begin, int end, uint32_t left, int at0, Score score,
-                                               int32_t* __restrict__ out) {
+template <int KEYS, typename Score, typename Emit>
+__device__ __forceinline__ void choose_largest(ChooseRoom<KEYS>& room, int begin, int end, uint32_t left, int at0,
+                                               const Score& score, const Emit& emit) {
   constexpr int T = kChooseWaves * 64, PER = kChooseBins / T;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   auto key = [&](int n) { return n - begin < KEYS ? room.key[n - begin] : score_key(score(n)); };
   uint32_t lo = 0xffffffffu, hi = 0;
 #pragma unroll 4
-  for (int n = begin + tid; n < end; n += T) {
-    const uint32_t k = score_key(score(n));
-    if (n - begin < KEYS) room.key[n - begin] = k;
-    lo = min(lo, k), hi = max(hi, k);
+  for (int n4 = (begin & ~3) + 4 * tid; n4 < end; n4 += 4 * T) {
+    const float4v s = score.four(n4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int n = n4 + e;
+      if (n < begin || n >= end) continue;
+      const uint32_t k = score_key(s[e]);
+      if (n - begin < KEYS) room.key[n - begin] = k;
+      lo = min(lo, k), hi = max(hi, k);
+    }
   }
   lo = ~wave_most(~lo), hi = wave_most(hi);
   if (lane == 0) room.wave[0][wave] = lo, room.wave[1][wave] = hi;
@@ -108,7 +116,7 @@ __device__ __forceinline__ void choose_largest(ChooseRoom<KEYS>& room, int begin
     const uint64_t bt = __ballot(is_tie);
     const bool keep = (n < n1 && k >= over) || (is_tie && before + (uint32_t)__popcll(bt & below) < left);
     const uint64_t bk = __ballot(keep);
-    if (keep) out[at + (uint32_t)__popcll(bk & below)] = n;
+    if (keep) emit((int)(at + (uint32_t)__popcll(bk & below)), n);
     at += (uint32_t)__popcll(bk), before += (uint32_t)__popcll(bt);
   }
 }

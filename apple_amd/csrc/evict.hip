@@ -6,11 +6,17 @@
 namespace rfsn {
 namespace {
 
-constexpr int kEvictKeys = 8192;
+constexpr int kEvictKeys = 16384;  // 72 KB of LDS with the counters: two blocks a CU
 
-// The positions that (sequence, head) keeps, ascending, and the sequences' new lengths.  A block a (sequence, head).
+// Where position n of sequence b lies, as row page_size * page + row of a head's rows, or -1.
+__device__ __forceinline__ int64_t row_of(const rfsn_paged& p, int shift, int b, int n) {
+  const int page = paged_page(p, b, n >> shift);
+  return page < 0 ? -1 : ((int64_t)page << shift) + (n & (p.page_size - 1));
+}
+
+// The rows that (sequence, head) keeps, in the order of their positions, and the sequences' new lengths.  A block a (sequence, head).
 __global__ void __launch_bounds__(kChooseWaves * 64)
-evict_choose_kernel(const rfsn_paged p, int shift, int keep, int first, int last, int32_t* __restrict__ kept,
+evict_choose_kernel(const rfsn_paged p, int shift, int keep, int first, int last, int64_t* __restrict__ kept,
                     int32_t* __restrict__ new_lens) {
   constexpr int T = kChooseWaves * 64;
   __shared__ ChooseRoom<kEvictKeys> room;
@@ -19,83 +25,85 @@ evict_choose_kernel(const rfsn_paged p, int shift, int keep, int first, int last
   const int len = paged_len(p, shift, b);
   if (h == 0 && tid == 0) new_lens[b] = min(len, keep);
   if (len <= keep) return;
-  int32_t* out = kept + ((int64_t)b * p.kv_heads + h) * keep;
+  int64_t* out = kept + ((int64_t)b * p.kv_heads + h) * keep;
   const int end = len - last;
-  auto weight = [&](int n) {
-    const int page = paged_page(p, b, n >> shift);
-    return page < 0 ? -__builtin_inff() : p.weight[((int64_t)page * p.kv_heads + h) * p.page_size + (n & (p.page_size - 1))];
+  struct Weights {
+    const rfsn_paged& p;
+    int shift, b, h;
+    __device__ float operator()(int n) const {
+      const int page = paged_page(p, b, n >> shift);
+      return page < 0 ? -__builtin_inff() : p.weight[((int64_t)page * p.kv_heads + h) * p.page_size + (n & (p.page_size - 1))];
+    }
+    __device__ float4v four(int n) const {
+      const int page = paged_page(p, b, n >> shift);
+      const float none = -__builtin_inff();
+      if (page < 0) return float4v{none, none, none, none};
+      return *reinterpret_cast<const float4v*>(p.weight + ((int64_t)page * p.kv_heads + h) * p.page_size + (n & (p.page_size - 1)));
+    }
   };
-  choose_largest(room, first, end, (uint32_t)(keep - first - last), first, weight, out);
-  for (int i = tid; i < first; i += T) out[i] = i;
-  for (int i = tid; i < last; i += T) out[keep - last + i] = end + i;
+  choose_largest(room, first, end, (uint32_t)(keep - first - last), first, Weights{p, shift, b, h},
+                 [&](int at, int n) { out[at] = row_of(p, shift, b, n); });
+  for (int i = tid; i < first; i += T) out[i] = row_of(p, shift, b, i);
+  for (int i = tid; i < last; i += T) out[keep - last + i] = row_of(p, shift, b, end + i);
 }
 
-// Row kept[j] to row j for j = 0, 1, ..., in place.  kept ascends and kept[j] >= j, so rows that are read later lie
-// behind all that is written now, and a set of rows may be written once all of its reads and those
-// of the sets before it are done: each set is loaded while the one before it waits for the block and is stored.
-// A thread moves `lanes`-th parts of T / lanes rows of a set, U of them.
+// Row kept[j] to position j for j = 0, 1, ..., in place.  Positions ascend and none is below j, so rows that are read later
+// lie behind all that is written now, and a set of them may be written once all of its reads are done: one barrier a set.
+// A thread moves `lanes`-th parts of T / lanes rows, U of them a set, at once.
 template <typename V, int T, int U>
-__device__ __forceinline__ void move_rows(const rfsn_paged& p, int shift, int b, int h, const int32_t* __restrict__ kept, int keep,
+__device__ __forceinline__ void move_rows(const rfsn_paged& p, int shift, int b, const int64_t* __restrict__ kept, int keep,
                                           uint8_t* base, int64_t page_bytes, int row_bytes, int lanes) {
-  const int slot = threadIdx.x / lanes, rows = T / lanes, set = rows * U;
+  const int slot = threadIdx.x / lanes, rows = T / lanes;
   uint8_t* const at = base + (threadIdx.x % lanes) * sizeof(V);
-  V x[2][U];
-  uint8_t* to[2][U];
-  auto load = [&](int j0, V (&v)[U], uint8_t* (&d)[U]) {
+  auto place = [&](int64_t row) { return at + (row >> shift) * page_bytes + (row & (p.page_size - 1)) * row_bytes; };
+#pragma unroll 1
+  for (int j0 = 0; j0 < keep; j0 += rows * U) {
+    int64_t from[U];
+    int page[U];
+    V x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = min(j0 + u * rows + slot, keep - 1);
+      from[u] = kept[j], page[u] = paged_page(p, b, j >> shift);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = j0 + u * rows + slot;
-      d[u] = nullptr, v[u] = V{};
-      if (j >= keep || slot >= rows) continue;
-      const int from = kept[j];
-      if (from == j) continue;
-      const int src = paged_page(p, b, from >> shift), dst = paged_page(p, b, j >> shift);
-      if (src >= 0) v[u] = *reinterpret_cast<const V*>(at + src * page_bytes + (int64_t)(from & (p.page_size - 1)) * row_bytes);
-      if (dst >= 0) d[u] = at + dst * page_bytes + (int64_t)(j & (p.page_size - 1)) * row_bytes;
+      if (j >= keep || slot >= rows || from[u] == ((int64_t)page[u] << shift) + (j & (p.page_size - 1))) page[u] = -1;  // stays
+      x[u] = V{};
+      if (page[u] >= 0 && from[u] >= 0) x[u] = *reinterpret_cast<const V*>(place(from[u]));
     }
-  };
-  auto store = [&](const V (&v)[U], uint8_t* const (&d)[U]) {
-    // the loads that this set is of have returned to every wave before any wave writes
+    // the set's loads have returned to every wave before any wave writes
 #pragma unroll
-    for (int u = 0; u < U; ++u) asm volatile("" ::"v"(v[u]) : "memory");
+    for (int u = 0; u < U; ++u) asm volatile("" ::"v"(x[u]) : "memory");
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (d[u]) *reinterpret_cast<V*>(d[u]) = v[u];
-  };
-  load(0, x[0], to[0]);
-  for (int j0 = 0; j0 < keep; j0 += 2 * set) {
-    load(j0 + set, x[1], to[1]);
-    store(x[0], to[0]);
-    load(j0 + 2 * set, x[0], to[0]);
-    store(x[1], to[1]);
+      if (page[u] >= 0) *reinterpret_cast<V*>(place(((int64_t)page[u] << shift) + ((j0 + u * rows + slot) & (p.page_size - 1)))) = x[u];
   }
 }
 
-// Blocks of a (sequence, head): `parts` slices of K rows, as many of V rows, and one of scales and weights.
-constexpr int kMoveThreads = 256;
+// Blocks of a (sequence, head): `parts` slices of K rows, as many of V rows, one of weights and, with codes, two of scales.
+constexpr int kMoveThreads = 1024, kMoveRows = 16;
 template <int RB, int SB>  // bytes of a row and of its scale
 __global__ void __launch_bounds__(kMoveThreads)
-evict_move_kernel(const rfsn_paged p, int shift, int parts, const int32_t* __restrict__ kept_of, int keep) {
+evict_move_kernel(const rfsn_paged p, int shift, int parts, const int64_t* __restrict__ kept_of, int keep) {
   const int x = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   if (paged_len(p, shift, b) <= keep) return;
-  const int32_t* kept = kept_of + ((int64_t)b * p.kv_heads + h) * keep;
+  const int64_t* kept = kept_of + ((int64_t)b * p.kv_heads + h) * keep;
   if (x < 2 * parts) {
     const int width = RB / parts;
     uint8_t* base = (uint8_t*)(x < parts ? p.k : p.v);
     const int64_t page_bytes = p.page_stride * RB / p.head_dim, head_bytes = p.head_stride * RB / p.head_dim;
-    move_rows<uint4w, kMoveThreads, 4>(p, shift, b, h, kept, keep, base + h * head_bytes + (x % parts) * width, page_bytes, RB, width / 16);
+    move_rows<uint4w, kMoveThreads, kMoveRows>(p, shift, b, kept, keep, base + h * head_bytes + (x % parts) * width, page_bytes, RB, width / 16);
     return;
   }
   auto words = [&](void* base, int row) {
     const int64_t head = (int64_t)p.page_size * row;
-    move_rows<uint32_t, kMoveThreads, 4>(p, shift, b, h, kept, keep, (uint8_t*)base + h * head, head * p.kv_heads, row, row / 4);
+    move_rows<uint32_t, kMoveThreads, 8>(p, shift, b, kept, keep, (uint8_t*)base + h * head, head * p.kv_heads, row, row / 4);
   };
-  words(p.weight, 4);
-  if constexpr (SB > 0) {
-    words(p.k_scale, SB);
-    words(p.v_scale, SB);
-  }
+  if (x == 2 * parts) words(p.weight, 4);
+  else if constexpr (SB > 0) words(x == 2 * parts + 1 ? p.k_scale : p.v_scale, SB);
 }
 
 // Bounds of the pages that hold the kept rows, from the keys as they are read back.  A wave a (page, head).
@@ -125,7 +133,7 @@ using namespace rfsn;
 
 extern "C" size_t rfsn_paged_evict_workspace_bytes(const rfsn_paged* p, int32_t keep) {
   if (p == nullptr || p->batch <= 0 || p->kv_heads <= 0 || keep <= 0) return 0;
-  return (size_t)p->batch * p->kv_heads * keep * sizeof(int32_t);
+  return (size_t)p->batch * p->kv_heads * keep * sizeof(int64_t);
 }
 
 extern "C" int rfsn_paged_evict(const rfsn_paged* p, int32_t keep, int32_t first, int32_t last, int32_t* new_lens,
@@ -140,7 +148,7 @@ extern "C" int rfsn_paged_evict(const rfsn_paged* p, int32_t keep, int32_t first
                "paged_evict: workspace too small or misaligned");
   const hipStream_t s = (hipStream_t)stream;
   const int shift = paged_shift(*p), D = p->head_dim;
-  int32_t* kept = (int32_t*)workspace;
+  int64_t* kept = (int64_t*)workspace;
   hipLaunchKernelGGL(evict_choose_kernel, dim3((unsigned)p->kv_heads, (unsigned)p->batch), dim3(kChooseWaves * 64), 0, s, *p,
                      shift, keep, first, last, kept, new_lens);
   if (int st = check_launch("paged_evict")) return st;
@@ -148,7 +156,7 @@ extern "C" int rfsn_paged_evict(const rfsn_paged* p, int32_t keep, int32_t first
 #define RFSN_EVICT(RB, SB)                                                                                          \
   do {                                                                                                              \
     const int parts = RB > 128 ? RB / 128 : 1;                                                                      \
-    hipLaunchKernelGGL((evict_move_kernel<RB, SB>), dim3(2 * parts + 1, (unsigned)p->kv_heads, (unsigned)p->batch), \
+    hipLaunchKernelGGL((evict_move_kernel<RB, SB>), dim3(2 * parts + 1 + (SB > 0 ? 2 : 0), (unsigned)p->kv_heads, (unsigned)p->batch), \
                        dim3(kMoveThreads), 0, s, *p, shift, parts, kept, keep);                                     \
   } while (0)
 #define RFSN_EVICT_D(DD)                                    \
