@@ -24,31 +24,51 @@ struct ChooseRoom {
 };
 
 // The `left` numbers of begin .. end - 1 (left below their count) with the largest score(n), ties to the lower number,
-// in ascending order to emit(at, n), emit(at + 1, n'), ...  score.four(n) has the scores of n .. n + 3, n a multiple of 4.
+// in ascending order to out[at], out[at + 1], ...  score.four(n) has the scores of n .. n + 3, n a multiple of 4 at most `end`.
 // The smallest key to keep is found by narrowing [lo, hi], at first the smallest and largest key: a histogram of
 // 2,048 equal parts of it says which part holds the key wanted.  Scores share their exponent mostly, so parts
 // of their range spread over the counters where their leading bits would meet in one; two rounds are the rule,
 // three the most (leading bits as counters: 50 us for 128 of 2,048 pages, 256 rows; so 6.3, latency of
 // some ten block barriers).  Then each of 16 waves counts what it keeps of its own run and writes it
 // behind the waves before it.  Keys past the LDS copy are read again from the scores.
-template <int KEYS, typename Score, typename Emit>
+template <int KEYS, typename Score>
 __device__ __forceinline__ void choose_largest(ChooseRoom<KEYS>& room, int begin, int end, uint32_t left, int at0,
-                                               const Score& score, const Emit& emit) {
+                                               const Score& score, int32_t* __restrict__ out) {
   constexpr int T = kChooseWaves * 64, PER = kChooseBins / T;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  auto key = [&](int n) { return n - begin < KEYS ? room.key[n - begin] : score_key(score(n)); };
-  uint32_t lo = 0xffffffffu, hi = 0;
-#pragma unroll 4
-  for (int n4 = (begin & ~3) + 4 * tid; n4 < end; n4 += 4 * T) {
-    const float4v s = score.four(n4);
+  const int held = end - begin < KEYS ? end : begin + KEYS;  // of numbers below it the keys are in LDS
+  // (Numbers past the last one are held in 32 bits without a sign: they may pass 2^31 by a few steps.)
+  // Each number n, n + step, ... below `to` with its key to f, four keys read at a time.  f is called alike by all lanes of a
+  // wave where `to` - n + lane is (numbers from `to` on come with `in` false).
+  auto each = [&](uint32_t n, uint32_t to, uint32_t step, auto&& f) {
+    constexpr int U = 4;
+    for (; n - lane < to; n += U * step) {
+      uint32_t k[U];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int n = n4 + e;
-      if (n < begin || n >= end) continue;
-      const uint32_t k = score_key(s[e]);
-      if (n - begin < KEYS) room.key[n - begin] = k;
-      lo = min(lo, k), hi = max(hi, k);
+      for (int u = 0; u < U; ++u) {
+        const int m = (int)min(n + u * step, to - 1);
+        k[u] = m < held ? room.key[m - begin] : score_key(score(m));
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) f((int)(n + u * step), k[u], n + u * step < to);
     }
+  };
+  uint32_t lo = 0xffffffffu, hi = 0;
+  constexpr int Q = 4;  // fours in flight
+  for (uint32_t n4 = (begin & ~3) + 4 * tid; n4 < (uint32_t)end; n4 += Q * 4 * T) {
+    float4v s[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) s[q] = score.four((int)min(n4 + q * 4 * T, (uint32_t)(end - 1) & ~3u));
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t n = n4 + q * 4 * T + e;
+        if (n < (uint32_t)begin || n >= (uint32_t)end) continue;
+        const uint32_t k = score_key(s[q][e]);
+        if (n - (uint32_t)begin < KEYS) room.key[n - begin] = k;
+        lo = min(lo, k), hi = max(hi, k);
+      }
   }
   lo = ~wave_most(~lo), hi = wave_most(hi);
   if (lane == 0) room.wave[0][wave] = lo, room.wave[1][wave] = hi;
@@ -66,10 +86,9 @@ __device__ __forceinline__ void choose_largest(ChooseRoom<KEYS>& room, int begin
 #pragma unroll
     for (int i = 0; i < PER; ++i) room.hist[tid + i * T] = 0;
     __syncthreads();
-    for (int n = begin + tid; n < end; n += T) {
-      const uint32_t k = key(n);
-      if (k >= lo && k <= hi) atomicAdd(&room.hist[(k - lo) >> sh], 1u);
-    }
+    each(begin + tid, end, T, [&](int, uint32_t k, bool in) {
+      if (in && k >= lo && k <= hi) atomicAdd(&room.hist[(k - lo) >> sh], 1u);
+    });
     __syncthreads();
     // keys in the parts above each thread's PER parts, from the top down
     uint32_t c[PER], mine = 0;
@@ -97,28 +116,26 @@ __device__ __forceinline__ void choose_largest(ChooseRoom<KEYS>& room, int begin
     }
   }
   __syncthreads();  // room.wave is written again
-  const int seg = ((end - begin + kChooseWaves - 1) / kChooseWaves + 63) / 64 * 64;
-  const int n0 = begin + wave * seg, n1 = min(end, n0 + seg);
+  const uint32_t seg = ((end - begin + kChooseWaves - 1) / kChooseWaves + 63) / 64 * 64;
+  const uint32_t n0 = min(begin + wave * seg, (uint32_t)end), n1 = min((uint32_t)end, n0 + seg);
   uint32_t kept = 0, ties = 0;
-  for (int n = n0 + lane; n - lane < n1; n += 64) {
-    const uint32_t k = n < n1 ? key(n) : 0;
-    kept += (uint32_t)__popcll(__ballot(n < n1 && k >= over));
-    ties += (uint32_t)__popcll(__ballot(n < n1 && left && k == tie));
-  }
+  each(n0 + lane, n1, 64, [&](int, uint32_t k, bool in) {
+    kept += (uint32_t)__popcll(__ballot(in && k >= over));
+    ties += (uint32_t)__popcll(__ballot(in && left && k == tie));
+  });
   if (lane == 0) room.wave[0][wave] = kept, room.wave[1][wave] = ties;
   __syncthreads();
   uint32_t before = before_wave(1), at = (uint32_t)at0 + before_wave(0);
   at += min(before, left);
   const uint64_t below = (1ull << lane) - 1;
-  for (int n = n0 + lane; n - lane < n1; n += 64) {
-    const uint32_t k = n < n1 ? key(n) : 0;
-    const bool is_tie = n < n1 && left && k == tie;
+  each(n0 + lane, n1, 64, [&](int n, uint32_t k, bool in) {
+    const bool is_tie = in && left && k == tie;
     const uint64_t bt = __ballot(is_tie);
-    const bool keep = (n < n1 && k >= over) || (is_tie && before + (uint32_t)__popcll(bt & below) < left);
+    const bool keep = (in && k >= over) || (is_tie && before + (uint32_t)__popcll(bt & below) < left);
     const uint64_t bk = __ballot(keep);
-    if (keep) emit((int)(at + (uint32_t)__popcll(bk & below)), n);
+    if (keep) out[at + (uint32_t)__popcll(bk & below)] = n;
     at += (uint32_t)__popcll(bk), before += (uint32_t)__popcll(bt);
-  }
+  });
 }
 
 }  // namespace

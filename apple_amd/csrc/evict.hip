@@ -8,15 +8,9 @@ namespace {
 
 constexpr int kEvictKeys = 16384;  // 72 KB of LDS with the counters: two blocks a CU
 
-// Where position n of sequence b lies, as row page_size * page + row of a head's rows, or -1.
-__device__ __forceinline__ int64_t row_of(const rfsn_paged& p, int shift, int b, int n) {
-  const int page = paged_page(p, b, n >> shift);
-  return page < 0 ? -1 : ((int64_t)page << shift) + (n & (p.page_size - 1));
-}
-
-// The rows that (sequence, head) keeps, in the order of their positions, and the sequences' new lengths.  A block a (sequence, head).
+// The positions that (sequence, head) keeps, ascending, and the sequences' new lengths.  A block a (sequence, head).
 __global__ void __launch_bounds__(kChooseWaves * 64)
-evict_choose_kernel(const rfsn_paged p, int shift, int keep, int first, int last, int64_t* __restrict__ kept,
+evict_choose_kernel(const rfsn_paged p, int shift, int keep, int first, int last, int32_t* __restrict__ kept,
                     int32_t* __restrict__ new_lens) {
   constexpr int T = kChooseWaves * 64;
   __shared__ ChooseRoom<kEvictKeys> room;
@@ -25,7 +19,7 @@ evict_choose_kernel(const rfsn_paged p, int shift, int keep, int first, int last
   const int len = paged_len(p, shift, b);
   if (h == 0 && tid == 0) new_lens[b] = min(len, keep);
   if (len <= keep) return;
-  int64_t* out = kept + ((int64_t)b * p.kv_heads + h) * keep;
+  int32_t* out = kept + ((int64_t)b * p.kv_heads + h) * keep;
   const int end = len - last;
   struct Weights {
     const rfsn_paged& p;
@@ -36,42 +30,42 @@ evict_choose_kernel(const rfsn_paged p, int shift, int keep, int first, int last
     }
     __device__ float4v four(int n) const {
       const int page = paged_page(p, b, n >> shift);
+      const float4v w = *reinterpret_cast<const float4v*>(p.weight + ((int64_t)max(page, 0) * p.kv_heads + h) * p.page_size +
+                                                          (n & (p.page_size - 1)));
       const float none = -__builtin_inff();
-      if (page < 0) return float4v{none, none, none, none};
-      return *reinterpret_cast<const float4v*>(p.weight + ((int64_t)page * p.kv_heads + h) * p.page_size + (n & (p.page_size - 1)));
+      return page < 0 ? float4v{none, none, none, none} : w;
     }
   };
-  choose_largest(room, first, end, (uint32_t)(keep - first - last), first, Weights{p, shift, b, h},
-                 [&](int at, int n) { out[at] = row_of(p, shift, b, n); });
-  for (int i = tid; i < first; i += T) out[i] = row_of(p, shift, b, i);
-  for (int i = tid; i < last; i += T) out[keep - last + i] = row_of(p, shift, b, end + i);
+  choose_largest(room, first, end, (uint32_t)(keep - first - last), first, Weights{p, shift, b, h}, out);
+  for (int i = tid; i < first; i += T) out[i] = i;
+  for (int i = tid; i < last; i += T) out[keep - last + i] = end + i;
 }
 
-// Row kept[j] to position j for j = 0, 1, ..., in place.  Positions ascend and none is below j, so rows that are read later
+// The row of position kept[j] to position j for j = 0, 1, ..., in place.  Positions ascend and none is below j, so rows that are read later
 // lie behind all that is written now, and a set of them may be written once all of its reads are done: one barrier a set.
 // A thread moves `lanes`-th parts of T / lanes rows, U of them a set, at once.
 template <typename V, int T, int U>
-__device__ __forceinline__ void move_rows(const rfsn_paged& p, int shift, int b, const int64_t* __restrict__ kept, int keep,
+__device__ __forceinline__ void move_rows(const rfsn_paged& p, int shift, int b, const int32_t* __restrict__ kept, int keep,
                                           uint8_t* base, int64_t page_bytes, int row_bytes, int lanes) {
   const int slot = threadIdx.x / lanes, rows = T / lanes;
   uint8_t* const at = base + (threadIdx.x % lanes) * sizeof(V);
-  auto place = [&](int64_t row) { return at + (row >> shift) * page_bytes + (row & (p.page_size - 1)) * row_bytes; };
+  auto place = [&](int page, int n) { return at + page * page_bytes + (int64_t)(n & (p.page_size - 1)) * row_bytes; };
 #pragma unroll 1
-  for (int j0 = 0; j0 < keep; j0 += rows * U) {
-    int64_t from[U];
-    int page[U];
+  for (uint32_t j0 = 0; j0 < (uint32_t)keep; j0 += rows * U) {
+    int from[U], source[U], page[U];
     V x[U];
 #pragma unroll
+    for (int u = 0; u < U; ++u) from[u] = kept[min(j0 + u * rows + slot, (uint32_t)keep - 1)];
+#pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int j = min(j0 + u * rows + slot, keep - 1);
-      from[u] = kept[j], page[u] = paged_page(p, b, j >> shift);
+      const uint32_t j = j0 + u * rows + slot;
+      source[u] = paged_page(p, b, from[u] >> shift);
+      page[u] = j >= (uint32_t)keep || slot >= rows || from[u] == (int)j ? -1 : paged_page(p, b, j >> shift);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int j = j0 + u * rows + slot;
-      if (j >= keep || slot >= rows || from[u] == ((int64_t)page[u] << shift) + (j & (p.page_size - 1))) page[u] = -1;  // stays
       x[u] = V{};
-      if (page[u] >= 0 && from[u] >= 0) x[u] = *reinterpret_cast<const V*>(place(from[u]));
+      if (page[u] >= 0 && source[u] >= 0) x[u] = *reinterpret_cast<const V*>(place(source[u], from[u]));
     }
     // the set's loads have returned to every wave before any wave writes
 #pragma unroll
@@ -79,23 +73,23 @@ __device__ __forceinline__ void move_rows(const rfsn_paged& p, int shift, int b,
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (page[u] >= 0) *reinterpret_cast<V*>(place(((int64_t)page[u] << shift) + ((j0 + u * rows + slot) & (p.page_size - 1)))) = x[u];
+      if (page[u] >= 0) *reinterpret_cast<V*>(place(page[u], j0 + u * rows + slot)) = x[u];
   }
 }
 
 // Blocks of a (sequence, head): `parts` slices of K rows, as many of V rows, one of weights and, with codes, two of scales.
-constexpr int kMoveThreads = 1024, kMoveRows = 16;
-template <int RB, int SB>  // bytes of a row and of its scale
+constexpr int kMoveThreads = 1024;
+template <int RB, int SB, int U>  // bytes of a row and of its scale
 __global__ void __launch_bounds__(kMoveThreads)
-evict_move_kernel(const rfsn_paged p, int shift, int parts, const int64_t* __restrict__ kept_of, int keep) {
+evict_move_kernel(const rfsn_paged p, int shift, int parts, const int32_t* __restrict__ kept_of, int keep) {
   const int x = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   if (paged_len(p, shift, b) <= keep) return;
-  const int64_t* kept = kept_of + ((int64_t)b * p.kv_heads + h) * keep;
+  const int32_t* kept = kept_of + ((int64_t)b * p.kv_heads + h) * keep;
   if (x < 2 * parts) {
     const int width = RB / parts;
     uint8_t* base = (uint8_t*)(x < parts ? p.k : p.v);
     const int64_t page_bytes = p.page_stride * RB / p.head_dim, head_bytes = p.head_stride * RB / p.head_dim;
-    move_rows<uint4w, kMoveThreads, kMoveRows>(p, shift, b, kept, keep, base + h * head_bytes + (x % parts) * width, page_bytes, RB, width / 16);
+    move_rows<uint4w, kMoveThreads, U>(p, shift, b, kept, keep, base + h * head_bytes + (x % parts) * width, page_bytes, RB, width / 16);
     return;
   }
   auto words = [&](void* base, int row) {
@@ -133,7 +127,7 @@ using namespace rfsn;
 
 extern "C" size_t rfsn_paged_evict_workspace_bytes(const rfsn_paged* p, int32_t keep) {
   if (p == nullptr || p->batch <= 0 || p->kv_heads <= 0 || keep <= 0) return 0;
-  return (size_t)p->batch * p->kv_heads * keep * sizeof(int64_t);
+  return (size_t)p->batch * p->kv_heads * keep * sizeof(int32_t);
 }
 
 extern "C" int rfsn_paged_evict(const rfsn_paged* p, int32_t keep, int32_t first, int32_t last, int32_t* new_lens,
@@ -148,16 +142,22 @@ extern "C" int rfsn_paged_evict(const rfsn_paged* p, int32_t keep, int32_t first
                "paged_evict: workspace too small or misaligned");
   const hipStream_t s = (hipStream_t)stream;
   const int shift = paged_shift(*p), D = p->head_dim;
-  int64_t* kept = (int64_t*)workspace;
+  int32_t* kept = (int32_t*)workspace;
   hipLaunchKernelGGL(evict_choose_kernel, dim3((unsigned)p->kv_heads, (unsigned)p->batch), dim3(kChooseWaves * 64), 0, s, *p,
                      shift, keep, first, last, kept, new_lens);
   if (int st = check_launch("paged_evict")) return st;
   if ((int64_t)p->table_width * p->page_size <= keep) return RFSN_OK;  // nothing can be longer
+  // Slices of a line of 128 bytes, narrower where that leaves blocks for the chip (2,048 rows of 8 heads of 64, fp16, one
+  // sequence: 16 blocks of 128 bytes 13.8 us, 64 of 32 8.9).  Sets of 16 pieces a thread, or 4 where those hold all rows.
+#define RFSN_EVICT_U(RB, SB, U)                                                                                     \
+  hipLaunchKernelGGL((evict_move_kernel<RB, SB, U>), grid, dim3(kMoveThreads), 0, s, *p, shift, parts, kept, keep)
 #define RFSN_EVICT(RB, SB)                                                                                          \
   do {                                                                                                              \
-    const int parts = RB > 128 ? RB / 128 : 1;                                                                      \
-    hipLaunchKernelGGL((evict_move_kernel<RB, SB>), dim3(2 * parts + 1 + (SB > 0 ? 2 : 0), (unsigned)p->kv_heads, (unsigned)p->batch), \
-                       dim3(kMoveThreads), 0, s, *p, shift, parts, kept, keep);                                     \
+    int parts = RB > 128 ? RB / 128 : 1;                                                                            \
+    while (RB / parts > 32 && (int64_t)2 * parts * p->kv_heads * p->batch < 256) parts *= 2;                        \
+    const dim3 grid(2 * parts + 1 + (SB > 0 ? 2 : 0), (unsigned)p->kv_heads, (unsigned)p->batch);                   \
+    if ((int64_t)keep * (RB / parts) <= 4 * 16 * kMoveThreads) RFSN_EVICT_U(RB, SB, 4);                             \
+    else RFSN_EVICT_U(RB, SB, 16);                                                                                  \
   } while (0)
 #define RFSN_EVICT_D(DD)                                    \
   do {                                                      \
@@ -170,6 +170,7 @@ extern "C" int rfsn_paged_evict(const rfsn_paged* p, int32_t keep, int32_t first
   else RFSN_EVICT_D(256);
 #undef RFSN_EVICT_D
 #undef RFSN_EVICT
+#undef RFSN_EVICT_U
   if (int st = check_launch("paged_evict")) return st;
   if (p->bounds == nullptr) return RFSN_OK;
   const dim3 grid((unsigned)ceil_div(keep, p->page_size), (unsigned)p->kv_heads, (unsigned)p->batch);

@@ -509,7 +509,7 @@ page_choose_kernel(const rfsn_paged p, int shift, const float* __restrict__ scor
       return float4v{s[n], s[min(n + 1, held - 1)], s[min(n + 2, held - 1)], s[min(n + 3, held - 1)]};
     }
   };
-  choose_largest(room, begin, end, (uint32_t)(count - first - last), first, Scores{s, held}, [&](int at, int n) { out[at] = n; });
+  choose_largest(room, begin, end, (uint32_t)(count - first - last), first, Scores{s, held}, out);
   for (int i = tid; i < first; i += T) out[i] = i;
   for (int i = tid; i < last; i += T) out[count - last + i] = end + i;
 }

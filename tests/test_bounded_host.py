@@ -66,7 +66,7 @@ def test_four_bit_pools_are_refused_before_a_launch(lib):
     ((16, 9, 8, 4096, 4096, 1 << 30, None), "keep"), ((16, -1, 8, 4096, 4096, 1 << 30, None), "keep"),
     ((16, 0, -8, 4096, 4096, 1 << 30, None), "keep"), ((16, 4, 4, None, 4096, 1 << 30, None), "null output"),
     ((16, 2 ** 31 - 1, 2 ** 31 - 1, 4096, 4096, 1 << 30, None), "keep"),
-    ((16, 4, 4, 4096, None, 1 << 30, None), "workspace"), ((16, 4, 4, 4096, 4096, 2 * 8 * 16 * 8 - 1, None), "workspace")])
+    ((16, 4, 4, 4096, None, 1 << 30, None), "workspace"), ((16, 4, 4, 4096, 4096, 2 * 8 * 16 * 4 - 1, None), "workspace")])
 def test_evictions_are_refused_before_a_launch(lib, args, says):
     assert lib.rfsn_paged_evict(ctypes.byref(block(weight=4096)), *args) == -1
     assert says.encode() in lib.rfsn_last_error(), lib.rfsn_last_error()
