@@ -187,13 +187,13 @@ __device__ __forceinline__ uint2v quantise(half8v x, uint32_t top, float& scale)
 // 8 values of a row as 4-bit codes, by the largest magnitude (as bits) of the 16 coordinates that share
 // the scale.  The scale has 4 significant bits, so x / scale is a midpoint of two codes or at least 2^-11 of
 // itself away from it: a quotient that is right to the last bit or two would do but for the midpoints, and the
-// step after the product with the reciprocal makes those exact.
+// step after the product with a reciprocal (of one more bit's error at most) makes those exact.  So for amax / 6.
 __device__ __forceinline__ uint32_t quantise_e2m1(half8v x, uint32_t top, uint32_t& byte) {
   if (top >= 0x7c00u) {  // not finite
     byte = 255;
     return 0;
   }
-  const float s = h2f((uint16_t)top) / 6.f;
+  const float amax = h2f((uint16_t)top), sixth = amax * (1.f / 6.f), s = fmaf(fmaf(-sixth, 6.f, amax), 1.f / 6.f, sixth);
   // to 3 mantissa bits: of fp32's from fp16's normal range on, to 2^-17 below it
   const uint32_t u = __builtin_bit_cast(uint32_t, s);
   float r = __builtin_bit_cast(float, (u + 0x7ffffu + ((u >> 20) & 1)) & 0xfff00000u);
@@ -201,7 +201,7 @@ __device__ __forceinline__ uint32_t quantise_e2m1(half8v x, uint32_t top, uint32
   r = fminf(r, 10240.f);
   byte = (uint32_t)(f2h(r) >> 7);
   if (r == 0.f) return 0;
-  const float inv = 1.f / r;
+  const float inv = __builtin_amdgcn_rcpf(r);
   float y[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -397,7 +397,7 @@ __device__ __forceinline__ double group_sum(double x) {
 // fused multiply-adds per coordinate and head.  2,048 pages x 4 KV heads of 64, 8 query heads each:
 // 5.3 us, latency; 32 x 2,048 pages x 8 KV heads, 4 query heads: 44 us for 134 MB, 63 % of the copy rate, with vector
 // instructions in some 60 % of the SIMDs' issue cycles; 32 ragged sequences of up to 2,048 pages: 11.8 us for 17 MB,
-// a third of them, and waves that wait in 56 % of their cycles.
+// a sixth of them, and waves that wait in 56 % of their cycles.
 constexpr int kScoreSets = 2;
 template <int D>
 __global__ void __launch_bounds__(256)

@@ -32,12 +32,17 @@ struct Parts {
   float* ml;    // [slots][q_heads][2]
   int32_t* seq; // [batch][2]
   // of a call that accumulates weights: each position's scores in base 2, and each query head's (m, l)
-  float* score;     // [batch][q_heads][positions]
+  float* score;     // [batch][kv_heads][positions / 16][G][16] (score_at)
   float* fin;       // [batch][q_heads][2]
   int64_t positions;
 };
 
 namespace {
+
+// Where the scores of query head g of G lie for the 16 positions from t on (a multiple of 16), `from` = (b kv_heads + h) positions:
+// what a wave writes at once, 16 positions of its heads, is one piece (a row of positions per head: 32 x 32,768 positions, 4 heads
+// each, 479 us instead of 466).
+__device__ __forceinline__ int64_t score_at(int64_t from, int G, int g, int64_t t) { return (from + t) * G + g * 16; }
 
 struct Chunk {
   int b;       // sequence, -1: none
@@ -310,7 +315,7 @@ __device__ __forceinline__ uint32_t load_scales(const uint8_t* a) {
 }
 
 template <int D, int TYPE, int kWaves, bool kOnce, bool kWeigh>
-__global__ void __launch_bounds__(kWaves * 64, kWaves > 4 ? 1 : D == 64 ? 4 : D == 128 ? 2 : 1)
+__global__ void __launch_bounds__(kWaves * 64, kWaves > 4 ? 1 : D == 64 ? 4 : D == 128 || TYPE == RFSN_PAGE_E2M1 ? 2 : 1)
 paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ table, const uint16_t* __restrict__ q, int G,
                   float scale_log2, const int32_t* __restrict__ chosen, int count, const Cut cut,
                   uint16_t* __restrict__ out, const Parts parts) {
@@ -512,13 +517,6 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
         }
       }
     }
-    if constexpr (kWeigh) {
-#pragma unroll
-      for (int u = 0; u < NG; ++u)
-        if (n[u] > 0 && col < heads)
-          *reinterpret_cast<float4v*>(parts.score + (row0 + col) * parts.positions + t + 16 * u + grp * 4) =
-              kSmall ? s[u] * factor : s[u];
-    }
     ++tile;
     if (t + step < t1) {
       if (tile % GT == 0) {  // the next GT tiles
@@ -527,6 +525,15 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
         locate(tile);
       }
       fetch(t + step, tile);
+    }
+    // The scores of 32 x 32,768 positions, 134 MB, cost fp16 pages 140 us: what is read with them comes at 4.9 TB/s and not 6.5, as in a
+    // copy.  Stored past the caches 480, without a branch (no wait for them, then) 466 as here.
+    if constexpr (kWeigh) {
+#pragma unroll
+      for (int u = 0; u < NG; ++u)
+        if (n[u] > 0 && col < heads)
+          *reinterpret_cast<float4v*>(parts.score + score_at(((int64_t)b * p.kv_heads + h) * parts.positions, G, g0 + col, t + 16 * u) + grp * 4) =
+              kSmall ? s[u] * factor : s[u];
     }
     float pw[4 * NG], ls;
     auto weights = [&]() {
@@ -674,13 +681,11 @@ paged_attn_kernel(const rfsn_paged p, int shift, const int32_t* __restrict__ tab
 // The (m, l) of 64 chunks are one load of a wave.  W waves share a row's chunks: 16 where few rows
 // have many (131,072 positions of one sequence, 128 chunks: the call 64 -> 59 us), 4 for the rows of
 // a batch (48 sequences x 32 heads: 25 us, and 27 with 16).
-template <int D, int W, bool kWeigh>
-__global__ void __launch_bounds__(W * 64)
-paged_merge_kernel(const rfsn_paged p, int shift, int q_heads, int per_seq, const Parts parts, uint16_t* __restrict__ out) {
+template <int D, int W>
+__device__ __forceinline__ void merge_row(const rfsn_paged& p, int shift, int q_heads, int per_seq, const Parts& parts,
+                                          uint16_t* __restrict__ out, int i, int b, float (&s_acc)[W][D]) {
   constexpr int E = D / 64, U = 4;
-  __shared__ float s_acc[W][D];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int i = blockIdx.x, b = blockIdx.y;
   int slot0 = b * per_seq, n = per_seq;
   if (!per_seq) {
     const int len = paged_len(p, shift, b);
@@ -722,10 +727,6 @@ paged_merge_kernel(const rfsn_paged p, int shift, int q_heads, int per_seq, cons
     }
     m = mn;
   }
-  if constexpr (kWeigh) {
-    const int64_t row = (int64_t)b * q_heads + i;
-    if (threadIdx.x == 0) parts.fin[2 * row] = m, parts.fin[2 * row + 1] = l;
-  }
 #pragma unroll
   for (int e = 0; e < E; ++e) s_acc[wave][lane * E + e] = acc[e];
   __syncthreads();
@@ -737,7 +738,19 @@ paged_merge_kernel(const rfsn_paged p, int shift, int q_heads, int per_seq, cons
   }
 }
 
-// The launches of a checked call.
+template <int D, int W>
+__global__ void __launch_bounds__(W * 64)
+paged_merge_kernel(const rfsn_paged p, int shift, int q_heads, int per_seq, const Parts parts, uint16_t* __restrict__ out) {
+  __shared__ float s_acc[W][D];
+  merge_row<D, W>(p, shift, q_heads, per_seq, parts, out, blockIdx.x, blockIdx.y, s_acc);
+}
+
+// Whether 16 waves share a row's chunks, or 4.
+inline bool merge_in_16(const rfsn_paged& p, const Plan& c, int q_heads) {
+  return c.split() && (c.cut.per_seq ? c.cut.per_seq : c.slots - p.batch + 1) > 16 && (int64_t)q_heads * p.batch <= 256;
+}
+
+// The blocks of a checked call.
 template <bool kWeigh>
 int attend_launch(const rfsn_paged* p, const Plan& c, const void* q, int q_heads, float sl2, const int32_t* chosen, int count,
                   void* out, const Parts& parts, hipStream_t s) {
@@ -763,24 +776,6 @@ int attend_launch(const rfsn_paged* p, const Plan& c, const void* q, int q_heads
   else RFSN_ATTEND_D(256, 4, false);
 #undef RFSN_ATTEND_D
 #undef RFSN_ATTEND
-  if (int st = check_launch("paged_attention")) return st;
-  if (c.split()) {
-    const dim3 rows((unsigned)q_heads, (unsigned)p->batch);
-    const bool many = (c.cut.per_seq ? c.cut.per_seq : c.slots - p->batch + 1) > 16 && (int64_t)q_heads * p->batch <= 256;
-#define RFSN_MERGE(DD)                                                                                              \
-  do {                                                                                                              \
-    if (many)                                                                                                       \
-      hipLaunchKernelGGL((paged_merge_kernel<DD, 16, kWeigh>), rows, dim3(1024), 0, s, *p, shift, q_heads, c.cut.per_seq,   \
-                         parts, (uint16_t*)out);                                                                    \
-    else                                                                                                            \
-      hipLaunchKernelGGL((paged_merge_kernel<DD, 4, kWeigh>), rows, dim3(256), 0, s, *p, shift, q_heads, c.cut.per_seq,     \
-                         parts, (uint16_t*)out);                                                                    \
-  } while (0)
-    if (p->head_dim == 64) RFSN_MERGE(64);
-    else if (p->head_dim == 128) RFSN_MERGE(128);
-    else RFSN_MERGE(256);
-#undef RFSN_MERGE
-  }
   return check_launch("paged_attention");
 }
 

@@ -62,7 +62,29 @@ extern "C" int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t 
   char* const w = (char*)workspace;
   Parts parts = {};
   if (c.split()) parts.acc = (float*)(w + r.acc), parts.ml = (float*)(w + r.ml), parts.seq = (int32_t*)(w + r.seq);
-  if (p->weight == nullptr) return attend_launch<false>(p, c, q, q_heads, sl2, chosen, count, out, parts, (hipStream_t)stream);
+  if (p->weight == nullptr) {
+    const hipStream_t s = (hipStream_t)stream;
+    const int shift = paged_shift(*p);
+    if (int st = attend_launch<false>(p, c, q, q_heads, sl2, chosen, count, out, parts, s)) return st;
+    if (c.split()) {
+      const dim3 rows((unsigned)q_heads, (unsigned)p->batch);
+      const bool many = merge_in_16(*p, c, q_heads);
+#define RFSN_MERGE(DD)                                                                                              \
+    do {                                                                                                              \
+      if (many)                                                                                                       \
+        hipLaunchKernelGGL((paged_merge_kernel<DD, 16>), rows, dim3(1024), 0, s, *p, shift, q_heads, c.cut.per_seq,   \
+                           parts, (uint16_t*)out);                                                                    \
+      else                                                                                                            \
+        hipLaunchKernelGGL((paged_merge_kernel<DD, 4>), rows, dim3(256), 0, s, *p, shift, q_heads, c.cut.per_seq,     \
+                           parts, (uint16_t*)out);                                                                    \
+    } while (0)
+      if (p->head_dim == 64) RFSN_MERGE(64);
+      else if (p->head_dim == 128) RFSN_MERGE(128);
+      else RFSN_MERGE(256);
+#undef RFSN_MERGE
+    }
+    return check_launch("paged_attention");
+  }
   parts.score = (float*)(w + r.score), parts.fin = (float*)(w + r.fin);
   parts.positions = (int64_t)p->table_width * p->page_size;
   return launch_weigh(p, c, q, q_heads, sl2, out, parts, (hipStream_t)stream);

@@ -92,9 +92,9 @@ inline Plan plan(const rfsn_paged& p, int q_heads, int count) {
     r.cut = {0, units, least, longest, {}, 128.f, {1.f, 1.f, 1.f}, true};
     if (!r.wide && p.type == RFSN_PAGE_E2M1) {
       // 4-bit rows are decoded by the vector units, which more waves keep busier: 32 x 32,768 positions, 8 KV heads of 64,
-      // take 173, 160 and 149 us as 2, 3 and 4 blocks per CU, 16 x 8,192 of 128 33.8, 32.5 and 35, of 256 82, 87 and 92.  A
+      // take 173, 160 and 149 us as 2, 3 and 4 blocks per CU, 16 x 8,192 of 128 33.8, 32.5 and 35, of 256 61, 74 and 80.  A
       // chunk's start weighs more beside them (131,072 positions of 4 heads of 64: 20.5, 22.4 and 24.4).
-      const float each[3][kTries] = {{1.f, 0.93f, 0.86f}, {1.f, 0.95f, 1.05f}, {1.f, 1.1f, 1.15f}};
+      const float each[3][kTries] = {{1.f, 0.93f, 0.86f}, {1.f, 0.95f, 1.05f}, {1.f, 1.2f, 1.3f}};
       r.cut.start = 300.f, r.cut.alike = false;
       for (int x = 0; x < kTries; ++x) r.cut.each[x] = each[p.head_dim == 64 ? 0 : p.head_dim == 128 ? 1 : 2][x];
     }
