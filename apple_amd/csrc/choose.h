@@ -24,7 +24,8 @@ struct ChooseRoom {
 };
 
 // The `left` numbers of begin .. end - 1 (left below their count) with the largest score(n), ties to the lower number,
-// in ascending order to out[at], out[at + 1], ...  score.four(n) has the scores of n .. n + 3, n a multiple of 4 at most `end`.
+// in ascending order to out[at], out[at + 1], ...  Scores that come in fours (kFours): score.four(n) has those of n .. n + 3, n a
+// multiple of 4 at most `end`.
 // The smallest key to keep is found by narrowing [lo, hi], at first the smallest and largest key: a histogram of
 // 2,048 equal parts of it says which part holds the key wanted.  Scores share their exponent mostly, so parts
 // of their range spread over the counters where their leading bits would meet in one; two rounds are the rule,
@@ -38,10 +39,10 @@ __device__ __forceinline__ void choose_largest(ChooseRoom<KEYS>& room, int begin
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int held = end - begin < KEYS ? end : begin + KEYS;  // of numbers below it the keys are in LDS
   // (Numbers past the last one are held in 32 bits without a sign: they may pass 2^31 by a few steps.)
-  // Each number n, n + step, ... below `to` with its key to f, four keys read at a time.  f is called alike by all lanes of a
+  // Each number n, n + step, ... below `to` with its key to f, U keys read at a time.  f is called alike by all lanes of a
   // wave where `to` - n + lane is (numbers from `to` on come with `in` false).
   auto each = [&](uint32_t n, uint32_t to, uint32_t step, auto&& f) {
-    constexpr int U = 4;
+    constexpr int U = Score::kFours ? 4 : 1;  // (thousands of positions, or some hundred pages)
     for (; n - lane < to; n += U * step) {
       uint32_t k[U];
 #pragma unroll
@@ -54,21 +55,28 @@ __device__ __forceinline__ void choose_largest(ChooseRoom<KEYS>& room, int begin
     }
   };
   uint32_t lo = 0xffffffffu, hi = 0;
-  constexpr int Q = 4;  // fours in flight
-  for (uint32_t n4 = (begin & ~3) + 4 * tid; n4 < (uint32_t)end; n4 += Q * 4 * T) {
-    float4v s[Q];
+  auto take = [&](uint32_t n, float x) {
+    const uint32_t k = score_key(x);
+    if (n - (uint32_t)begin < KEYS) room.key[n - begin] = k;
+    lo = min(lo, k), hi = max(hi, k);
+  };
+  if constexpr (Score::kFours) {
+    constexpr int Q = 4;  // fours in flight
+    for (uint32_t n4 = (begin & ~3) + 4 * tid; n4 < (uint32_t)end; n4 += Q * 4 * T) {
+      float4v s[Q];
 #pragma unroll
-    for (int q = 0; q < Q; ++q) s[q] = score.four((int)min(n4 + q * 4 * T, (uint32_t)(end - 1) & ~3u));
+      for (int q = 0; q < Q; ++q) s[q] = score.four((int)min(n4 + q * 4 * T, (uint32_t)(end - 1) & ~3u));
 #pragma unroll
-    for (int q = 0; q < Q; ++q)
+      for (int q = 0; q < Q; ++q)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t n = n4 + q * 4 * T + e;
-        if (n < (uint32_t)begin || n >= (uint32_t)end) continue;
-        const uint32_t k = score_key(s[q][e]);
-        if (n - (uint32_t)begin < KEYS) room.key[n - begin] = k;
-        lo = min(lo, k), hi = max(hi, k);
-      }
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t n = n4 + q * 4 * T + e;
+          if (n >= (uint32_t)begin && n < (uint32_t)end) take(n, s[q][e]);
+        }
+    }
+  } else {
+#pragma unroll 4
+    for (int n = begin + tid; n < end; n += T) take(n, score(n));
   }
   lo = ~wave_most(~lo), hi = wave_most(hi);
   if (lane == 0) room.wave[0][wave] = lo, room.wave[1][wave] = hi;

@@ -22,6 +22,7 @@ evict_choose_kernel(const rfsn_paged p, int shift, int keep, int first, int last
   int32_t* out = kept + ((int64_t)b * p.kv_heads + h) * keep;
   const int end = len - last;
   struct Weights {
+    enum { kFours = 1 };
     const rfsn_paged& p;
     int shift, b, h;
     __device__ float operator()(int n) const {

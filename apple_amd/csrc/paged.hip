@@ -503,13 +503,10 @@ page_choose_kernel(const rfsn_paged p, int shift, const float* __restrict__ scor
   const int begin = first, end = held - last;
   struct Scores {
     const float* s;
-    int held;
+    enum { kFours = 0 };
     __device__ float operator()(int n) const { return s[n]; }
-    __device__ float4v four(int n) const {
-      return float4v{s[n], s[min(n + 1, held - 1)], s[min(n + 2, held - 1)], s[min(n + 3, held - 1)]};
-    }
   };
-  choose_largest(room, begin, end, (uint32_t)(count - first - last), first, Scores{s, held}, out);
+  choose_largest(room, begin, end, (uint32_t)(count - first - last), first, Scores{s}, out);
   for (int i = tid; i < first; i += T) out[i] = i;
   for (int i = tid; i < last; i += T) out[count - last + i] = end + i;
 }

@@ -162,6 +162,7 @@ void rotary_launch(const rfsn_rotary_params& p, bool same, hipStream_t s) {
   const int threads = units <= 256 ? 256 : 1024;
   int64_t per = (int64_t)(threads / units) * U / heads;
   if (per > ceil_div(p.rows, 1024)) per = ceil_div(p.rows, 1024);
+  if (per * p.rotary_dim * 4 > 32768) per = 32768 / (p.rotary_dim * 4);  // bytes of LDS
   if (per < 1) per = 1;
   const dim3 grid((unsigned)ceil_div(p.rows, per));
   const size_t lds = (size_t)per * p.rotary_dim / 2 * sizeof(Turn);
