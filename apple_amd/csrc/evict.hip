@@ -8,6 +8,13 @@ namespace {
 
 constexpr int kEvictKeys = 16384;  // 72 KB of LDS with the counters: two blocks a CU
 
+// Table entry of a position below the sequence's length, which the table has room for: a load without a condition, so that many
+// are in flight.  Outside [0, pages) it is no page.
+__device__ __forceinline__ int entry_of(const rfsn_paged& p, int shift, int b, int n) {
+  return p.table[(int64_t)b * p.table_stride + (n >> shift)];
+}
+__device__ __forceinline__ bool is_page(const rfsn_paged& p, int page) { return page >= 0 && page < p.pages; }
+
 // The positions that (sequence, head) keeps, ascending, and the sequences' new lengths.  A block a (sequence, head).
 __global__ void __launch_bounds__(kChooseWaves * 64)
 evict_choose_kernel(const rfsn_paged p, int shift, int keep, int first, int last, int32_t* __restrict__ kept,
@@ -26,15 +33,16 @@ evict_choose_kernel(const rfsn_paged p, int shift, int keep, int first, int last
     const rfsn_paged& p;
     int shift, b, h;
     __device__ float operator()(int n) const {
-      const int page = paged_page(p, b, n >> shift);
-      return page < 0 ? -__builtin_inff() : p.weight[((int64_t)page * p.kv_heads + h) * p.page_size + (n & (p.page_size - 1))];
+      const int page = entry_of(p, shift, b, n);
+      const float w = p.weight[((int64_t)(is_page(p, page) ? page : 0) * p.kv_heads + h) * p.page_size + (n & (p.page_size - 1))];
+      return is_page(p, page) ? w : -__builtin_inff();
     }
     __device__ float4v four(int n) const {
-      const int page = paged_page(p, b, n >> shift);
-      const float4v w = *reinterpret_cast<const float4v*>(p.weight + ((int64_t)max(page, 0) * p.kv_heads + h) * p.page_size +
-                                                          (n & (p.page_size - 1)));
+      const int page = entry_of(p, shift, b, n);
+      const int64_t row = ((int64_t)(is_page(p, page) ? page : 0) * p.kv_heads + h) * p.page_size + (n & (p.page_size - 1));
+      const float4v w = *reinterpret_cast<const float4v*>(p.weight + row);
       const float none = -__builtin_inff();
-      return page < 0 ? float4v{none, none, none, none} : w;
+      return is_page(p, page) ? w : float4v{none, none, none, none};
     }
   };
   choose_largest(room, first, end, (uint32_t)(keep - first - last), first, Weights{p, shift, b, h}, out);
@@ -60,13 +68,15 @@ __device__ __forceinline__ void move_rows(const rfsn_paged& p, int shift, int b,
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t j = j0 + u * rows + slot;
-      source[u] = paged_page(p, b, from[u] >> shift);
-      page[u] = j >= (uint32_t)keep || slot >= rows || from[u] == (int)j ? -1 : paged_page(p, b, j >> shift);
+      source[u] = entry_of(p, shift, b, from[u]);
+      page[u] = entry_of(p, shift, b, (int)min(j, (uint32_t)keep - 1));
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      const uint32_t j = j0 + u * rows + slot;
+      if (j >= (uint32_t)keep || slot >= rows || from[u] == (int)j || !is_page(p, page[u])) page[u] = -1;
       x[u] = V{};
-      if (page[u] >= 0 && source[u] >= 0) x[u] = *reinterpret_cast<const V*>(place(source[u], from[u]));
+      if (page[u] >= 0 && is_page(p, source[u])) x[u] = *reinterpret_cast<const V*>(place(source[u], from[u]));
     }
     // the set's loads have returned to every wave before any wave writes
 #pragma unroll
@@ -149,7 +159,7 @@ extern "C" int rfsn_paged_evict(const rfsn_paged* p, int32_t keep, int32_t first
   if (int st = check_launch("paged_evict")) return st;
   if ((int64_t)p->table_width * p->page_size <= keep) return RFSN_OK;  // nothing can be longer
   // Slices of a line of 128 bytes, narrower where that leaves blocks for the chip (2,048 rows of 8 heads of 64, fp16, one
-  // sequence: 16 blocks of 128 bytes 13.8 us, 64 of 32 8.9).  Sets of 16 pieces a thread, or 4 where those hold all rows.
+  // sequence: 16 blocks of 128 bytes 13.8 us, 64 of 32 12.0).  Sets of 16 pieces a thread, or 4 where those hold all rows.
 #define RFSN_EVICT_U(RB, SB, U)                                                                                     \
   hipLaunchKernelGGL((evict_move_kernel<RB, SB, U>), grid, dim3(kMoveThreads), 0, s, *p, shift, parts, kept, keep)
 #define RFSN_EVICT(RB, SB)                                                                                          \
