@@ -148,6 +148,7 @@ extern "C" int rfsn_paged_evict(const rfsn_paged* p, int32_t keep, int32_t first
   RFSN_REQUIRE(keep > 0 && first >= 0 && last >= 0 && (int64_t)first + last <= keep,
                "paged_evict: keep must be positive and have room for the first and last positions");
   if (p->batch == 0) return RFSN_OK;
+  RFSN_REQUIRE(p->batch == 1 || p->table_stride != 0, "paged_evict: sequences share a table");
   RFSN_REQUIRE(new_lens != nullptr, "paged_evict: null output");
   RFSN_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= rfsn_paged_evict_workspace_bytes(p, keep),
                "paged_evict: workspace too small or misaligned");

@@ -48,6 +48,8 @@ extern "C" int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t 
   RFSN_REQUIRE((chosen == nullptr) == (count == 0) && count >= 0, "paged_attention: chosen and count go together");
   RFSN_REQUIRE((int64_t)count * p->page_size <= (1ll << 31) - 1024, "paged_attention: too many chosen pages");
   RFSN_REQUIRE(chosen == nullptr || p->weight == nullptr, "paged_attention: weights are of whole sequences, not of chosen pages");
+  RFSN_REQUIRE(p->weight == nullptr || p->batch <= 1 || p->table_stride != 0,
+               "paged_attention: weights of sequences that share a table");
   const float sl2 = scale * 1.44269504088896340736f;
   RFSN_REQUIRE(sl2 == sl2 && sl2 < __builtin_inff() && sl2 > -__builtin_inff(),
                "paged_attention: scale must be finite, in base 2 as well");

@@ -1038,7 +1038,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     if inv_freq.dim() != 1 or inv_freq.dtype is not torch.float64 or inv_freq.get_device() != dev \
             or not 2 <= 2 * inv_freq.shape[0] <= D:
         raise ValueError(f"rotary: inv_freq must be float64 of 1 to {D // 2} frequencies on q's device")
-    watched = q.requires_grad
+    watched = q.requires_grad or inv_freq.requires_grad
     (qs, qh, qc), Hk, (ks, kh, kc) = q.stride(), 0, (0, 0, 1)
     if k is not None:
         if k.dim() != 3 or k.shape[0] != N or k.shape[2] != D or k.dtype is not dtype or k.get_device() != dev:

@@ -671,7 +671,7 @@ int rfsn_page_select(const rfsn_paged* p, const void* q, int32_t q_heads, int32_
  * With p->weight each position's softmax weight, summed over the query heads of
  * the KV head, is added to its row's (nothing to attend: nothing is added; a head
  * whose weights are NaN adds NaN to all of the sequence's positions); chosen has to be NULL
- * then, and no two sequences of the call may hold one page.
+ * then, and no two sequences of the call may hold one page (a table_stride of 0 is refused).
  * The workspace size depends on q_heads, whether there are weights and, with chosen, count (0: dense). */
 size_t rfsn_paged_attention_workspace_bytes(const rfsn_paged* p, int32_t q_heads, int32_t count);
 int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t q_heads, float scale, const int32_t* chosen,
@@ -687,7 +687,7 @@ int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t q_heads, fl
  * become those of the keys that lie there then, as rfsn_paged_read gives them.
  * Sequences with at most `keep` positions stay as they are.  new_lens
  * [batch]: min(lens, keep).  No two sequences of the call, nor two entries of a sequence's
- * table, may name one page. */
+ * table, may name one page (a table_stride of 0 is refused). */
 size_t rfsn_paged_evict_workspace_bytes(const rfsn_paged* p, int32_t keep);
 int rfsn_paged_evict(const rfsn_paged* p, int32_t keep, int32_t first, int32_t last, int32_t* new_lens,
                      void* workspace, size_t workspace_bytes, void* stream);

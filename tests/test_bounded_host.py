@@ -92,6 +92,14 @@ def test_weights_go_with_whole_sequences(lib):
     assert lib.rfsn_paged_attention(none, None, 8, 0.125, None, 0, None, None, 0, None) == 0
 
 
+def test_weights_of_sequences_that_share_a_table_are_refused(lib):
+    shared = block(weight=4096, table_stride=0)
+    assert lib.rfsn_paged_attention(ctypes.byref(shared), 4096, 8, 0.125, None, 0, 4096, 4096, 1 << 30, None) == -1
+    assert b"share a table" in lib.rfsn_last_error()
+    assert lib.rfsn_paged_evict(ctypes.byref(shared), 16, 4, 4, 4096, 4096, 1 << 30, None) == -1
+    assert b"share a table" in lib.rfsn_last_error()
+
+
 def test_rotary_calls_are_refused_before_a_launch(lib):
     from apple_amd import _lib
 

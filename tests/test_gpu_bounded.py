@@ -702,6 +702,24 @@ def test_wrappers_refuse(device):
 
 # ------------------------------------------------------------------ the cache
 
+def test_calls_that_would_lose_gradients_or_race_are_refused(device):
+    K = kernels()
+    pool = B.Pool("fp16", 8, 2, 16, 64, seed=61)
+    pages, n, w = pool.pages(device), i32([5, 6], device), pool.weight.to(device)
+    q = torch.zeros((2, 4, 64), dtype=D16, device=device)
+    one = torch.zeros((1, 4), dtype=torch.int32, device=device)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        K.rotary(q, None, i32([1, 2], device), freq(64, device).requires_grad_())
+    with torch.no_grad():
+        K.rotary(q, None, i32([1, 2], device), freq(64, device).requires_grad_())
+    with pytest.raises(ValueError, match="share a table"):
+        K.paged_attention(q, pages, one.expand(2, 4), n, 0.1, weight=w)
+    with pytest.raises(ValueError, match="share a table"):
+        K.paged_evict(pages, one.expand(2, 4), n, w, 4, first=0, last=0)
+    K.paged_attention(q, pages, one.expand(2, 4), n, 0.1)  # read alone they may
+    K.paged_attention(q[:1], pages, one, n[:1], 0.1, weight=w)
+
+
 @pytest.mark.parametrize("kind, dim, size", [("e2m1", 64, 16), ("e2m1", 128, 32), ("fp16", 64, 16), ("int8", 256, 16)])
 def test_cache_in_bounded_memory(device, kind, dim, size):
     """Prompts, steps with rotary positions, evictions, a sequence that ends and one that takes its place."""
