@@ -16,6 +16,8 @@ __device__ __forceinline__ int entry_of(const rfsn_paged& p, int shift, int b, i
 __device__ __forceinline__ bool is_page(const rfsn_paged& p, int page) { return page >= 0 && page < p.pages; }
 
 // The positions that (sequence, head) keeps, ascending, and the sequences' new lengths.  A block a (sequence, head).
+// Bound: latency (launch, table, weights, some ten block barriers): 2,111 positions of 8 heads 8.6 us; 32 sequences of up to 16,000 18,
+// 1.9 MB from HBM.
 __global__ void __launch_bounds__(kChooseWaves * 64)
 evict_choose_kernel(const rfsn_paged p, int shift, int keep, int first, int last, int32_t* __restrict__ kept,
                     int32_t* __restrict__ new_lens) {
@@ -53,6 +55,8 @@ evict_choose_kernel(const rfsn_paged p, int shift, int keep, int first, int last
 // The row of position kept[j] to position j for j = 0, 1, ..., in place.  Positions ascend and none is below j, so rows that are read later
 // lie behind all that is written now, and a set of them may be written once all of its reads are done: one barrier a set.
 // A thread moves `lanes`-th parts of T / lanes rows, U of them a set, at once.
+// Bound: the loads in turn of a set (list, table, row), then HBM: 2,048 rows of 8 heads of 64, fp16, 11.2 us; 32 sequences to 4,096 rows
+// of 8 heads of 128 in 4 bits 16.5 us, 79 MB.
 template <typename V, int T, int U>
 __device__ __forceinline__ void move_rows(const rfsn_paged& p, int shift, int b, const int32_t* __restrict__ kept, int keep,
                                           uint8_t* base, int64_t page_bytes, int row_bytes, int lanes) {
