@@ -6,8 +6,6 @@
 namespace rfsn {
 namespace {
 
-constexpr int kEvictKeys = 16384;  // 72 KB of LDS with the counters: two blocks a CU
-
 // Table entry of a position below the sequence's length, which the table has room for: a load without a condition, so that many
 // are in flight.  Outside [0, pages) it is no page.
 __device__ __forceinline__ int entry_of(const rfsn_paged& p, int shift, int b, int n) {
@@ -15,72 +13,72 @@ __device__ __forceinline__ int entry_of(const rfsn_paged& p, int shift, int b, i
 }
 __device__ __forceinline__ bool is_page(const rfsn_paged& p, int page) { return page >= 0 && page < p.pages; }
 
-// The positions that (sequence, head) keeps, ascending, and the sequences' new lengths.  A block a (sequence, head).
-// Bound: latency (launch, table, weights, some ten block barriers): 2,111 positions of 8 heads 8.6 us; 32 sequences of up to 16,000 18,
-// 1.9 MB from HBM.
+// The rows of the positions that (sequence, head) keeps, in their order, by their number in the pool (page times page_size + row; kNone:
+// no page), and the sequences' new lengths.  A block a (sequence, head).
+// Bound: latency (launch, table, weights, some eight block barriers): 2,111 positions of 8 heads 8.3 us; 32 sequences of up to
+// 16,000 13.3, 1.9 MB from HBM (keys in LDS, counted and written by waves with ballots: 18.0).
 __global__ void __launch_bounds__(kChooseWaves * 64)
-evict_choose_kernel(const rfsn_paged p, int shift, int keep, int first, int last, int32_t* __restrict__ kept,
+evict_choose_kernel(const rfsn_paged p, int shift, int keep, int first, int last, uint32_t* __restrict__ kept,
                     int32_t* __restrict__ new_lens) {
   constexpr int T = kChooseWaves * 64;
-  __shared__ ChooseRoom<kEvictKeys> room;
+  __shared__ ChooseBins room;
   const int tid = threadIdx.x;
   const int h = blockIdx.x, b = blockIdx.y;
   const int len = paged_len(p, shift, b);
   if (h == 0 && tid == 0) new_lens[b] = min(len, keep);
   if (len <= keep) return;
-  int32_t* out = kept + ((int64_t)b * p.kv_heads + h) * keep;
+  uint32_t* out = kept + ((int64_t)b * p.kv_heads + h) * keep;
   const int end = len - last;
-  struct Weights {
-    enum { kFours = 1 };
-    const rfsn_paged& p;
-    int shift, b, h;
-    __device__ float operator()(int n) const {
-      const int page = entry_of(p, shift, b, n);
-      const float w = p.weight[((int64_t)(is_page(p, page) ? page : 0) * p.kv_heads + h) * p.page_size + (n & (p.page_size - 1))];
-      return is_page(p, page) ? w : -__builtin_inff();
-    }
-    __device__ float4v four(int n) const {
-      const int page = entry_of(p, shift, b, n);
-      const int64_t row = ((int64_t)(is_page(p, page) ? page : 0) * p.kv_heads + h) * p.page_size + (n & (p.page_size - 1));
-      const float4v w = *reinterpret_cast<const float4v*>(p.weight + row);
-      const float none = -__builtin_inff();
-      return is_page(p, page) ? w : float4v{none, none, none, none};
-    }
+  auto name_of = [&](int page, int n) {
+    return is_page(p, page) ? ((uint32_t)page << shift) + (uint32_t)(n & (p.page_size - 1)) : kNone;
   };
-  choose_largest(room, first, end, (uint32_t)(keep - first - last), first, Weights{p, shift, b, h}, out);
-  for (int i = tid; i < first; i += T) out[i] = i;
-  for (int i = tid; i < last; i += T) out[keep - last + i] = end + i;
+  struct Four {
+    float4v score;
+    uint32_t name;
+  };
+  auto load = [&](int n) {
+    const int page = entry_of(p, shift, b, n);
+    const int64_t row = ((int64_t)(is_page(p, page) ? page : 0) * p.kv_heads + h) * p.page_size + (n & (p.page_size - 1));
+    const float4v w = *reinterpret_cast<const float4v*>(p.weight + row);
+    const float none = -__builtin_inff();
+    return Four{is_page(p, page) ? w : float4v{none, none, none, none}, name_of(page, n)};
+  };
+  for (int i = tid; i < first; i += T) out[i] = name_of(entry_of(p, shift, b, i), i);
+  for (int i = tid; i < last; i += T) out[keep - last + i] = name_of(entry_of(p, shift, b, end + i), end + i);
+  choose_fours(room, first, end, (uint32_t)(keep - first - last), first, load, out);
 }
 
-// The row of position kept[j] to position j for j = 0, 1, ..., in place.  Positions ascend and none is below j, so rows that are read later
-// lie behind all that is written now, and a set of them may be written once all of its reads are done: one barrier a set.
-// A thread moves `lanes`-th parts of T / lanes rows, U of them a set, at once.
-// Bound: the loads in turn of a set (list, table, row), then HBM: 2,048 rows of 8 heads of 64, fp16, 11.2 us; 32 sequences to 4,096 rows
-// of 8 heads of 128 in 4 bits 16.5 us, 79 MB.
+// The rows that the list names to positions 0, 1, ... of the sequence, in place.  Their positions ascend and none is below where its row
+// goes, so rows that are read later lie behind all that is written now, and a set of them may be written once all of its reads are done: one
+// barrier a set.  A thread moves `lanes`-th parts of T / lanes rows, U of them a set, at once.
+// Bound: the loads in turn of a set (list, row), then HBM: 2,048 rows of 8 heads of 64, fp16, 11.0 us; 32 sequences to 4,096 rows
+// of 8 heads of 128 in 4 bits 16.3 us, 79 MB, 4.8 TB/s.
 template <typename V, int T, int U>
-__device__ __forceinline__ void move_rows(const rfsn_paged& p, int shift, int b, const int32_t* __restrict__ kept, int keep,
+__device__ __forceinline__ void move_rows(const rfsn_paged& p, int shift, int b, const uint32_t* __restrict__ kept, int keep,
                                           uint8_t* base, int64_t page_bytes, int row_bytes, int lanes) {
   const int slot = threadIdx.x / lanes, rows = T / lanes;
   uint8_t* const at = base + (threadIdx.x % lanes) * sizeof(V);
-  auto place = [&](int page, int n) { return at + page * page_bytes + (int64_t)(n & (p.page_size - 1)) * row_bytes; };
+  auto place = [&](uint32_t name) {
+    return at + (int64_t)(name >> shift) * page_bytes + (int64_t)(name & (uint32_t)(p.page_size - 1)) * row_bytes;
+  };
 #pragma unroll 1
   for (uint32_t j0 = 0; j0 < (uint32_t)keep; j0 += rows * U) {
-    int from[U], source[U], page[U];
+    uint32_t from[U], to[U];
     V x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) from[u] = kept[min(j0 + u * rows + slot, (uint32_t)keep - 1)];
-#pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t j = j0 + u * rows + slot;
-      source[u] = entry_of(p, shift, b, from[u]);
-      page[u] = entry_of(p, shift, b, (int)min(j, (uint32_t)keep - 1));
+      const uint32_t j = min(j0 + u * rows + slot, (uint32_t)keep - 1);
+      from[u] = kept[j];
+      to[u] = (uint32_t)entry_of(p, shift, b, (int)j);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t j = j0 + u * rows + slot;
-      if (j >= (uint32_t)keep || slot >= rows || from[u] == (int)j || !is_page(p, page[u])) page[u] = -1;
+      const bool there = j < (uint32_t)keep && slot < rows && is_page(p, (int)to[u]);
+      to[u] = there ? (to[u] << shift) + (j & (uint32_t)(p.page_size - 1)) : kNone;
+      if (from[u] == to[u]) to[u] = kNone;
       x[u] = V{};
-      if (page[u] >= 0 && is_page(p, source[u])) x[u] = *reinterpret_cast<const V*>(place(source[u], from[u]));
+      if (to[u] != kNone && is_page(p, (int)(from[u] >> shift))) x[u] = *reinterpret_cast<const V*>(place(from[u]));
     }
     // the set's loads have returned to every wave before any wave writes
 #pragma unroll
@@ -88,7 +86,7 @@ __device__ __forceinline__ void move_rows(const rfsn_paged& p, int shift, int b,
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (page[u] >= 0) *reinterpret_cast<V*>(place(page[u], j0 + u * rows + slot)) = x[u];
+      if (to[u] != kNone) *reinterpret_cast<V*>(place(to[u])) = x[u];
   }
 }
 
@@ -96,10 +94,10 @@ __device__ __forceinline__ void move_rows(const rfsn_paged& p, int shift, int b,
 constexpr int kMoveThreads = 1024;
 template <int RB, int SB, int U>  // bytes of a row and of its scale
 __global__ void __launch_bounds__(kMoveThreads)
-evict_move_kernel(const rfsn_paged p, int shift, int parts, const int32_t* __restrict__ kept_of, int keep) {
+evict_move_kernel(const rfsn_paged p, int shift, int parts, const uint32_t* __restrict__ kept_of, int keep) {
   const int x = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   if (paged_len(p, shift, b) <= keep) return;
-  const int32_t* kept = kept_of + ((int64_t)b * p.kv_heads + h) * keep;
+  const uint32_t* kept = kept_of + ((int64_t)b * p.kv_heads + h) * keep;
   if (x < 2 * parts) {
     const int width = RB / parts;
     uint8_t* base = (uint8_t*)(x < parts ? p.k : p.v);
@@ -142,7 +140,7 @@ using namespace rfsn;
 
 extern "C" size_t rfsn_paged_evict_workspace_bytes(const rfsn_paged* p, int32_t keep) {
   if (p == nullptr || p->batch <= 0 || p->kv_heads <= 0 || keep <= 0) return 0;
-  return (size_t)p->batch * p->kv_heads * keep * sizeof(int32_t);
+  return (size_t)p->batch * p->kv_heads * keep * sizeof(uint32_t);
 }
 
 extern "C" int rfsn_paged_evict(const rfsn_paged* p, int32_t keep, int32_t first, int32_t last, int32_t* new_lens,
@@ -152,13 +150,14 @@ extern "C" int rfsn_paged_evict(const rfsn_paged* p, int32_t keep, int32_t first
   RFSN_REQUIRE(keep > 0 && first >= 0 && last >= 0 && (int64_t)first + last <= keep,
                "paged_evict: keep must be positive and have room for the first and last positions");
   if (p->batch == 0) return RFSN_OK;
+  RFSN_REQUIRE((int64_t)p->pages * p->page_size < (int64_t)kNone, "paged_evict: too many rows");
   RFSN_REQUIRE(p->batch == 1 || p->table_stride != 0, "paged_evict: sequences share a table");
   RFSN_REQUIRE(new_lens != nullptr, "paged_evict: null output");
   RFSN_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= rfsn_paged_evict_workspace_bytes(p, keep),
                "paged_evict: workspace too small or misaligned");
   const hipStream_t s = (hipStream_t)stream;
   const int shift = paged_shift(*p), D = p->head_dim;
-  int32_t* kept = (int32_t*)workspace;
+  uint32_t* kept = (uint32_t*)workspace;
   hipLaunchKernelGGL(evict_choose_kernel, dim3((unsigned)p->kv_heads, (unsigned)p->batch), dim3(kChooseWaves * 64), 0, s, *p,
                      shift, keep, first, last, kept, new_lens);
   if (int st = check_launch("paged_evict")) return st;

@@ -504,7 +504,6 @@ page_choose_kernel(const rfsn_paged p, int shift, const float* __restrict__ scor
   const int begin = first, end = held - last;
   struct Scores {
     const float* s;
-    enum { kFours = 0 };
     __device__ float operator()(int n) const { return s[n]; }
   };
   choose_largest(room, begin, end, (uint32_t)(count - first - last), first, Scores{s}, out);

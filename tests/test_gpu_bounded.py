@@ -385,6 +385,25 @@ def test_evict_long_sequences(device, n, keep):
     evict(device, pool, pool.tables([n]), [n], keep, 4, 64)
 
 
+@pytest.mark.parametrize("n, keep, first, last", [(1000, 500, 4, 64), (16400, 5000, 3, 17), (35001, 20000, 7, 9), (35001, 70, 5, 1)])
+def test_evict_by_weights_of_any_spread(device, n, keep, first, last):
+    """Weights over all exponents, a step of fp32 apart, of few values, and alike but for some: the search for the last one
+    kept takes from none to three histograms, or ends among 64."""
+    g = torch.Generator().manual_seed(n + keep)
+    size = 256
+    P = -(-n // size)
+    any_bits = torch.randint(0, 0x7f800000, (P * size,), generator=g, dtype=torch.int64).to(torch.int32).view(torch.float32)
+    signed = any_bits * (torch.randint(0, 2, any_bits.shape, generator=g) * 2 - 1)
+    steps = (torch.randint(0, 1 << 13, (P * size,), generator=g, dtype=torch.int32) + 0x3f800000).view(torch.float32)
+    few = torch.randint(0, 3, (P * size,), generator=g).float()
+    alike_but = torch.ones(P * size)
+    alike_but[torch.randperm(n, generator=g)[:keep - first - last - 3]] = 1.0 + 2.0 ** -23
+    for i, w in enumerate((any_bits, signed, steps, few, alike_but, torch.zeros(P * size), torch.rand(P * size, generator=g).log().neg())):
+        pool = B.Pool("e2m1", P, 1, size, 64, seed=i, bounds=False)
+        pool.weight = w.reshape(P, 1, size).clone()
+        evict(device, pool, torch.arange(P, dtype=torch.int32).view(1, P), [n], keep, first, last)
+
+
 def test_evict_ties_infinities_nan_and_missing_pages(device):
     """Ties go to the older position, NaN counts as infinite, a missing page's positions are given up first and
     move as zeros; what has no page is not written."""
