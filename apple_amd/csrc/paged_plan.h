@@ -92,17 +92,22 @@ inline Plan plan(const rfsn_paged& p, int q_heads, int count) {
     r.cut = {0, units, least, longest, {}, 128.f, {1.f, 1.f, 1.f}, true};
     if (!r.wide && p.type == RFSN_PAGE_E2M1) {
       // 4-bit rows are decoded by the vector units, which more waves keep busier: 32 x 32,768 positions, 8 KV heads of 64,
-      // take 173, 160 and 149 us as 2, 3 and 4 blocks per CU, 16 x 8,192 of 128 33.8, 32.5 and 35, of 256 61, 74 and 80.  A
+      // take 173, 160 and 149 us as 2, 3 and 4 blocks per CU, 16 x 8,192 of 128 35.9, 34.9 and 34.6, of 256 61, 74 and 80.  A
       // chunk's start weighs more beside them (131,072 positions of 4 heads of 64: 20.5, 22.4 and 24.4).
-      const float each[3][kTries] = {{1.f, 0.93f, 0.86f}, {1.f, 0.95f, 1.05f}, {1.f, 1.2f, 1.3f}};
+      const float each[3][kTries] = {{1.f, 0.93f, 0.86f}, {1.f, 0.95f, 0.87f}, {1.f, 1.2f, 1.3f}};
       r.cut.start = 300.f, r.cut.alike = false;
       for (int x = 0; x < kTries; ++x) r.cut.each[x] = each[p.head_dim == 64 ? 0 : p.head_dim == 128 ? 1 : 2][x];
     }
+    // A batch that fills the chip by itself is weighed in 1, 4/3 and 5/3 chunks a sequence as well, of 4-bit rows of 128 (24
+    // ragged sequences of up to 12,001, 32 heads: 60.4 -> 55.1 us, 100 of 3,000 84 -> 81; of 64, 64 of up to 9,000: 57.7, so 60.5).
+    const bool full = p.batch <= 4096 && aim(first + kTries - 1, units, p.batch) == p.batch;  // (the grid ends at 65,535 chunks)
     int64_t most_chunks = 0;
     for (int x = 0; x < kTries; ++x) {
-      const int n = aim(first + x, units, p.batch);
+      int n = aim(first + x, units, p.batch);
+      const int finer = full ? p.batch * (3 + x) / 3 : n;
+      if (!r.cut.alike && full && p.head_dim == 128) n = finer, r.cut.each[x] = 1.f;
       r.cut.one_over[x] = 1.f / (float)n;
-      most_chunks = n > most_chunks ? n : most_chunks;
+      most_chunks = finer > most_chunks ? finer : most_chunks;  // alike for all types, as the workspace is
     }
     // The sum of ceil(len / size) is at most total / size + batch, and size at least total / target - 0.02
     // (find_chunk) and `least`: below 32767 (0.02 / 512 + 2^-21) < 2 chunks over the target (wide blocks

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from tests import bounded_reference as B
-from tests.test_paged_host import ROOT, block, config, lib  # noqa: F401
+from tests.test_paged_host import ROOT, block, chunks_by_lengths, config, lib, plan  # noqa: F401
 
 
 def four(**kw):
@@ -90,6 +90,33 @@ def test_weights_go_with_whole_sequences(lib):
     none = ctypes.byref(block(batch=0, table=0, lens=0, weight=4096))
     assert lib.rfsn_paged_evict(none, 16, 4, 4, None, None, 0, None) == 0
     assert lib.rfsn_paged_attention(none, None, 8, 0.125, None, 0, None, None, 0, None) == 0
+
+
+def test_four_bit_chunks_have_slots_in_a_workspace_that_knows_no_type(plan, lib):
+    import random
+
+    rng = random.Random(9)
+    codes = dict(type=4, k_scale=4096, v_scale=4096)
+    seen = 0
+    for i in range(500):
+        batch, size = rng.choice([1, 2, 17, 24, 64, 65, 500, 4000, 4097, 20000, 32000]), rng.choice([16, 64, 256])
+        heads, group, dim = rng.choice([1, 2, 8, 32, 512]), rng.choice([1, 4, 20]), rng.choice([64, 128, 256])
+        width = max(1, int(2 ** rng.uniform(7, 24)) // size)
+        kw = dict(batch=batch, table_width=width, table_stride=width, page_size=size, kv_heads=heads, head_dim=dim,
+                  head_stride=size * dim, page_stride=heads * size * dim)
+        cut = plan(heads * group, **codes, **kw)
+        assert cut["slots"] == plan(heads * group, **kw)["slots"] <= 65535
+        sizes = [lib.rfsn_paged_attention_workspace_bytes(ctypes.byref(block(**of, **kw)), heads * group, 0) for of in (codes, {})]
+        assert sizes[0] == sizes[1]
+        if cut["per_seq"]:
+            continue
+        seen += 1
+        lens = [width * size if rng.random() < 0.5 else int((width * size) ** rng.random()) for _ in range(min(batch, 300))]
+        lens = (lens * -(-batch // len(lens)))[:batch]
+        for all_of in (lens, [width * size] * batch, [0] * (batch - 1) + [width * size]):
+            for chunks, longest in chunks_by_lengths(cut, all_of):
+                assert chunks <= cut["slots"] and longest <= max(cut["longest"], cut["chunk"]), (cut, chunks, longest)
+    assert seen > 150
 
 
 def test_weights_of_sequences_that_share_a_table_are_refused(lib):
