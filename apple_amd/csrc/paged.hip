@@ -3,8 +3,8 @@
 //
 // Append and read move each row once and are bound by HBM from some 30 MB on (16,384 rows
 // x 32 heads of 128, K and V: fp16 with bounds 537 MB in 101 us, 5.3 TB/s, and 98 us back; int8
-// 403 MB in 97 us and 84 us back; 4 bits: 2,663 rows x 32 heads of 128, 56 MB in 18 us, 3.2 TB/s, and
-// 16 us back, 3.5 TB/s); below it by the loads that wait for one another (sequence,
+// 403 MB in 97 us and 84 us back; 4 bits: 2,663 rows x 32 heads of 128, 56 MB in 16 us, 3.5 TB/s, and
+// 13 us back, 4.4 TB/s); below it by the loads that wait for one another (sequence,
 // page, row): 32 rows of 8 heads 3.5 us.
 #include "choose.h"
 #include "paged.h"

@@ -13,8 +13,8 @@
 // that there are, the matrix cores 6 % busy, VALU 15 %, no LDS conflicts; int8 205 us,
 // 5.6 TB/s; 4 x 8,001, 32 KV heads of 128: 77 to 84 us, 6.2 to 6.8 TB/s).  Of 4-bit pages
 // the same 32 x 32,768 positions are 604 MB in 116 us, 5.2 TB/s, called again and again 130 to 150 at
-// a lower clock (vector units 16 %, matrix cores 18 % busy; loads alone 107, arithmetic alone 83); with
-// 32 KV heads of one query head, 24 of up to 12,001 positions of 128, 138 MB in 38 us.  Below some
+// a lower clock (vector units 66 %, matrix cores 18 % busy; loads alone 107, arithmetic alone 83); with
+// 32 KV heads of one query head, 24 of up to 12,001 positions of 128, 138 MB in 35 us.  Below some
 // 50 MB the chain of dependent loads (length, page, rows), the launch and the merge:
 // 1,021 positions x 8 KV heads 8.8 to 9.4 us, 8,192 of int8 8.5 us and 3 to 4 for the merge.
 // One wave per head and chunk with fp32 FMAs (attend_row, now for sums that are not
