@@ -153,6 +153,8 @@ extern "C" int rfsn_paged_evict(const rfsn_paged* p, int32_t keep, int32_t first
   RFSN_REQUIRE((int64_t)p->pages * p->page_size < (int64_t)kNone, "paged_evict: too many rows");
   RFSN_REQUIRE(p->batch == 1 || p->table_stride != 0, "paged_evict: sequences share a table");
   RFSN_REQUIRE(new_lens != nullptr, "paged_evict: null output");
+  RFSN_REQUIRE((uintptr_t)new_lens >= (uintptr_t)(p->lens + p->batch) || (uintptr_t)p->lens >= (uintptr_t)(new_lens + p->batch),
+               "paged_evict: new_lens overlaps lens, which the launches read");
   RFSN_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= rfsn_paged_evict_workspace_bytes(p, keep),
                "paged_evict: workspace too small or misaligned");
   const hipStream_t s = (hipStream_t)stream;

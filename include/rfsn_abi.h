@@ -686,8 +686,9 @@ int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t q_heads, fl
  * page moves as a row of zeros.  Bounds of all of the sequence's pages up to position keep - 1
  * become those of the keys that lie there then, as rfsn_paged_read gives them.
  * Sequences with at most `keep` positions stay as they are.  new_lens
- * [batch]: min(lens, keep).  No two sequences of the call, nor two entries of a sequence's
- * table, may name one page (a table_stride of 0 is refused). */
+ * [batch]: min(lens, keep); it may not overlap lens, which the launches read (refused).
+ * No two sequences of the call, nor two entries of a sequence's table, may name one page
+ * (a table_stride of 0 is refused). */
 size_t rfsn_paged_evict_workspace_bytes(const rfsn_paged* p, int32_t keep);
 int rfsn_paged_evict(const rfsn_paged* p, int32_t keep, int32_t first, int32_t last, int32_t* new_lens,
                      void* workspace, size_t workspace_bytes, void* stream);
