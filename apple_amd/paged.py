@@ -81,6 +81,7 @@ class RFSNPagedKVCache:
         self._ended = set()  # released, and without tokens since
         self._given_up = new((batch,), torch.int32)  # tokens that the sequences hold no longer
         self._gaps: List[int] = [0] * batch          # rows at the front of each that may not be neighbours' any more
+        self._unseen: List[int] = [0] * batch        # newest tokens of each that no attention has given weights yet
 
     @property
     def free_pages(self) -> int:
@@ -143,6 +144,7 @@ class RFSNPagedKVCache:
             K.paged_append(self.pages, self.table, self.lens, k, v, on[0], **kept)
             self.lens.add_(on[1, :-1])
         self.num_tokens = [n + c for n, c in zip(self.num_tokens, each)]
+        self._unseen = [n + c for n, c in zip(self._unseen, each)]
         if self._ended:
             self._ended = {b for b in self._ended if not self.num_tokens[b]}
 
@@ -162,7 +164,7 @@ class RFSNPagedKVCache:
         self.table[b].fill_(-1)
         self.lens[b:b + 1].zero_()
         self._given_up[b:b + 1].zero_()
-        self._gaps[b] = 0
+        self._gaps[b] = self._unseen[b] = 0
         self._ended.add(b)
 
     def positions(self, counts: Optional[Sequence[int]] = None) -> torch.Tensor:
@@ -189,7 +191,10 @@ class RFSNPagedKVCache:
     def evict(self, keep: int, first: int = 4, last: int = 64) -> None:
         """Sequences of more than ``keep`` tokens give up the others, each KV
         head its own: kept are the ``first`` oldest, the ``last`` newest and those with the most attention
-        weight (``kernels.paged_evict``).  Pages that are not needed any more return to the pool."""
+        weight (``kernels.paged_evict``).  Pages that are not needed any more return to the pool.
+        Weights come from ``attention_forward`` alone: tokens that were appended behind the last one (a
+        prompt's) have none, and a call that would choose among them is refused, so attend first or keep them all
+        by ``last``."""
         if self.weight is None:
             raise ValueError("evict goes by attention weights: the cache keeps none (weights=True)")
         if keep <= 0 or first < 0 or last < 0 or first + last > keep:
@@ -197,6 +202,11 @@ class RFSNPagedKVCache:
         long = [b for b, n in enumerate(self.num_tokens) if n > keep]
         if not long:
             return
+        if first + last < keep:
+            for b in long:
+                if self._unseen[b] > last:
+                    raise ValueError(f"the {self._unseen[b]} newest tokens of sequence {b} have had no attention_forward "
+                                     f"and so no weight, and only the last {last} are kept without one")
         new = K.paged_evict(self.pages, self._live_table(), self.lens, self.weight, keep, first=first, last=last)
         self._given_up.add_(self.lens - new)
         self.lens.copy_(new)
@@ -204,7 +214,9 @@ class RFSNPagedKVCache:
         for b in long:
             self._free.extend(reversed(self._held[b][need:]))
             del self._held[b][need:]
-            whole = min(last, self.num_tokens[b] - self._gaps[b])  # newest tokens without a gap
+            n, unseen = self.num_tokens[b], self._unseen[b]
+            whole = min(last, n - self._gaps[b])  # newest tokens without a gap
+            self._unseen[b] = min(unseen, last) + max(0, first - (n - unseen))
             self.num_tokens[b], self._gaps[b] = keep, keep - whole
         self.table[torch.tensor(long, device=self.device), need:] = -1
 
@@ -230,7 +242,10 @@ class RFSNPagedKVCache:
             chosen = K.page_select(qh, self.pages, table, self.lens, sparse_pages)
         held = self.pages.k.shape[0] - len(self._free)
         kept = {} if self.weight is None or chosen is not None else {"weight": self.weight}
-        return K.paged_attention(qh, self.pages, table, self.lens, self.scale, chosen, held, **kept).to(q.dtype)
+        out = K.paged_attention(qh, self.pages, table, self.lens, self.scale, chosen, held, **kept)
+        if kept:
+            self._unseen = [0] * self.batch
+        return out.to(q.dtype)
 
     def prompt_attention(self, b: int, q: torch.Tensor) -> torch.Tensor:
         """q [S, Hq, D], the newest S tokens of sequence b, each over the

@@ -19,3 +19,79 @@ def test_new_lengths_over_the_old_ones_are_refused(lib, offset):
     for apart in (8, -8):  # two sequences' lengths further on, or before
         assert evict(p.lens + apart) == -1
         assert b"workspace" in lib.rfsn_last_error(), lib.rfsn_last_error()
+
+
+def quiet_cache(monkeypatch, batch, calls=None, pages=64, **kw):
+    """A cache on the host whose kernels do nothing; attention calls' (lens, table, held) go to ``calls``."""
+    from apple_amd import kernels as K
+    from apple_amd.paged import RFSNPagedKVCache
+    from tests.test_paged_host import config
+
+    def attention(q, pages, table, lens, scale, chosen=None, held=0, weight=None):
+        if calls is not None:
+            calls.append((q, table.clone(), lens.tolist(), held, weight))
+        return q + 1
+
+    monkeypatch.setattr(K, "paged_append", lambda pages, table, lens, k, v, cu=None, weight=None: None)
+    monkeypatch.setattr(K, "paged_evict", lambda pages, table, lens, weight, keep, *, first, last: lens.clamp_max(keep))
+    monkeypatch.setattr(K, "paged_attention", attention)
+    monkeypatch.setattr(K, "page_select", lambda *a: torch.zeros((batch, 2, 2), dtype=torch.int32))
+    return RFSNPagedKVCache(config(), batch=batch, pages=pages, page_size=16, device="cpu", weights=True, **kw)
+
+
+def rows(n):
+    return torch.zeros((n, 2, 64), dtype=torch.float16)
+
+
+def test_tokens_without_weights_are_not_chosen_among(monkeypatch):
+    """A prompt's rows have weight 0 until a token attends them: an eviction by it would keep the oldest of them."""
+    c = quiet_cache(monkeypatch, 2)
+    q = torch.zeros((2, 8, 64))
+    c.prefill(0, rows(300), rows(300))
+    before = (c.num_tokens[:], c.free_pages, c.table.clone())
+    with pytest.raises(ValueError, match="300 newest tokens of sequence 0"):
+        c.evict(100)
+    c.attention_forward(q, sparse_pages=2)  # adds no weights
+    with pytest.raises(ValueError, match="weight"):
+        c.evict(100)
+    assert (c.num_tokens, c.free_pages) == before[:2] and torch.equal(c.table, before[2])
+    c.evict(300)   # nothing to give up
+    c.evict(100, 30, 70)  # nothing to choose
+    assert c.num_tokens == [100, 0]
+    with pytest.raises(ValueError, match="weight"):
+        c.evict(80)
+    c.attention_forward(q)
+    c.evict(80)
+    assert c.num_tokens == [80, 0]
+    # a chunk of a prompt behind it: its newest `last` are kept whatever they weigh, the others not
+    c.prefill(0, rows(65), rows(65))
+    with pytest.raises(ValueError, match="65 newest"):
+        c.evict(90)
+    c.evict(90, last=65)
+    assert c.num_tokens == [90, 0]
+    # the other sequence has no more than it may keep
+    c.append(rows(50), rows(50), [0, 50])
+    c.attention_forward(q)
+    c.append(rows(40), rows(40), [0, 40])
+    c.evict(90, last=10)
+    with pytest.raises(ValueError, match="40 newest tokens of sequence 1"):
+        c.evict(60, last=30)
+    c.release(1)
+    c.evict(60, last=30)
+    assert c.num_tokens == [60, 0]
+    c.append(rows(200), rows(200), [0, 200])
+    with pytest.raises(ValueError, match="200 newest tokens of sequence 1"):
+        c.evict(80)
+
+
+def test_tokens_without_weights_after_an_eviction_without_a_choice(monkeypatch):
+    """Those kept at either end still count."""
+    c = quiet_cache(monkeypatch, 1)
+    c.prefill(0, rows(40), rows(40))
+    c.attention_forward(torch.zeros((1, 8, 64)))
+    c.prefill(0, rows(60), rows(60))
+    c.evict(70, 50, 20)  # 10 of the 60 among the first 50, 20 among the last
+    with pytest.raises(ValueError, match="30 newest"):
+        c.evict(60, 4, 29)
+    c.evict(60, 4, 30)
+    assert c.num_tokens == [60]
