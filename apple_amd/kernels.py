@@ -1022,7 +1022,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     (i, i + R / 2) (``layout`` "half") or (2 i, 2 i + 1) ("interleaved") by
     positions[n] * inv_freq[i] and scaled by ``factor`` (``rfsn_rotary``); the
     others are copied.  ``positions`` [N] int32 or int64, ``inv_freq`` float64
-    (``layer.rope_inv_freq``).  New contiguous tensors, or with ``inplace`` q and k themselves."""
+    (``layer.rope_inv_freq``).  New contiguous tensors, or with ``inplace`` q and k themselves,
+    whose autograd versions grow as with torch's own in-place operators."""
     dev = q.get_device()
     if dev < 0:
         L.require_device(q, "rotary")
@@ -1050,6 +1051,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     if inplace:
         if qc != 1 or kc != 1 or not _apart(q) or k is not None and (not _apart(k) or N and Hq and Hk and not _clear_of(q, k)):
             raise ValueError("rotary: in place, the coordinates must be dense and no two elements share memory")
+        torch.autograd.graph.increment_version(q if k is None else (q, k))  # gradients of what read the rows before
         qo, ko, qos, qoh, kos, koh = q, k, qs, qh, ks, kh
     else:
         qo = q.new_empty(shape)
