@@ -35,6 +35,11 @@ from .storage import RFSNConfig
 
 PAGE_DTYPES = {"fp16": torch.float16, "int8": torch.int8, "e4m3": torch.float8_e4m3fn, "e2m1": torch.uint8}
 
+# Weighted attention keeps 4 bytes of scores per query head and position of its table's room: the batch times its longest sequence.
+# Up to this many bytes, which are little beside 288 GB, a call takes the batch as it is; past it no more than
+# the pool has rows for.
+SCORES_AT_LEAST = 256 << 20
+
 
 class RFSNPagedKVCache:
     """``pages`` pages of ``page_size`` tokens for up to ``batch`` sequences of up to ``max_tokens`` tokens (default:
@@ -224,13 +229,28 @@ class RFSNPagedKVCache:
         """The table's columns that some sequence uses."""
         return self.table[:, :max(1, max(len(h) for h in self._held))]
 
+    def _runs(self, q_heads: int) -> List[Tuple[int, int]]:
+        """Neighbouring sequences [begin, end) whose scores keep to the pool's size: a long one among short ones would
+        need room for each of them as long."""
+        most = max(self.pages.k.shape[0], SCORES_AT_LEAST // (4 * self.page_size * q_heads))
+        if self.batch * max(len(h) for h in self._held) <= most:
+            return [(0, self.batch)]
+        runs, begin, longest = [], 0, 0
+        for b, held in enumerate(self._held):
+            longest = max(longest, len(held))
+            if b > begin and (b + 1 - begin) * longest > most:
+                runs.append((begin, b))
+                begin, longest = b, len(held)
+        return runs + [(begin, self.batch)]
+
     def attention_forward(self, q: torch.Tensor, sparse_pages: int = 0) -> torch.Tensor:
         """q [B, Hq, D], each sequence's newest token, over the sequence's
         positions -> [B, Hq, D] in q's dtype; an empty sequence gives zeros.
         ``sparse_pages``: over that many of its pages per KV head, the first, the
         newest and those whose bounds promise the largest scores (of keys before
         their rounding to 8 or 4 bits).  A cache with ``weights`` adds up those of whole
-        sequences, not of ``sparse_pages``."""
+        sequences, not of ``sparse_pages``, and attends the batch in parts where its
+        scores would need more room than the pool's rows (``SCORES_AT_LEAST``)."""
         if q.dim() != 3 or q.shape[0] != self.batch or q.shape[2] != self.D:
             raise ValueError(f"q must be [{self.batch}, heads, {self.D}]")
         qh = q.to(device=self.device, dtype=torch.float16)
@@ -241,10 +261,19 @@ class RFSNPagedKVCache:
                 raise ValueError("sparse_pages must have room for the first and the newest page")
             chosen = K.page_select(qh, self.pages, table, self.lens, sparse_pages)
         held = self.pages.k.shape[0] - len(self._free)
-        kept = {} if self.weight is None or chosen is not None else {"weight": self.weight}
-        out = K.paged_attention(qh, self.pages, table, self.lens, self.scale, chosen, held, **kept)
-        if kept:
-            self._unseen = [0] * self.batch
+        if self.weight is None or chosen is not None:
+            return K.paged_attention(qh, self.pages, table, self.lens, self.scale, chosen, held).to(q.dtype)
+        runs = self._runs(q.shape[1])
+        if len(runs) == 1:
+            out = K.paged_attention(qh, self.pages, table, self.lens, self.scale, None, held, weight=self.weight)
+        else:
+            parts = []
+            for begin, end in runs:
+                pages = [len(h) for h in self._held[begin:end]]
+                parts.append(K.paged_attention(qh[begin:end], self.pages, table[begin:end, :max(1, max(pages))],
+                                               self.lens[begin:end], self.scale, None, sum(pages), weight=self.weight))
+            out = torch.cat(parts)
+        self._unseen = [0] * self.batch
         return out.to(q.dtype)
 
     def prompt_attention(self, b: int, q: torch.Tensor) -> torch.Tensor:

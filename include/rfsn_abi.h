@@ -672,7 +672,9 @@ int rfsn_page_select(const rfsn_paged* p, const void* q, int32_t q_heads, int32_
  * the KV head, is added to its row's (nothing to attend: nothing is added; a head
  * whose weights are NaN adds NaN to all of the sequence's positions); chosen has to be NULL
  * then, and no two sequences of the call may hold one page (a table_stride of 0 is refused).
- * The workspace size depends on q_heads, whether there are weights and, with chosen, count (0: dense). */
+ * The workspace size depends on q_heads, whether there are weights and, with chosen, count (0: dense).
+ * Weights take batch * q_heads * table_width * page_size * 4 bytes of it, so a table as wide as the call's longest
+ * sequence needs, and one that is far longer than the others is better attended in a call of its own. */
 size_t rfsn_paged_attention_workspace_bytes(const rfsn_paged* p, int32_t q_heads, int32_t count);
 int rfsn_paged_attention(const rfsn_paged* p, const void* q, int32_t q_heads, float scale, const int32_t* chosen,
                          int32_t count, void* out, void* workspace, size_t workspace_bytes, void* stream);

@@ -95,3 +95,51 @@ def test_tokens_without_weights_after_an_eviction_without_a_choice(monkeypatch):
         c.evict(60, 4, 29)
     c.evict(60, 4, 30)
     assert c.num_tokens == [60]
+
+
+def score_bytes(q, table, page_size):
+    return table.shape[0] * table.shape[1] * page_size * q.shape[1] * 4
+
+
+@pytest.mark.parametrize("lens, most", [
+    ([2000] + [10] * 40, None), ([10] * 40 + [2000], None), ([10] * 20 + [1500] + [10] * 20 + [500] + [0] * 9, 5),
+    ([500, 10] * 4 + [0, 0, 3], 9), ([100] * 20, 1), ([0, 0, 1], 1), ([16 * 100 // (i + 1) for i in range(30)], 8)])
+def test_scores_never_need_more_than_the_pool(monkeypatch, lens, most):
+    """A batch under one wide table would need room for its scores by its longest sequence, times the batch."""
+    from apple_amd import paged
+
+    calls, batch = [], len(lens)
+    c = quiet_cache(monkeypatch, batch, calls, pages=sum(-(-n // 16) for n in lens) + 2)
+    c.append(rows(sum(lens)), rows(sum(lens)), lens)
+    q = torch.arange(batch * 8 * 64, dtype=torch.float32).view(batch, 8, 64).remainder(512)
+    out = c.attention_forward(q)
+    assert len(calls) == 1 and torch.equal(out, q + 1)  # 256 MiB are no matter
+    del calls[:]
+    monkeypatch.setattr(paged, "SCORES_AT_LEAST", 0)
+    c._unseen = [n for n in lens]
+    out = c.attention_forward(q)
+    assert torch.equal(out, q + 1) and out.dtype == q.dtype and c._unseen == [0] * batch
+    assert len(calls) <= (most or 4), len(calls)
+    assert [n for call in calls for n in call[2]] == lens
+    b = 0
+    for x, table, n, held, weight in calls:
+        assert weight is c.weight and torch.equal(x, q[b:b + len(n)].half())
+        assert torch.equal(table, c.table[b:b + len(n), :table.shape[1]])
+        assert all(-(-t // 16) <= table.shape[1] for t in n) and held == sum(-(-t // 16) for t in n)
+        assert score_bytes(x, table, 16) <= c.pages.k.shape[0] * 16 * 8 * 4
+        b += len(n)
+    # without weights there are no scores
+    del calls[:]
+    c.weight = None
+    c.attention_forward(q)
+    assert len(calls) == 1
+
+
+def test_scores_of_a_long_sequence_among_short_ones(monkeypatch):
+    calls = []
+    c = quiet_cache(monkeypatch, 64, calls, pages=8700, max_tokens=140000)
+    lens = [16 * 4] * 20 + [131072] + [16 * 6] * 43
+    c.append(rows(sum(lens)), rows(sum(lens)), lens)
+    c.attention_forward(torch.zeros((64, 32, 64)))
+    assert [len(n) for _, _, n, _, _ in calls] == [20, 16, 28]
+    assert max(score_bytes(q, table, 16) for q, table, *_ in calls) <= 256 << 20  # 1,074 MB in one
