@@ -6,7 +6,8 @@ import ctypes
 import pytest
 import torch
 
-from tests.test_paged_host import block, lib  # noqa: F401
+from tests.test_gpu_bounded_paths import CALLS, shape_of
+from tests.test_paged_host import block, chunks_by_lengths, lib, plan  # noqa: F401
 
 
 @pytest.mark.parametrize("offset", [0, 4, -4])
@@ -143,3 +144,40 @@ def test_scores_of_a_long_sequence_among_short_ones(monkeypatch):
     c.attention_forward(torch.zeros((64, 32, 64)))
     assert [len(n) for _, _, n, _, _ in calls] == [20, 16, 28]
     assert max(score_bytes(q, table, 16) for q, table, *_ in calls) <= 256 << 20  # 1,074 MB in one
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_calls_take_the_variants_that_they_are_for(plan, call):
+    """The GPU tests' calls: which blocks they run in, how rows are loaded, how many chunks there are."""
+    c = CALLS[call]
+    for kind, code in (("fp16", 0), ("int8", 1), ("e4m3", 2), ("e2m1", 4)):
+        for dim in c["dims"]:
+            pages, width = shape_of(call, kind, dim)
+            kw = dict(type=code, batch=len(c["lens"]), pages=pages, table_width=width, table_stride=width, page_size=c["size"],
+                      kv_heads=c["kv"], head_dim=dim, head_stride=c["size"] * dim, page_stride=c["kv"] * c["size"] * dim)
+            if code:
+                kw.update(k_scale=4096, v_scale=4096)
+            cut = plan(c["kv"] * c["group"], **kw)
+            assert max(c["lens"]) <= width * c["size"]
+            assert (cut["wide"], cut["once"], cut["per_seq"] != 1) == (c["wide"], c["once"], c["cut"]), (kind, dim, cut)
+            if call == "full" and code == 4:  # three and more chunks of two sequences, by one of the ways to cut at least
+                assert len(set(cut["one_over"])) == (3 if dim == 128 else 1), cut
+            if not c["cut"]:
+                continue
+            sizes = list(chunks_by_lengths(cut, c["lens"]))
+            if call == "many_tiles":
+                assert min(longest for _, longest in sizes) > 32 * 4 * 32  # tiles of 32 positions, 4 waves, 32 at once
+            if call.startswith("many_chunks"):
+                for one_over in cut["one_over"]:
+                    size = max(cut["chunk"], -(-int(sum(c["lens"]) * one_over + 0.98) // 128) * 128)
+                    assert -(-max(c["lens"]) // size) > 64
+    if call.startswith("second_round"):
+        heads = c["kv"] * len(c["lens"])
+        assert max(c["lens"]) > 1024 * -(-4096 // heads)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_list_of_pages_takes_chunks_of_many_tiles(plan, dim):
+    cut = plan(4096, count=330, type=4, k_scale=4096, v_scale=4096, batch=1, table_width=1250, table_stride=1250, pages=1253,
+               page_size=64, kv_heads=1, head_dim=dim, head_stride=64 * dim, page_stride=64 * dim)
+    assert not cut["wide"] and cut["per_seq"] > 1 and cut["chunk"] > 32 * 4 * 32
