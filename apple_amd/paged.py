@@ -232,7 +232,7 @@ class RFSNPagedKVCache:
     def _runs(self, q_heads: int) -> List[Tuple[int, int]]:
         """Neighbouring sequences [begin, end) whose scores keep to the pool's size: a long one among short ones would
         need room for each of them as long."""
-        most = max(self.pages.k.shape[0], SCORES_AT_LEAST // (4 * self.page_size * q_heads))
+        most = max(self.pages.k.shape[0], SCORES_AT_LEAST // (4 * self.page_size * max(1, q_heads)))
         if self.batch * max(len(h) for h in self._held) <= most:
             return [(0, self.batch)]
         runs, begin, longest = [], 0, 0

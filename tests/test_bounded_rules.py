@@ -136,6 +136,13 @@ def test_scores_never_need_more_than_the_pool(monkeypatch, lens, most):
     assert len(calls) == 1
 
 
+def test_a_query_without_heads_is_left_to_the_kernels_check(monkeypatch):
+    c = quiet_cache(monkeypatch, 1, calls := [])
+    c.append(rows(5), rows(5), [5])
+    c.attention_forward(torch.zeros((1, 0, 64)))
+    assert calls[0][0].shape == (1, 0, 64)
+
+
 def test_scores_of_a_long_sequence_among_short_ones(monkeypatch):
     calls = []
     c = quiet_cache(monkeypatch, 64, calls, pages=8700, max_tokens=140000)
