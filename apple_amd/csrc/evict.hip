@@ -114,6 +114,9 @@ evict_move_kernel(const rfsn_paged p, int shift, int parts, const uint32_t* __re
 }
 
 // Bounds of the pages that hold the kept rows, from the keys as they are read back.  A wave a (page, head).
+// Bound: latency, a page's loads in turn (calls with bounds and without: 2,048 rows of 8 heads of 64, fp16, in pages of 16, 64
+// and 256 rows 20.6, 22.3 and 28.5 us, and 17.2, 16.7 and 16.7; 32 sequences to 4,096 rows of 8 heads of 128, 4 bits, in
+// pages of 32 and 256 rows 38.9 and 54.4, and 26.1 and 26.1).
 template <int D, int TYPE>
 __global__ void __launch_bounds__(64)
 evict_bounds_kernel(const rfsn_paged p, int shift, int keep) {

@@ -1,4 +1,5 @@
-// What the paged KV cache's kernels share (paged.hip, paged_attention.hip).
+// What the paged KV cache's kernels share: rows in pages, bounds and page choice (paged.hip, choose.h), attention and weights
+// (paged_attention.h, paged_weigh.hip), eviction (evict.hip).
 #pragma once
 
 #include "rfsn_common.h"

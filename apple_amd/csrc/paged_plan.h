@@ -32,12 +32,12 @@ inline int aim(int k, int units, int batch) {
 
 constexpr double kLastLevelCache = 256 * 1024 * 1024;
 // Of fp16 pages a wave drops weights below 2^-33 of the largest that it sees from its products with V, and
-// rounds others by as much (paged_attention.hip), so a chunk of four waves is off by at most 2^20 2^-33 of the
+// rounds others by as much (paged_attention.h), so a chunk of four waves is off by at most 2^20 2^-33 of the
 // largest |v|, a quarter of fp16's half step.
 constexpr int64_t kLongestChunk = 1 << 22;
 constexpr int kWideTiles = 8192;   // tiles of 32 positions of a call up to which blocks have many waves
 
-// By sizes and the sequences' capacity; paged_attention.hip cuts by the lengths within it.
+// By sizes and the sequences' capacity; find_chunk (paged_attention.h) cuts by the lengths within it.
 struct Plan {
   int64_t slots;  // of partial results
   Cut cut;
@@ -99,7 +99,8 @@ inline Plan plan(const rfsn_paged& p, int q_heads, int count) {
       for (int x = 0; x < kTries; ++x) r.cut.each[x] = each[p.head_dim == 64 ? 0 : p.head_dim == 128 ? 1 : 2][x];
     }
     // A batch that fills the chip by itself is weighed in 1, 4/3 and 5/3 chunks a sequence as well, of 4-bit rows of 128 (24
-    // ragged sequences of up to 12,001, 32 heads: 60.4 -> 55.1 us, 100 of 3,000 84 -> 81; of 64, 64 of up to 9,000: 57.7, so 60.5).
+    // ragged sequences of up to 12,001, 32 heads: 60.4 -> 55.1 us, 100 of 3,000 84 -> 81; of 64, 64 of up to 9,000: 57.7, so 60.5; of 256
+    // alike within 2 %: 24 of up to 12,001, 32 heads, 110.6, so 107.9, 17 of up to 5,000 52.4 and 52.7, 100 of 3,000 522 and 519).
     const bool full = p.batch <= 4096 && aim(first + kTries - 1, units, p.batch) == p.batch;  // (the grid ends at 65,535 chunks)
     int64_t most_chunks = 0;
     for (int x = 0; x < kTries; ++x) {

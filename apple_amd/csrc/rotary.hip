@@ -58,8 +58,8 @@ __device__ __forceinline__ void store_vec(V x, T* a) {
 // ("interleaved"; with pieces of one value the two of a pair), or a piece to copy, and goes through the block's
 // (row, head) lines, U of them in flight.  The block's rows' turns are made once, while the first lines come.
 //
-// Bound: HBM.  8,191 rows of 40 heads of 64, fp16: 84 MB in 16.1 us, 5.2 TB/s; 16,384 of 64 of 128, bf16, interleaved: 537 MB
-// in 82 us, 6.5 TB/s.  A thread a pair with divisions for its place took 32 and 269 us.
+// Bound: HBM.  8,191 rows of 40 heads of 64, fp16: 84 MB in 13.3 to 15.6 us, 5.4 to 6.3 TB/s; 16,384 of 64 of 128, bf16,
+// interleaved: 537 MB in 82 us, 6.5 TB/s.  A thread a pair with divisions for its place took 32 and 269 us.
 template <int TYPE, int LAYOUT, int PB, int U, bool kOnce>
 __global__ void __launch_bounds__(1024)
 rotary_kernel(const rfsn_rotary_params p, int per, int turning, int units, float over_heads) {
@@ -169,7 +169,7 @@ void rotary_launch(const rfsn_rotary_params& p, bool same, hipStream_t s) {
   // Results of 256 MB, the size of the last-level cache, or more are gone from it before anything reads them: rows and
   // results pass the caches by (16,384 rows of 64 heads of 128, fp16: 101 -> 83 us interleaved, 102 -> 92 in halves; 8,191
   // of 72 of 256: 115 -> 103), where a wave's pieces are whole lines of 128 bytes (halves of 64: 100 -> 103).
-  // Smaller ones stay (8,191 of 40 of 64: 16.2, so 19.6; fp32 25.3, so 28.1), as do rows turned in place (44, so 57).
+  // Smaller ones stay (8,191 of 40 of 64: interleaved 14.9, so 17.0; fp32 25.4, so 28.4), as do rows turned in place (44, so 57).
   const bool once = PB == 16 && !same && (double)p.rows * heads * p.head_dim * size >= 256.0 * 1024 * 1024 &&
                     (p.layout == RFSN_ROTARY_INTERLEAVED || p.rotary_dim / 2 * size >= 128);
 #define RFSN_ROTARY_LAUNCH(LL, ONCE)                                                                                  \

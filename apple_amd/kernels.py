@@ -923,7 +923,9 @@ def paged_attention(q: torch.Tensor, pages: KVPages, table: torch.Tensor, lens: 
     Codes are attended as code * scale in fp32, not rounded to fp16 (in which those of 4 bits are exact).
     ``weight`` [P, Hkv, S] fp32 (without ``chosen``): each position's softmax
     weight, summed over the KV head's query heads, is added to its row's; no two
-    sequences may hold one page then.
+    sequences may hold one page then, nor one sequence a page twice.  The scores take 4 bytes of
+    workspace per query head, sequence and position of the table's room: give the table the width that the call's longest
+    sequence needs, and one that is far longer than the others a call of its own.
     ``held_pages``: the pages that the sequences hold together, where the caller
     knows it; without it a call counts as reading what its table has room for,
     which costs up to a tenth where that is far more."""

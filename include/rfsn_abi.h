@@ -586,7 +586,7 @@ int rfsn_ref_table_stats(const rfsn_ref_params* p, float* stats_dev, void* strea
  * mantissa bits): scale = min(amax / 6 rounded to such a number, 10240), code =
  * x / scale rounded to nearest, ties to the even code; a group with a value that
  * is not finite has scale byte 255 (NaN) and codes 0.  code * scale is exact in
- * fp16.  bounds
+ * fp16.  The scale is none of the OCP MX formats', whose blocks of 32 have powers of two.  bounds
  * holds, per page and KV head, the smallest and the largest key of each
  * coordinate, as fp16 of the rows before they are quantised; a NaN key makes
  * both NaN.
@@ -671,7 +671,8 @@ int rfsn_page_select(const rfsn_paged* p, const void* q, int32_t q_heads, int32_
  * With p->weight each position's softmax weight, summed over the query heads of
  * the KV head, is added to its row's (nothing to attend: nothing is added; a head
  * whose weights are NaN adds NaN to all of the sequence's positions); chosen has to be NULL
- * then, and no two sequences of the call may hold one page (a table_stride of 0 is refused).
+ * then, and no two sequences of the call, nor two entries of a sequence's table, may name one page (a table_stride
+ * of 0 is refused).
  * The workspace size depends on q_heads, whether there are weights and, with chosen, count (0: dense).
  * Weights take batch * q_heads * table_width * page_size * 4 bytes of it, so a table as wide as the call's longest
  * sequence needs, and one that is far longer than the others is better attended in a call of its own. */
